@@ -778,7 +778,8 @@ def main():
     torch.cuda.set_device(local)
     dev = torch.device("cuda", local)
     import __graft_entry__
-    if rank == 0:
+    from dynamicpdb_amd import _lib
+    if rank == 0 and not os.path.exists(_lib.LIB_PATH):
         __graft_entry__.build()
     if world > 1:
         dist.barrier()
