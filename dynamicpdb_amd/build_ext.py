@@ -6,6 +6,7 @@ The .so is built IN-TREE (it is git-ignored but travels to the GPU box with the 
 """
 import hashlib
 import os
+import re
 import subprocess
 import sys
 from concurrent.futures import ThreadPoolExecutor
@@ -28,10 +29,22 @@ def sources():
     return sorted(f for f in os.listdir(CSRC) if f.endswith(".hip"))
 
 
+def _with_headers(srcs):
+    """the sources and every header they include, directly or not"""
+    seen, todo = [], list(srcs)
+    while todo:
+        f = todo.pop(0)
+        if f not in seen:
+            seen.append(f)
+            with open(os.path.join(CSRC, f)) as fh:
+                todo += re.findall(r'^\s*#include "([^"]+)"', fh.read(), flags=re.M)
+    return seen
+
+
 def _digest(srcs=None):
-    """of the flags, the headers and the sources (all of them, or `srcs`)"""
+    """of the flags, the sources (all of them, or `srcs`) and the headers they include"""
     h = hashlib.sha256()
-    for f in (sources() if srcs is None else srcs) + sorted(f for f in os.listdir(CSRC) if f.endswith(".h")) + ["../../include/dfold_hip.h"]:
+    for f in _with_headers(sources() if srcs is None else srcs):
         with open(os.path.join(CSRC, f), "rb") as fh:
             h.update(f.encode())
             h.update(fh.read())

@@ -1,0 +1,213 @@
+// Attention of one sequence over another (seq_attn_fwd.hip, seq_attn_bwd.hip): tile images, operand fragments and the bucketed
+// relative position bias that the forward and the backward kernels share.
+//
+// Everything runs on v_mfma_f32_32x32x16 (bf16 / f16 operands, fp32 accumulators).  Its accumulator holds column lane & 31 and rows
+// 8 (r / 4) + 4 (lane / 32) + r % 4, r = 0 .. 15, so a product whose COLUMNS are the softmax rows (S^T = K Q^T) leaves every lane
+// with scores of one row only: maxima and sums are a register tree and one exchange between the two lane halves, and eight
+// consecutive accumulator registers ARE a B operand of the next product once its A operand counts the reduction index in the same
+// order: slot s of half h of 16-block c <-> index 16 c + 8 (s / 4) + 4 h + s % 4.  A operands of that order come out of LDS by the
+// transpose read (4 rows x 16 columns per 16 lanes); P and dS never touch LDS.
+#pragma once
+#include "dfold_common.h"
+#include "../../include/dfold_hip.h"
+
+#define SA_LOG2E 1.44269504088896341f
+#define SA_KT 64                       // rows of an LDS tile
+#define SA_WAVES 4
+#define SA_REACH 64                    // distances a 32 x 32 block can lie beyond W and still not be uniform
+#define SA_ROWS (32 * SA_WAVES)        // softmax rows (forward, dQ) or keys (dK, dV) of a workgroup
+
+typedef __attribute__((ext_vector_type(4))) unsigned sa_u32x4;
+typedef __attribute__((ext_vector_type(4))) short sa_s16x4;
+typedef __attribute__((ext_vector_type(8))) short sa_s16x8;
+typedef __attribute__((ext_vector_type(8))) _Float16 sa_f16x8;
+typedef __attribute__((ext_vector_type(2))) _Float16 sa_f16x2;
+typedef __attribute__((address_space(3))) char sa_lchar;
+typedef __attribute__((address_space(3))) sa_s16x4 sa_ls16x4;
+
+template <int DT>
+__device__ __forceinline__ f32x16 sa_mfma(const sa_u32x4 a, const sa_u32x4 b, const f32x16 c) {
+  if constexpr (DT == DFOLD_DT_BF16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(sa_f16x8, a), __builtin_bit_cast(sa_f16x8, b), c, 0, 0, 0);
+}
+// two fp32 values rounded to nearest even in the operand type
+template <int DT>
+__device__ __forceinline__ uint32_t sa_pack2(float lo, float hi) {
+  if constexpr (DT == DFOLD_DT_BF16) return pack2bf_hw(lo, hi);
+  const dfold_f32x2 v = {lo, hi};
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(v, sa_f16x2));
+}
+template <int DT>
+__device__ __forceinline__ float sa_lo(uint32_t pair) {
+  if constexpr (DT == DFOLD_DT_BF16) return bf_lo(pair);
+  return (float)__builtin_bit_cast(sa_f16x2, pair)[0];
+}
+template <int DT>
+__device__ __forceinline__ float sa_hi(uint32_t pair) {
+  if constexpr (DT == DFOLD_DT_BF16) return bf_hi(pair);
+  return (float)__builtin_bit_cast(sa_f16x2, pair)[1];
+}
+// combine the two lane halves (lane, lane ^ 32) of a value
+__device__ __forceinline__ float sa_xmax(float v) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+__device__ __forceinline__ float sa_xsum(float v) {
+  auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+__device__ __forceinline__ float sa_exp2(float v) { return __builtin_amdgcn_exp2f(v); }
+
+// workgroup id -> work id: blockIdx round-robins over the 8 XCDs, consecutive work ids (which share K and V) stay on one of them
+__device__ __forceinline__ unsigned sa_work_id() {
+  const unsigned nwg = gridDim.x, bid = blockIdx.x;
+  const unsigned q = nwg >> 3, r = nwg & 7, xcd = bid & 7, idx = bid >> 3;
+  return (xcd < r ? xcd * (q + 1) : r * (q + 1) + (xcd - r) * q) + idx;
+}
+
+// ---- LDS tiles: SA_KT rows of DP 16-bit values, 16-byte chunks XOR-permuted within a row.  The key makes both kinds of read
+//      conflict-free: 16 consecutive rows at one chunk (operand rows) and 4 consecutive rows at 4 consecutive chunks (transpose
+//      reads; rows 0 .. 3 of a quadruple must land in different 64-byte groups of the 256-byte bank line) ----
+template <int DP>
+struct SaTile {
+  static constexpr int CPR = DP / 8;                       // chunks per row: 4, 8, 16
+  static constexpr int BYTES = SA_KT * DP * 2;
+  static constexpr int NCH = SA_KT * CPR / (64 * SA_WAVES);  // chunks per thread of a staged tile
+  static __device__ __forceinline__ int key(int row) {
+    if constexpr (CPR == 16) return ((row & 3) << 2) | ((row >> 2) & 3);
+    if constexpr (CPR == 8) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
+    return (row >> 2) & 3;
+  }
+  static __device__ __forceinline__ int off(int row, int chunk) { return row * (DP * 2) + ((chunk ^ key(row)) << 4); }
+  // operand rows: lane holds row `row`, elements 16 ks + 8 h .. + 8
+  static __device__ __forceinline__ sa_u32x4 rows(const char* t, int row, int ks, int h) {
+    return *(const sa_u32x4*)(t + off(row, 2 * ks + h));
+  }
+  // transposed operand: lane holds column 32 dt + (lane & 31), rows r0 + 4 h + 0 .. 3 and r0 + 8 + 4 h + 0 .. 3
+  static __device__ __forceinline__ sa_u32x4 cols(const char* t, int r0, int dt, int lane) {
+    const int i = lane & 15, row = r0 + 4 * (lane >> 5) + (i >> 2);
+    const int chunk = 4 * dt + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1), sub = (i & 1) * 8;
+    sa_lchar* b = (sa_lchar*)t;
+    const sa_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((sa_ls16x4*)(b + off(row, chunk) + sub));
+    const sa_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((sa_ls16x4*)(b + off(row + 8, chunk) + sub));
+    return __builtin_bit_cast(sa_u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+  }
+};
+
+// registers of a tile on its way to LDS: rows row0 .. row0 + SA_KT of a [rows][D] matrix with row stride `rs` elements.  Rows at or
+// past `end` and columns at or past D read as zeros; `live` (one bit per row) zeroes rows whose content must not be used.
+template <int DP>
+struct SaStage {
+  using T = SaTile<DP>;
+  sa_u32x4 v[T::NCH];
+  __device__ __forceinline__ void load(const char* base, long rs, int row0, int end, int D, int tid) {
+#pragma unroll
+    for (int i = 0; i < T::NCH; ++i) {
+      const int c = tid + i * 64 * SA_WAVES, row = row0 + c / T::CPR, cc = c % T::CPR;
+      v[i] = (sa_u32x4){0u, 0u, 0u, 0u};
+      if (row < end && cc * 8 < D) v[i] = *(const sa_u32x4*)(base + ((long)row * rs + cc * 8) * 2);
+    }
+  }
+  __device__ __forceinline__ void mask(unsigned long live, int tid) {
+#pragma unroll
+    for (int i = 0; i < T::NCH; ++i) {
+      const int row = (tid + i * 64 * SA_WAVES) / T::CPR;
+      if (!((live >> row) & 1)) v[i] = (sa_u32x4){0u, 0u, 0u, 0u};
+    }
+  }
+  __device__ __forceinline__ void store(char* t, int tid) const {
+#pragma unroll
+    for (int i = 0; i < T::NCH; ++i) {
+      const int c = tid + i * 64 * SA_WAVES;
+      *(sa_u32x4*)(t + T::off(c / T::CPR, c % T::CPR)) = v[i];
+    }
+  }
+};
+
+// ---- bucketed relative position bias ----
+struct SaRel {
+  const float* table;      // [num_buckets][H]
+  const int32_t* q_offsets;  // [B] or null: position of query 0 minus position of key 0
+  int q_offset, H, half, exact, nfar, W, both;   // W: every |distance| >= W is in the last bucket of its side
+  int16_t far[DFOLD_REL_FAR];                    // far[k]: first distance of bucket exact + 1 + k
+};
+// first distance of one-sided bucket j
+__device__ __forceinline__ int sa_bucket_lo(const SaRel& r, int j) { return j <= r.exact ? j : r.far[j - r.exact - 1]; }
+__device__ __forceinline__ int sa_bucket(const SaRel& r, int delta) {
+  const int n = r.both ? abs(delta) : max(-delta, 0);
+  const int base = r.both && delta > 0 ? r.half : 0;
+  if (n < r.exact) return base + n;
+  int lo = 0, hi = r.nfar;              // number of borders <= n
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (r.far[mid] <= n) lo = mid + 1; else hi = mid;
+  }
+  return base + r.exact + lo;
+}
+// bias x log2(e).  A finite entry stays finite: entries near the type's lowest value act as a mask that still orders (a row of
+// nothing but such entries is an ordinary softmax), only a true -inf removes a key.
+__device__ __forceinline__ float sa_bias_log2(float b) {
+  const float v = b * SA_LOG2E;
+  return __builtin_isfinite(b) ? fminf(fmaxf(v, -3.3e38f), 3.3e38f) : v;
+}
+// position of query 0 of batch item b; far beyond every sequence it only saturates (no 32-bit wrap in key - query)
+__device__ __forceinline__ int sa_q_offset(const SaRel& r, int b) {
+  return min(max(r.q_offsets ? r.q_offsets[b] : r.q_offset, -(1 << 29)), 1 << 29);
+}
+// LDS rows of 2 W + 1 values per head: entry W + delta, delta = key position - query position in [-W, W]
+__device__ __forceinline__ void sa_fill_bias(float* lds, const SaRel& r, int head0, int nheads, int tid) {
+  const int n = 2 * r.W + 1;
+  for (int i = tid; i < n * nheads; i += 64 * SA_WAVES) {
+    const int h = i / n, d = i - h * n - r.W;
+    lds[i] = sa_bias_log2(r.table[(long)sa_bucket(r, d) * r.H + head0 + h]);
+  }
+}
+
+// one wave's share of a workgroup: the histogram over distances (hist[reach + delta], |delta| <= reach) summed into buckets j = w,
+// w + waves, ...; out[j].  A bucket is a run of distances on one side.
+__device__ __forceinline__ void sa_bucket_sums(const SaRel& r, const float* hist, int reach, int num_buckets, float* out, int w, int lane) {
+  for (int j = w; j < num_buckets; j += SA_WAVES) {
+    const bool pos = r.both && j >= r.half;
+    const int jj = pos ? j - r.half : j;
+    const int nlo = max(sa_bucket_lo(r, jj), pos ? 1 : 0);
+    const int nhi = jj == r.half - 1 ? reach : min(sa_bucket_lo(r, jj + 1) - 1, reach);
+    float a = 0.f;
+    for (int n = nlo + lane; n <= nhi; n += 64) a += hist[reach + (pos ? n : -n)];
+    if (!r.both && jj == 0)              // keys behind the query all count as distance 0
+      for (int n = 1 + lane; n <= reach; n += 64) a += hist[reach + n];
+    a = wave_sum(a);
+    if (lane == 0) out[j] = a;
+  }
+}
+// host side: validates the bias part of a descriptor and fills SaRel; false: rejected
+static inline bool sa_make_rel(const dfold_rel_bias* d, int H, SaRel* r) {
+  if (!d->table || d->num_buckets < 2 || d->num_buckets > 2 * DFOLD_REL_FAR) return false;
+  const bool both = d->bidirectional != 0;
+  if (both && (d->num_buckets & 1)) return false;
+  const int half = both ? d->num_buckets / 2 : d->num_buckets, exact = half / 2, nfar = half - exact - 1;
+  if (exact < 1 || nfar < 0 || nfar > DFOLD_REL_FAR) return false;
+  r->table = d->table; r->q_offsets = d->q_offsets; r->q_offset = d->q_offset;
+  r->H = H; r->half = half; r->exact = exact; r->nfar = nfar; r->both = both;
+  int prev = exact;
+  for (int i = 0; i < nfar; ++i) {
+    if (d->far_border[i] < prev || d->far_border[i] > DFOLD_REL_MAX_DISTANCE) return false;
+    r->far[i] = (int16_t)(prev = d->far_border[i]);
+  }
+  r->W = nfar ? prev : exact;
+  return true;
+}
+
+// what both directions require of the forward descriptor (an empty key axis is allowed: k, v may then be null)
+static inline bool sa_desc_ok(const dfold_seq_attn_desc* d) {
+  if (!d || !d->q || !d->o || (d->Lk > 0 && (!d->k || !d->v))) return false;
+  if (d->dtype != DFOLD_DT_BF16 && d->dtype != DFOLD_DT_F16) return false;
+  if (d->B <= 0 || d->Lq <= 0 || d->Lk < 0 || d->H <= 0 || d->Hkv <= 0 || d->H % d->Hkv) return false;
+  if (d->D <= 0 || d->D > 128 || d->D % 8 || d->Lq > (1 << 30) || d->Lk > (1 << 30)) return false;
+  if (((uintptr_t)d->q | (uintptr_t)d->k | (uintptr_t)d->v | (uintptr_t)d->o | (uintptr_t)d->ws) & 15) return false;
+  const int64_t st[12] = {d->q_sb, d->q_sl, d->q_sh, d->k_sb, d->k_sl, d->k_sh, d->v_sb, d->v_sl, d->v_sh, d->o_sb, d->o_sl, d->o_sh};
+  for (int i = 0; i < 12; ++i)
+    if (st[i] % 8 || st[i] < 0) return false;
+  return d->mask_sb >= 0;
+}

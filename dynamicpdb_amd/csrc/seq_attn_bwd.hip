@@ -1,0 +1,505 @@
+// Attention of one sequence over another, backward.  With P = softmax row from the forward's log-sum, dP = dO V^T and
+// delta = rowsum(dO O) = rowsum(P dP):   dS = P (dP - delta),  dV = P^T dO,  dK = scale dS^T Q,  dQ = scale dS K,
+// dtable[bucket] = sum of dS over the bucket's diagonals.
+//
+// Two passes, each recomputing S and dP (7 products instead of 5) rather than adding to one of the gradients with atomics: results do
+// not depend on the order of workgroups.
+//   * dQ pass: the forward's walk (128 rows, key tiles of 64).  S^T and dP^T have the softmax rows as columns, so the row's log-sum
+//     and delta are one register each, and dS^T is at once the B operand of dQ^T = K^T dS^T.  delta = dO O comes from the lane's own
+//     operand of dO and the stored O, whose two roundings (P's and its own) it inherits; exact arithmetic makes a row of dS sum to
+//     zero, so the row sum that is left, taken in fp32, is what delta lacks: delta + that sum goes to the second pass.
+//   * dK, dV pass: 128 keys per workgroup, K^T and V^T operands in registers, query tiles of 64 of all heads of the group in LDS:
+//     the sum over shared heads is the accumulator's.  The bias gradient (an fp32 result) is formed here, from fp32 dS with the
+//     corrected delta.
+// Bias gradient: 32 x 32 blocks beyond the last border add to one register per side; nearer blocks add dS to a histogram over the
+// distance in LDS, one per wave and lane half.  Within one instruction the 32 lanes of a half hit 32 different distances, and a
+// wave's LDS operations stay in order: no order of additions is left open.
+#include "seq_attn.h"
+#include "seq_dtable.h"
+#include <math.h>
+
+struct SaBwdParams {
+  const char *q, *k, *v, *o, *d_o;
+  char *dq, *dk, *dv;
+  const float* lse;
+  float *delta, *ws_q, *ws_k, *ws_t, *dtable;
+  const uint8_t* key_mask;
+  const int32_t* kv_lens;
+  long q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh, o_sb, o_sl, o_sh, do_sb, do_sl, do_sh, mask_sb;
+  int B, Lq, Lk, H, Hkv, D, splits_q, splits_k, nrb, num_buckets;
+  float scale, sl2;
+  SaRel rel;
+};
+
+// logits x log2 e of a block held with columns `c` and rows 8 (r / 4) + 4 h + r % 4; sgn = +1: rows are keys, -1: rows are queries
+template <bool REL>
+__device__ __forceinline__ void sa_logits(f32x16& s, float sl2, const float* myb, int W, int far, float farv, int d0, int sgn) {
+  if constexpr (REL) {
+    if (far) {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], sl2, farv);
+    } else {
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        const int d = d0 + sgn * (8 * (r >> 2) + (r & 3));
+        s[r] = __builtin_fmaf(s[r], sl2, myb[min(max(d, -W), W)]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] *= sl2;
+  }
+}
+
+template <int DT, int DP, bool REL>
+__global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_dq_kernel(const SaBwdParams p) {
+  using T = SaTile<DP>;
+  constexpr int KS = DP / 16, NT = DP / 32;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  float* const ldsB = (float*)(smem + 4 * T::BYTES);
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l31 = lane & 31, h = lane >> 5;
+  unsigned id = sa_work_id();
+  const int rb = id % p.nrb; id /= p.nrb;
+  const int sp = id % p.splits_q; id /= p.splits_q;
+  const int head = id % p.H, b = id / p.H, hkv = head / (p.H / p.Hkv);
+  const int row_w = rb * SA_ROWS + w * 32, row = row_w + l31;
+  const bool wave_on = row_w < p.Lq, on = row < p.Lq;
+  const int qi = min(row, p.Lq - 1);
+
+  int kv_end = p.Lk;
+  if (p.kv_lens) kv_end = min(max(p.kv_lens[b], 0), p.Lk);
+  const int nt = (kv_end + SA_KT - 1) / SA_KT, per = (nt + p.splits_q - 1) / p.splits_q;
+  const int t0 = sp * per, t1 = min(nt, t0 + per);
+
+  int qpos = 0, qlo = 0, qhi = 0;
+  float bL = 0.f, bR = 0.f;
+  const float* myb = ldsB + p.rel.W;
+  if constexpr (REL) {
+    sa_fill_bias(ldsB, p.rel, head, 1, tid);
+    const int off = sa_q_offset(p.rel, b);
+    qpos = qi + off;
+    qlo = row_w + off;
+    qhi = min(row_w + 31, p.Lq - 1) + off;
+    __syncthreads();
+    bL = myb[-p.rel.W];
+    bR = myb[p.rel.W];
+  }
+
+  sa_u32x4 qf[KS], of[KS];
+  float dl = 0.f;
+  {
+    const char* sq = p.q + ((long)b * p.q_sb + (long)qi * p.q_sl + (long)head * p.q_sh) * 2;
+    const char* sg = p.d_o + ((long)b * p.do_sb + (long)qi * p.do_sl + (long)head * p.do_sh) * 2;
+    const char* so = p.o + ((long)b * p.o_sb + (long)qi * p.o_sl + (long)head * p.o_sh) * 2;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int d = ks * 16 + h * 8;
+      qf[ks] = of[ks] = (sa_u32x4){0u, 0u, 0u, 0u};
+      if (d < p.D) {
+        qf[ks] = *(const sa_u32x4*)(sq + d * 2);
+        of[ks] = *(const sa_u32x4*)(sg + d * 2);
+        const sa_u32x4 o = *(const sa_u32x4*)(so + d * 2);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          dl = __builtin_fmaf(sa_lo<DT>(of[ks][e]), sa_lo<DT>(o[e]), dl);
+          dl = __builtin_fmaf(sa_hi<DT>(of[ks][e]), sa_hi<DT>(o[e]), dl);
+        }
+      }
+    }
+  }
+  dl = sa_xsum(dl);
+  const long rowi = ((long)b * p.H + head) * p.Lq + qi;
+  const float lse = on ? p.lse[rowi] : INFINITY;
+
+  const char* const kb_ = p.k + ((long)b * p.k_sb + (long)hkv * p.k_sh) * 2;
+  const char* const vb_ = p.v + ((long)b * p.v_sb + (long)hkv * p.v_sh) * 2;
+  const uint8_t* const mb_ = p.key_mask ? p.key_mask + (long)b * p.mask_sb : nullptr;
+  f32x16 dq[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dq[i][r] = 0.f;
+
+  float left = 0.f;          // row sum of dS
+  SaStage<DP> sk, sv;
+  int kmask = 0;
+  auto fetch = [&](int t) {
+    sk.load(kb_, p.k_sl, t * SA_KT, kv_end, p.D, tid);
+    sv.load(vb_, p.v_sl, t * SA_KT, kv_end, p.D, tid);
+    const int key = t * SA_KT + lane;
+    kmask = key < kv_end ? (mb_ ? mb_[key] : 1) : 0;
+  };
+  if (t0 < t1) fetch(t0);
+  for (int t = t0; t < t1; ++t) {
+    char* const lk = smem + (t & 1) * 2 * T::BYTES;
+    char* const lv = lk + T::BYTES;
+    const unsigned long live = __ballot(kmask != 0);
+    if (mb_ && live != ~0ul) {
+      sk.mask(live, tid);
+      sv.mask(live, tid);
+    }
+    sk.store(lk, tid);
+    sv.store(lv, tid);
+    __syncthreads();
+    if (t + 1 < t1) fetch(t + 1);
+    if (live == 0 || !wave_on) continue;
+#pragma unroll
+    for (int kb = 0; kb < 2; ++kb) {
+      f32x16 s, dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        s = sa_mfma<DT>(T::rows(lk, kb * 32 + l31, ks, h), qf[ks], s);
+        dp = sa_mfma<DT>(T::rows(lv, kb * 32 + l31, ks, h), of[ks], dp);
+      }
+      const int k0 = t * SA_KT + kb * 32;
+      const int far = !REL ? 0 : k0 - qhi >= p.rel.W ? 1 : k0 + 31 - qlo <= -p.rel.W ? -1 : 0;
+      const int d0 = k0 + 4 * h - qpos;
+      sa_logits<REL>(s, p.sl2, myb, p.rel.W, far, far > 0 ? bR : bL, d0, 1);
+      if (live != ~0ul) {
+        const unsigned bits = (unsigned)(live >> (kb * 32)) >> (4 * h);
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+          if (!((bits >> (8 * (r >> 2) + (r & 3))) & 1)) s[r] = -INFINITY;
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[r] = sa_exp2(s[r] - lse) * (dp[r] - dl);
+        left += s[r];
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        sa_u32x4 df;      // dS in the operand type: relative error 2^-9 (bf16) / 2^-12 (f16) of each term of dQ's sum
+#pragma unroll
+        for (int e = 0; e < 4; ++e) df[e] = sa_pack2<DT>(s[8 * c + 2 * e], s[8 * c + 2 * e + 1]);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) dq[i] = sa_mfma<DT>(T::cols(lk, kb * 32 + c * 16, i, lane), df, dq[i]);
+      }
+    }
+  }
+
+  left = sa_xsum(left);
+  if (on && h == 0) {
+    // parts of the key axis: plane 0 holds delta, plane 1 + part the part's row sum (seq_attn_delta_kernel adds them up)
+    if (p.splits_q == 1) p.delta[rowi] = dl + left;
+    else {
+      if (sp == 0) p.delta[rowi] = dl;
+      p.delta[(long)(1 + sp) * p.B * p.H * p.Lq + rowi] = left;
+    }
+  }
+  if (on) {
+    const long r1 = ((long)b * p.Lq + qi) * p.H + head;
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int d = i * 32 + g * 8 + h * 4;
+        if (d >= p.D) continue;
+        float o[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o[e] = dq[i][g * 4 + e] * p.scale;
+        if (p.splits_q == 1)
+          *(uint2*)(p.dq + (r1 * p.D + d) * 2) = (uint2){sa_pack2<DT>(o[0], o[1]), sa_pack2<DT>(o[2], o[3])};
+        else
+          *(f32x4*)(p.ws_q + ((long)sp * p.B * p.Lq * p.H + r1) * p.D + d) = (f32x4){o[0], o[1], o[2], o[3]};
+      }
+  }
+}
+
+template <int DT, int DP, bool REL>
+__global__ __launch_bounds__(64 * SA_WAVES, DP == 128 ? 1 : 2) void seq_attn_dkv_kernel(const SaBwdParams p) {
+  using T = SaTile<DP>;
+  constexpr int KS = DP / 16, NT = DP / 32;
+  extern __shared__ __attribute__((aligned(16))) char smem[];
+  float* const ldsL = (float*)(smem + 4 * T::BYTES);            // [stage][log-sum | delta][SA_KT]
+  float* const ldsB = ldsL + 4 * SA_KT;
+  float* const ldsH = ldsB + (REL ? 2 * p.rel.W + 1 : 0);       // [wave][lane half][distance]
+  const int hn = REL ? 2 * (p.rel.W + SA_REACH) + 1 : 0;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l31 = lane & 31, h = lane >> 5;
+  unsigned id = sa_work_id();
+  const int nkb = (p.Lk + SA_ROWS - 1) / SA_ROWS, G = p.H / p.Hkv;
+  const int kbk = id % nkb; id /= nkb;
+  const int sp = id % p.splits_k; id /= p.splits_k;
+  const int hkv = id % p.Hkv, b = id / p.Hkv;
+  const int key_w = kbk * SA_ROWS + w * 32, key = key_w + l31;
+
+  int kv_end = p.Lk;
+  if (p.kv_lens) kv_end = min(max(p.kv_lens[b], 0), p.Lk);
+  const bool wg_on = kbk * SA_ROWS < kv_end, wave_on = key_w < kv_end;
+  bool key_on = key < kv_end;
+  if (key_on && p.key_mask) key_on = p.key_mask[(long)b * p.mask_sb + key] != 0;
+
+  // units of work: (head of the group, query tile), this part's share
+  const int nqt = (p.Lq + SA_KT - 1) / SA_KT, nu = G * nqt, per = (nu + p.splits_k - 1) / p.splits_k;
+  const int u0 = sp * per, u1 = wg_on ? min(nu, u0 + per) : 0;
+
+  sa_u32x4 kf[KS], vf[KS];
+  {
+    const char* sk = p.k + ((long)b * p.k_sb + (long)key * p.k_sl + (long)hkv * p.k_sh) * 2;
+    const char* sv = p.v + ((long)b * p.v_sb + (long)key * p.v_sl + (long)hkv * p.v_sh) * 2;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+      const int d = ks * 16 + h * 8;
+      kf[ks] = vf[ks] = (sa_u32x4){0u, 0u, 0u, 0u};
+      if (key_on && d < p.D) {
+        kf[ks] = *(const sa_u32x4*)(sk + d * 2);
+        vf[ks] = *(const sa_u32x4*)(sv + d * 2);
+      }
+    }
+  }
+  f32x16 dk[NT], dv[NT];
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dk[i][r] = dv[i][r] = 0.f;
+
+  int off = 0, head_in = -1;
+  const float* myb = ldsB + p.rel.W;
+  float* const myh = ldsH + (w * 2 + h) * hn + p.rel.W + SA_REACH;
+  float accL = 0.f, accR = 0.f;
+  auto table_part = [&](int head) { return p.ws_t + ((((long)b * p.H + head) * p.splits_k + sp) * nkb + kbk) * p.num_buckets; };
+  // a head's histogram over distances -> its buckets; the far sums belong to the last bucket of their side
+  auto flush = [&](int head) {
+    accL = wave_sum(accL);
+    accR = wave_sum(accR);
+    if (lane == 0) {           // (half 0's histogram: entries -W and W carry their buckets)
+      myh[-p.rel.W] += accL;
+      myh[p.rel.W] += accR;
+    }
+    accL = accR = 0.f;
+    __syncthreads();
+    for (int i = tid; i < hn; i += 64 * SA_WAVES) {
+      float a = 0.f;
+#pragma unroll
+      for (int c = 0; c < 2 * SA_WAVES; ++c) a += ldsH[c * hn + i];
+      ldsH[i] = a;             // (entry i of every copy is this thread's)
+    }
+    __syncthreads();
+    sa_bucket_sums(p.rel, ldsH, p.rel.W + SA_REACH, p.num_buckets, table_part(head), w, lane);
+    __syncthreads();
+  };
+  if constexpr (REL) {
+    off = sa_q_offset(p.rel, b);
+    for (int g = 0; g < G; ++g)          // heads this part does not touch
+      if (max(u0, g * nqt) >= min(u1, (g + 1) * nqt))
+        for (int j = tid; j < p.num_buckets; j += 64 * SA_WAVES) table_part(hkv * G + g)[j] = 0.f;
+  }
+
+  SaStage<DP> sq, sg;
+  float lse_r = 0.f, del_r = 0.f;
+  auto fetch = [&](int u) {
+    const int head = hkv * G + u / nqt, q0 = (u % nqt) * SA_KT;
+    sq.load(p.q + ((long)b * p.q_sb + (long)head * p.q_sh) * 2, p.q_sl, q0, p.Lq, p.D, tid);
+    sg.load(p.d_o + ((long)b * p.do_sb + (long)head * p.do_sh) * 2, p.do_sl, q0, p.Lq, p.D, tid);
+    if (tid < SA_KT) {
+      const int qi = q0 + tid;
+      const long r = ((long)b * p.H + head) * p.Lq + qi;
+      lse_r = qi < p.Lq ? p.lse[r] : INFINITY;       // rows past the end: P = 0
+      del_r = qi < p.Lq ? p.delta[r] : 0.f;
+    }
+  };
+  if (u0 < u1) fetch(u0);
+  for (int u = u0; u < u1; ++u) {
+    char* const lq = smem + (u & 1) * 2 * T::BYTES;
+    char* const lg = lq + T::BYTES;
+    float* const ll = ldsL + (u & 1) * 2 * SA_KT;
+    if constexpr (REL) {
+      const int head = hkv * G + u / nqt;
+      if (head != head_in) {       // (uniform)
+        if (head_in >= 0) flush(head_in);      // (ends in a barrier: nobody reads the previous head's rows any more)
+        for (int i = tid; i < 2 * SA_WAVES * hn; i += 64 * SA_WAVES) ldsH[i] = 0.f;
+        sa_fill_bias(ldsB, p.rel, head, 1, tid);
+        head_in = head;
+      }
+    }
+    sq.store(lq, tid);
+    sg.store(lg, tid);
+    if (tid < SA_KT) {
+      ll[tid] = lse_r;
+      ll[SA_KT + tid] = del_r;
+    }
+    __syncthreads();
+    if (u + 1 < u1) fetch(u + 1);
+    if (!wave_on) continue;
+    const int q0 = (u % nqt) * SA_KT;
+#pragma unroll
+    for (int qb = 0; qb < 2; ++qb) {
+      if (q0 + qb * 32 >= p.Lq) continue;
+      f32x16 s, dp;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks) {
+        s = sa_mfma<DT>(T::rows(lq, qb * 32 + l31, ks, h), kf[ks], s);
+        dp = sa_mfma<DT>(T::rows(lg, qb * 32 + l31, ks, h), vf[ks], dp);
+      }
+      const int qlo = q0 + qb * 32 + off, qhi = qlo + 31;
+      const int far = !REL ? 0 : key_w - qhi >= p.rel.W ? 1 : key_w + 31 - qlo <= -p.rel.W ? -1 : 0;
+      const float farv = REL ? myb[far > 0 ? p.rel.W : -p.rel.W] : 0.f;
+      sa_logits<REL>(s, p.sl2, myb, p.rel.W, far, farv, key - qlo - 4 * h, -1);
+      f32x4 rl[4], rd[4];
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        rl[g] = *(const f32x4*)(ll + qb * 32 + g * 8 + h * 4);
+        rd[g] = *(const f32x4*)(ll + SA_KT + qb * 32 + g * 8 + h * 4);
+      }
+#pragma unroll
+      for (int r = 0; r < 16; ++r) {
+        s[r] = key_on ? sa_exp2(s[r] - rl[r >> 2][r & 3]) : 0.f;
+        dp[r] = s[r] * (dp[r] - rd[r >> 2][r & 3]);
+      }
+      if constexpr (REL) {
+        if (far) {
+          float a = 0.f;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) a += dp[r];
+          if (far > 0) accR += a; else accL += a;
+        } else {
+          const int d0 = key - qlo - 4 * h;
+#pragma unroll
+          for (int r = 0; r < 16; ++r)
+            __hip_atomic_fetch_add(myh + d0 - 8 * (r >> 2) - (r & 3), dp[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        sa_u32x4 pf, df;      // P and dS in the operand type: relative error 2^-9 (bf16) / 2^-12 (f16) of each term
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          pf[e] = sa_pack2<DT>(s[8 * c + 2 * e], s[8 * c + 2 * e + 1]);
+          df[e] = sa_pack2<DT>(dp[8 * c + 2 * e], dp[8 * c + 2 * e + 1]);
+        }
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          dv[i] = sa_mfma<DT>(T::cols(lg, qb * 32 + c * 16, i, lane), pf, dv[i]);
+          dk[i] = sa_mfma<DT>(T::cols(lq, qb * 32 + c * 16, i, lane), df, dk[i]);
+        }
+      }
+    }
+  }
+
+  if constexpr (REL)
+    if (head_in >= 0) flush(head_in);
+  if (key >= p.Lk) return;
+  const long r1 = ((long)b * p.Lk + key) * p.Hkv + hkv, n = (long)p.B * p.Lk * p.Hkv;
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      const int d = i * 32 + g * 8 + h * 4;
+      if (d >= p.D) continue;
+      f32x4 a, c;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        a[e] = dk[i][g * 4 + e] * p.scale;
+        c[e] = dv[i][g * 4 + e];
+      }
+      if (p.splits_k == 1) {
+        *(uint2*)(p.dk + (r1 * p.D + d) * 2) = (uint2){sa_pack2<DT>(a[0], a[1]), sa_pack2<DT>(a[2], a[3])};
+        *(uint2*)(p.dv + (r1 * p.D + d) * 2) = (uint2){sa_pack2<DT>(c[0], c[1]), sa_pack2<DT>(c[2], c[3])};
+      } else {
+        *(f32x4*)(p.ws_k + ((long)(2 * sp) * n + r1) * p.D + d) = a;
+        *(f32x4*)(p.ws_k + ((long)(2 * sp + 1) * n + r1) * p.D + d) = c;
+      }
+    }
+}
+
+// out[i] = sum of the parts in order, 8 elements per thread; part s at ws + s * stride
+template <int DT>
+__global__ __launch_bounds__(256) void seq_attn_sum_kernel(const float* __restrict__ ws, long stride, int parts, char* __restrict__ out, long n8) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n8) return;
+  f32x4 a = (f32x4){0.f, 0.f, 0.f, 0.f}, b = a;
+  for (int s = 0; s < parts; ++s) {
+    a += *(const f32x4*)(ws + s * stride + i * 8);
+    b += *(const f32x4*)(ws + s * stride + i * 8 + 4);
+  }
+  *(sa_u32x4*)(out + i * 16) = (sa_u32x4){sa_pack2<DT>(a[0], a[1]), sa_pack2<DT>(a[2], a[3]), sa_pack2<DT>(b[0], b[1]), sa_pack2<DT>(b[2], b[3])};
+}
+
+// delta + the parts' row sums, in order
+__global__ __launch_bounds__(256) void seq_attn_delta_kernel(float* __restrict__ delta, int parts, long n) {
+  const long i = (long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  float a = delta[n + i];
+  for (int s = 2; s <= parts; ++s) a += delta[s * n + i];
+  delta[i] += a;
+}
+
+template <typename K>
+static int sa_launch_bwd(K kernel, const SaBwdParams& p, long nwg, int lds, hipStream_t st) {
+  if (lds > 65536 && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
+    return DFOLD_ELAUNCH;
+  DFOLD_LAUNCH(kernel, dim3((unsigned)nwg), dim3(64 * SA_WAVES), lds, st, p);
+  return dfold_check_launch();
+}
+template <int DT, int DP, bool REL>
+static int sa_bwd_dp(const SaBwdParams& p, hipStream_t st) {
+  const int bias = REL ? (2 * p.rel.W + 1) * 4 : 0, hist = REL ? 2 * SA_WAVES * (2 * (p.rel.W + SA_REACH) + 1) * 4 : 0;
+  int rc = sa_launch_bwd(seq_attn_dq_kernel<DT, DP, REL>, p, (long)p.nrb * p.splits_q * p.H * p.B, 4 * SaTile<DP>::BYTES + bias, st);
+  if (rc != DFOLD_OK) return rc;
+  if (p.splits_q > 1) {
+    const long n8 = (long)p.B * p.Lq * p.H * p.D / 8;
+    DFOLD_LAUNCH(seq_attn_sum_kernel<DT>, dim3((unsigned)((n8 + 255) / 256)), dim3(256), 0, st, (const float*)p.ws_q, n8 * 8, p.splits_q, p.dq, n8);
+    if ((rc = dfold_check_launch()) != DFOLD_OK) return rc;
+    const long nd = (long)p.B * p.H * p.Lq;
+    DFOLD_LAUNCH(seq_attn_delta_kernel, dim3((unsigned)((nd + 255) / 256)), dim3(256), 0, st, p.delta, p.splits_q, nd);
+    if ((rc = dfold_check_launch()) != DFOLD_OK) return rc;
+  }
+  const long nkb = (p.Lk + SA_ROWS - 1) / SA_ROWS;
+  rc = sa_launch_bwd(seq_attn_dkv_kernel<DT, DP, REL>, p, nkb * p.splits_k * p.Hkv * p.B, 4 * SaTile<DP>::BYTES + 4 * SA_KT * 4 + bias + hist, st);
+  if (rc != DFOLD_OK) return rc;
+  if (REL) {
+    DFOLD_LAUNCH(seq_dtable_kernel, dim3(p.H, (p.num_buckets + 63) / 64), dim3(1024), 0, st, (const float*)p.ws_t, p.dtable, p.num_buckets,
+                 p.B, p.H, (int)nkb * p.splits_k);
+    if ((rc = dfold_check_launch()) != DFOLD_OK) return rc;
+  }
+  if (p.splits_k == 1) return DFOLD_OK;
+  const long n = (long)p.B * p.Lk * p.Hkv * p.D, n8 = n / 8;
+  for (int i = 0; i < 2; ++i) {
+    DFOLD_LAUNCH(seq_attn_sum_kernel<DT>, dim3((unsigned)((n8 + 255) / 256)), dim3(256), 0, st, (const float*)(p.ws_k + i * n), 2 * n, p.splits_k,
+                 i ? p.dv : p.dk, n8);
+    if ((rc = dfold_check_launch()) != DFOLD_OK) return rc;
+  }
+  return DFOLD_OK;
+}
+template <int DT>
+static int sa_bwd(const SaBwdParams& p, bool rel, hipStream_t st) {
+  if (p.D <= 32) return rel ? sa_bwd_dp<DT, 32, true>(p, st) : sa_bwd_dp<DT, 32, false>(p, st);
+  if (p.D <= 64) return rel ? sa_bwd_dp<DT, 64, true>(p, st) : sa_bwd_dp<DT, 64, false>(p, st);
+  return rel ? sa_bwd_dp<DT, 128, true>(p, st) : sa_bwd_dp<DT, 128, false>(p, st);
+}
+
+extern "C" int dfold_seq_attn_bwd(const dfold_seq_attn_desc* d, const dfold_seq_attn_grad* g, void* stream) {
+  SaBwdParams p;
+  if (!sa_desc_ok(d) || d->Lk == 0 || !g || !d->lse || !g->d_o || !g->dq || !g->delta || !g->dk || !g->dv) return DFOLD_EINVAL;
+  if (g->splits_q < 1 || g->splits_q > 4096 || g->splits_k < 1 || g->splits_k > 4096) return DFOLD_EINVAL;
+  if (((uintptr_t)g->d_o | (uintptr_t)g->dq | (uintptr_t)g->dk | (uintptr_t)g->dv | (uintptr_t)g->ws) & 15) return DFOLD_EINVAL;
+  if ((g->do_sb | g->do_sl | g->do_sh) % 8 || g->do_sb < 0 || g->do_sl < 0 || g->do_sh < 0) return DFOLD_EINVAL;
+  const bool rel = d->rel.table != nullptr;
+  if (rel && (!g->dtable || !sa_make_rel(&d->rel, d->H, &p.rel))) return DFOLD_EINVAL;
+  if ((rel || g->splits_q > 1 || g->splits_k > 1) && !g->ws) return DFOLD_EINVAL;
+  if (!rel) p.rel.W = 0;
+  p.q = (const char*)d->q; p.k = (const char*)d->k; p.v = (const char*)d->v; p.o = (const char*)d->o;
+  p.d_o = (const char*)g->d_o; p.dq = (char*)g->dq; p.dk = (char*)g->dk; p.dv = (char*)g->dv;
+  p.lse = d->lse; p.delta = g->delta; p.dtable = g->dtable; p.key_mask = d->key_mask; p.kv_lens = d->kv_lens;
+  p.q_sb = d->q_sb; p.q_sl = d->q_sl; p.q_sh = d->q_sh; p.k_sb = d->k_sb; p.k_sl = d->k_sl; p.k_sh = d->k_sh;
+  p.v_sb = d->v_sb; p.v_sl = d->v_sl; p.v_sh = d->v_sh; p.o_sb = d->o_sb; p.o_sl = d->o_sl; p.o_sh = d->o_sh;
+  p.do_sb = g->do_sb; p.do_sl = g->do_sl; p.do_sh = g->do_sh; p.mask_sb = d->mask_sb;
+  p.B = d->B; p.Lq = d->Lq; p.Lk = d->Lk; p.H = d->H; p.Hkv = d->Hkv; p.D = d->D;
+  p.splits_q = g->splits_q; p.splits_k = g->splits_k; p.num_buckets = rel ? d->rel.num_buckets : 0;
+  p.scale = d->scale; p.sl2 = d->scale * SA_LOG2E;
+  p.nrb = (d->Lq + SA_ROWS - 1) / SA_ROWS;
+  const long nq = (long)d->B * d->Lq * d->H * d->D, nk = (long)d->B * d->Lk * d->Hkv * d->D, lim = 0x7fffffffL;
+  if ((long)p.nrb * p.splits_q * p.H * p.B > lim || (((long)d->Lk + SA_ROWS - 1) / SA_ROWS) * p.splits_k * p.Hkv * p.B > lim ||
+      nq / 2048 > lim - 1 || nk / 2048 > lim - 1 || d->H > 0x7fffffff / 64)
+    return DFOLD_EINVAL;
+  auto up4 = [](long x) { return (x + 3) & ~3L; };
+  p.ws_q = g->ws;
+  p.ws_k = g->ws + (p.splits_q > 1 ? up4(p.splits_q * nq) : 0);
+  p.ws_t = p.ws_k + (p.splits_k > 1 ? up4(2 * p.splits_k * nk) : 0);
+  return d->dtype == DFOLD_DT_BF16 ? sa_bwd<DFOLD_DT_BF16>(p, rel, (hipStream_t)stream) : sa_bwd<DFOLD_DT_F16>(p, rel, (hipStream_t)stream);
+}

@@ -601,6 +601,100 @@ int dfold_adam_amsgrad(const dfold_adam_tensor* table, const int32_t* chunk_star
                        double lr, double beta1, double beta2, double eps, int64_t step, void* stream);
 int dfold_adam_chunk(void);
 
+/* ----------------------------------------------------------------------------------------------
+ * Sequence-track operators: attention of one sequence over another, bucketed relative position bias, norm + rotation of query /
+ * key heads.  (No counterpart in the reference's own model: its sequence tracks meet only through IPA and the pair tensor.)
+ *
+ * Element types of q / k / v and of the bias matrix.
+ * ---------------------------------------------------------------------------------------------- */
+#define DFOLD_DT_BF16 0
+#define DFOLD_DT_F16 1
+#define DFOLD_DT_F32 2
+
+/* Learned relative position bias: logits of (query i, key j) get table[bucket(j - i - offset)][head].
+ * half = num_buckets / 2 (bidirectional: even; distances > 0 use the second half) or num_buckets (distances > 0 count as 0);
+ * exact = half / 2 >= 1; distance n < exact is bucket n, n >= exact is bucket exact + (number of far borders <= n), the
+ * half - exact - 1 borders non-decreasing in [exact, DFOLD_REL_MAX_DISTANCE].  The borders travel by value. */
+#define DFOLD_REL_FAR 256
+#define DFOLD_REL_MAX_DISTANCE 1024
+typedef struct {
+  const float* table;        /* [num_buckets][H]; NULL: no bias */
+  const int32_t* q_offsets;  /* [B] or NULL: per batch item, instead of q_offset (ignored by dfold_relpos_*) */
+  int32_t q_offset;          /* position of query 0 minus position of key 0 */
+  int32_t num_buckets, bidirectional;
+  int32_t reserved;
+  int16_t far_border[DFOLD_REL_FAR];
+} dfold_rel_bias;
+
+/* out [H][Lq][Lk] of type dtype = the bias matrix; backward: g of type dtype -> dtable [num_buckets][H] fp32 (overwritten;
+ * deterministic; ws: dfold_relpos_ws(H, Lq, num_buckets) floats). */
+int dfold_relpos_fwd(const dfold_rel_bias* rel, void* out, int32_t dtype, int32_t H, int32_t Lq, int32_t Lk, void* stream);
+int dfold_relpos_bwd(const dfold_rel_bias* rel, const void* g, int32_t dtype, int32_t H, int32_t Lq, int32_t Lk, float* dtable, float* ws,
+                     void* stream);
+int dfold_relpos_ws(int32_t H, int32_t Lq, int32_t num_buckets);
+
+/* o = softmax(scale q k^T + bias) v.  q [B][Lq][H][D], k, v [B][Lk][Hkv][D], o like q: bf16 or f16, the last axis dense, other
+ * strides in elements, multiples of 8, base pointers 16-byte aligned; D a multiple of 8, <= 128; H a multiple of Hkv (query head h
+ * reads key head h / (H / Hkv)).  Keys j >= kv_lens[b] and keys with key_mask[b * mask_sb + j] == 0 do not exist: their K and V
+ * are never used (they may hold NaN); a row without any key gives zeros.
+ *   lse [B][H][Lq] fp32 (optional): log2 of the row's sum of exp2 (logits x log2 e); +inf for a row without keys.
+ *   splits > 1: the keys are cut into that many parts; ws: splits * B * H * Lq * (D + 1) floats.
+ *   pack = 1, or H / Hkv (rows of the query heads of a group share tiles: few queries). */
+typedef struct {
+  const void *q, *k, *v;
+  void* o;
+  float *lse, *ws;
+  const uint8_t* key_mask;
+  const int32_t* kv_lens;
+  int64_t q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh, o_sb, o_sl, o_sh, mask_sb;
+  int32_t dtype, B, Lq, Lk, H, Hkv, D, splits, pack;
+  float scale;
+  dfold_rel_bias rel;
+} dfold_seq_attn_desc;
+int dfold_seq_attn_fwd(const dfold_seq_attn_desc* desc, void* stream);
+
+/* Backward (Lk >= 1).  fwd: the descriptor of the forward call (o, lse as written there; splits, pack, ws unused).  d_o like o (strides
+ * do_*); dq [B][Lq][H][D], dk, dv [B][Lk][Hkv][D] dense (every element is written; masked keys get zeros).  delta [B][H][Lq] fp32
+ * scratch (1 + splits_q planes of it if splits_q > 1).  dtable [num_buckets][H] fp32 (NULL without bias).  splits_q / splits_k: parts of the key axis in the dQ pass / of the
+ * (head of group, query) axis in the dK, dV pass.  ws, floats: (splits_q > 1: splits_q B Lq H D) + (splits_k > 1: 2 splits_k B Lk
+ * Hkv D) + (bias: splits_k B H ceil(Lk / 128) num_buckets), the three parts each rounded up to a multiple of 4.  No atomics on
+ * global memory: deterministic. */
+typedef struct {
+  const void* d_o;
+  int64_t do_sb, do_sl, do_sh;
+  void *dq, *dk, *dv;
+  float *delta, *dtable, *ws;
+  int32_t splits_q, splits_k;
+} dfold_seq_attn_grad;
+int dfold_seq_attn_bwd(const dfold_seq_attn_desc* fwd, const dfold_seq_attn_grad* grad, void* stream);
+
+/* y = R(position) (x * rsqrt(mean(x^2) + eps) * w) for every head of q [B][Lq][H][D] and k [B][Lk][Hkv][D] in one launch (either may
+ * be NULL).  bf16, f16 or fp32, the last axis dense, other strides in elements, multiples of 16 bytes, D a multiple of 8, <= 256;
+ * outputs dense.  w [D] fp32 or NULL (ones).  Rotation of the first rotary_dim dimensions (a multiple of 16, 0: none): pairs
+ * (i, i + rotary_dim / 2), or (2 i, 2 i + 1) if interleaved, turned by position * base^(-2 i / rotary_dim); positions int64 [B][L],
+ * row stride pos_sb (0: shared by the batch), or NULL: 0, 1, ...  The angle is reduced in fp64: exact to fp32 rounding for every
+ * position.  Backward: dx like x but dense, dw [D] fp32 (optional; ws: dfold_qk_norm_rope_ws() floats). */
+typedef struct {
+  const void* x;
+  void* y;             /* output; backward: dx */
+  const void* g;       /* backward: gradient of y, strides g_s* */
+  const float* w;
+  float* dw;
+  const int64_t* pos;
+  int64_t x_sb, x_sl, x_sh, g_sb, g_sl, g_sh, pos_sb;
+  int32_t L, H;
+} dfold_norm_rope_part;
+typedef struct {
+  dfold_norm_rope_part part[2];   /* q, k; x == NULL: absent */
+  float* ws;
+  double base;
+  float eps;
+  int32_t dtype, B, D, rotary_dim, interleaved;
+} dfold_norm_rope_desc;
+int dfold_qk_norm_rope_fwd(const dfold_norm_rope_desc* desc, void* stream);
+int dfold_qk_norm_rope_bwd(const dfold_norm_rope_desc* desc, void* stream);
+int dfold_qk_norm_rope_ws(void);
+
 #ifdef __cplusplus
 }
 #endif

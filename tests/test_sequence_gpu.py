@@ -1,0 +1,579 @@
+"""Sequence-track operators on the GPU against their definitions in fp64 on the same inputs.
+
+Tolerances are element-wise bounds of the roundings the kernels make, u = half a step of the operand type (bf16 2^-8, fp16 2^-11):
+  o    P is rounded to the operand type before P V and the result is rounded:           u sum p |v| + u |o|
+  dV   likewise:                                                                         u sum P |dO| + u |dV|
+  dS   = P (dP - delta), rounded before it meets K or Q; dP and delta carry fp32 sums of |dO| |v| and sum P |dP|:
+                                                                                         u |dS| + E P (|dO| |v| + sum P |dO| |v|)
+       for dQ, delta = dO O has the roundings of o and of P in o:                        + P (u sum |dO| |o| + u sum P |dP|)
+  dQ, dK   scale times the sums of that with |k|, |q|, and one rounding of the result; the table's gradient is summed from dS in fp32.
+E = 2^-14 covers the fp32 arithmetic of logits and exponentials (|logit| < 64: absolute error below 64 * 2^-22) and u^2.  fp16 operands
+below 2^-14 have an absolute step of 2^-24: a further 2^-25 per rounded P or dS (for o in delta: 2^-25 sum |dO| (1 + sum |v|))."""
+import math
+
+import pytest
+import torch
+
+from dynamicpdb_amd.model import sequence_attention as S
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+E = 2.0 ** -14
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+def bucket_matrix(Lq, Lk, nb, dist, both, off):
+    """bucket of every (query, key), whole-number arithmetic only; off: int or [B] list -> [B or 1, Lq, Lk]"""
+    offs = torch.as_tensor(off).reshape(-1, 1, 1)
+    d = torch.arange(Lk)[None, None, :] - torch.arange(Lq)[None, :, None] - offs
+    half = nb // 2 if both else nb
+    n = d.abs() if both else (-d).clamp(min=0)
+    e = half // 2
+    far = torch.tensor(S.far_borders(nb, dist, both), dtype=torch.long)
+    b = torch.where(n < e, n, e + torch.searchsorted(far, n.clamp(max=4096).contiguous(), right=True) if len(far) else torch.full_like(n, e))
+    return (b + (half * (d > 0) if both else 0)).to(DEV)
+
+
+def reference(q, k, v, g, live, table, buckets, scale):
+    """fp64 outputs, gradients and the element-wise magnitudes of the bounds above"""
+    B, Lq, H, D = q.shape
+    Hkv = k.shape[2]
+    G = H // Hkv
+    u = torch.finfo(q.dtype).eps / 2
+    sub = 2.0 ** -25 if q.dtype == HF else 0.0
+    t = lambda x, r=1: x.double().transpose(1, 2).repeat_interleave(r, 1)          # [B, H, L, D]
+    q64, k64, v64, g64 = t(q), t(k, G), t(v, G), t(g)
+    lv = live[:, None, None, :]
+    k64, v64 = (torch.where(live[:, None, :, None], x, torch.zeros((), dtype=torch.float64, device=DEV)) for x in (k64, v64))
+    s = q64 @ k64.transpose(-1, -2) * scale
+    if table is not None:
+        s = s + table.double()[buckets].permute(0, 3, 1, 2)
+    s = torch.where(lv, s, torch.full_like(s, -math.inf))
+    m = s.amax(-1, keepdim=True) if s.shape[-1] else torch.zeros_like(s[..., :0].sum(-1, keepdim=True))
+    m = torch.where(m == -math.inf, torch.zeros_like(m), m)
+    p = torch.exp(s - m)
+    l = p.sum(-1, keepdim=True)
+    p = p / torch.where(l == 0, torch.ones_like(l), l)
+    o = p @ v64
+    delta = (o * g64).sum(-1, keepdim=True)
+    dp = g64 @ v64.transpose(-1, -2)
+    ds = p * (dp - delta)
+    a_dp = g64.abs() @ v64.abs().transpose(-1, -2)
+    a_delta = (p * a_dp).sum(-1, keepdim=True)
+    q_delta = u * (o.abs() * g64.abs()).sum(-1, keepdim=True) + u * (p * dp.abs()).sum(-1, keepdim=True)
+    if sub:
+        q_delta = q_delta + sub * (g64.abs() * (1 + (v64.abs() * live[:, None, :, None].double()).sum(-2, keepdim=True))).sum(-1, keepdim=True)
+    # without keys, P and dS are exact zeros
+    lvf = lv.double() * (l > 0)
+    ds_err = (u + E) * ds.abs() + p * E * (a_dp + a_delta) + sub * lvf
+    p_err = (u + E) * p + sub * lvf
+    fold = lambda x: x.unflatten(1, (Hkv, G)).sum(2)                                # heads of a group
+    back = lambda x: x.transpose(1, 2)
+    outs = dict(o=(o, p_err @ v64.abs()), dq=(ds @ k64 * scale, (ds_err + p * q_delta) @ k64.abs() * scale),
+                dk=(fold(ds.transpose(-1, -2) @ q64 * scale), fold(ds_err.transpose(-1, -2) @ q64.abs() * scale)),
+                dv=(fold(p.transpose(-1, -2) @ g64), fold(p_err.transpose(-1, -2) @ g64.abs())))
+    outs = {n: (back(x), back(e) + u * back(x).abs() + 2.0 ** -24 * (1 if q.dtype == HF else 0) + 1e-30) for n, (x, e) in outs.items()}
+    if table is not None:
+        nb = table.shape[0]
+        bk = buckets.expand(B, *buckets.shape[1:]).reshape(B, 1, -1).expand(B, H, -1)
+        add = lambda x: torch.zeros(B, H, nb, dtype=torch.float64, device=DEV).scatter_add_(2, bk, x.reshape(B, H, -1)).sum(0).t()
+        # (dS enters unrounded: no u; sums of n terms in fp32, blocked: 2^-18 of the sum of magnitudes)
+        err = E * ds.abs() + p * E * (a_dp + a_delta)
+        outs["dtable"] = (add(ds), add(err) + 2.0 ** -18 * add(ds.abs()) + 1e-30)
+    return outs
+
+
+def within(name, got, ref):
+    x, bound = ref
+    assert got.shape == x.shape, name
+    bad = (got.double() - x).abs() / bound
+    bad = torch.where(torch.isnan(bad), torch.full_like(bad, math.inf), bad)
+    worst = bad.max().item() if bad.numel() else 0.0
+    assert worst <= 1.0, f"{name}: {worst:.3g} times its bound"
+
+
+def make(B, Lq, Lk, H, Hkv, D, dt, seed=0):
+    gen = torch.Generator(device=DEV).manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=gen, device=DEV).to(dt)
+    return r(B, Lq, H, D), r(B, Lk, Hkv, D), r(B, Lk, Hkv, D), r(B, Lq, H, D)
+
+
+def make_mask(kind, B, Lk, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    ones = torch.ones(B, Lk, dtype=torch.bool, device=DEV)
+    if kind == "none":
+        return ones, {}
+    if kind == "lens":
+        lens = torch.randint(0, Lk + 1, (B,), generator=gen).to(torch.int32)
+        lens[0] = Lk // 2 + 1 if Lk else 0
+        if B > 1:
+            lens[-1] = 0
+        lens = lens.to(DEV)
+        return torch.arange(Lk, device=DEV)[None] < lens[:, None], dict(kv_lens=lens)
+    keep = (torch.rand(B, Lk, generator=gen) < 0.7).to(DEV)
+    keep[:, 64:min(Lk, 192)] = False if Lk > 260 else keep[:, 64:min(Lk, 192)]     # whole tiles without a key
+    if kind == "both":
+        lens = torch.full((B,), Lk - Lk // 3, dtype=torch.int64, device=DEV)
+        return keep & (torch.arange(Lk, device=DEV)[None] < lens[:, None]), dict(key_mask=keep.float(), kv_lens=lens)
+    return keep, dict(key_mask=keep)
+
+
+def run(q, k, v, g, table=None, **kw):
+    leaves = [t.detach().requires_grad_(True) for t in (q, k, v)] + ([table.detach().requires_grad_(True)] if table is not None else [])
+    o = S.cross_attention(*leaves[:3], rel_table=leaves[3] if table is not None else None, **kw)
+    grads = torch.autograd.grad(o, leaves, g)
+    return dict(zip(("o", "dq", "dk", "dv", "dtable"), (o.detach(), *grads)))
+
+
+CASES = [
+    # B, Lq, Lk, H, Hkv, D, type, mask, (buckets, distance, both, offset) or None
+    (1, 1, 1, 1, 1, 8, BF, "none", None),
+    (2, 1, 77, 8, 8, 32, BF, "lens", None),
+    (3, 5, 130, 8, 2, 64, HF, "keys", None),
+    (1, 128, 64, 2, 1, 128, BF, "none", None),
+    (2, 129, 65, 4, 4, 40, HF, "both", None),
+    (1, 31, 63, 6, 2, 16, BF, "none", None),
+    (2, 33, 200, 4, 2, 96, BF, "keys", (32, 128, True, 0)),
+    (2, 300, 700, 4, 4, 64, BF, "lens", (32, 128, True, 0)),
+    (1, 64, 5000, 2, 1, 128, BF, "keys", None),
+    (1, 1, 9000, 4, 1, 128, HF, "none", None),
+    (2, 700, 40, 4, 1, 32, BF, "keys", None),
+    (1, 260, 260, 3, 3, 64, BF, "none", (17, 100, False, 5)),
+    (1, 200, 333, 2, 2, 128, HF, "keys", (64, 1024, True, -40)),
+    (4, 1, 1000, 8, 2, 64, BF, "lens", (32, 128, True, [999, 500, 0, 3])),
+    (2, 7, 50, 8, 1, 24, BF, "none", (4, 2, True, 20)),
+    (1, 513, 1025, 1, 1, 48, HF, "both", (48, 300, True, 0)),
+    (1, 100, 100, 2, 2, 32, BF, "none", (32, 128, True, 100000)),
+]
+
+
+@pytest.mark.parametrize("case", CASES, ids=lambda c: "x".join(str(x) for x in c[:6]) + f"-{str(c[6])[6:]}-{c[7]}-{c[8]}".replace(" ", ""))
+def test_attention_forward_and_gradients(case):
+    B, Lq, Lk, H, Hkv, D, dt, mask, rel = case
+    q, k, v, g = make(B, Lq, Lk, H, Hkv, D, dt)
+    live, kw = make_mask(mask, B, Lk)
+    table = buckets = None
+    if rel:
+        nb, dist, both, off = rel
+        table = torch.randn(nb, H, generator=torch.Generator(device=DEV).manual_seed(7), device=DEV)
+        buckets = bucket_matrix(Lq, Lk, nb, dist, both, off)
+        kw.update(max_distance=dist, bidirectional=both, q_offset=torch.tensor(off, device=DEV) if isinstance(off, list) else off)
+    got = run(q, k, v, g, table, **kw)
+    ref = reference(q, k, v, g, live, table, buckets, D ** -0.5)
+    for name in ref:
+        within(name, got[name], ref[name])
+    with torch.no_grad():                       # the call that keeps nothing for a backward pass gives the same bits
+        assert torch.equal(S.cross_attention(q, k, v, rel_table=table, **kw), got["o"])
+    again = run(q, k, v, g, table, **kw)
+    assert all(torch.equal(again[n], got[n]) for n in got)
+
+
+def test_attention_gradient_against_differences():
+    """directional derivatives of the fp64 definition by central differences (step 2^-12: truncation and fp64 rounding below 1e-6 of
+    the bound's scale) against the kernels' gradients; the bound is the element-wise one, summed over the direction"""
+    B, Lq, Lk, H, Hkv, D = 1, 20, 45, 2, 1, 32
+    q, k, v, g = make(B, Lq, Lk, H, Hkv, D, BF, seed=3)
+    table = torch.randn(8, H, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))
+    live, kw = make_mask("keys", B, Lk)
+    buckets = bucket_matrix(Lq, Lk, 8, 20, True, 0)
+    got = run(q, k, v, g, table, max_distance=20, **kw)
+    ref = reference(q, k, v, g, live, table, buckets, D ** -0.5)
+
+    def value(q, k, v, table):
+        s = torch.einsum("bihd,bjhd->bhij", q.cpu(), k.cpu().repeat_interleave(H // Hkv, 2)) * D ** -0.5 + table.cpu()[buckets.cpu()].permute(0, 3, 1, 2)
+        p = torch.softmax(s.masked_fill(~live.cpu()[:, None, None], -math.inf), -1)
+        return (torch.einsum("bhij,bjhd->bihd", p, v.cpu().repeat_interleave(H // Hkv, 2)) * g.double().cpu()).sum().item()
+    args = [t.double() for t in (q, k, v, table)]
+    for i, name in enumerate(("dq", "dk", "dv", "dtable")):
+        way = torch.randn(args[i].shape, generator=torch.Generator().manual_seed(i), dtype=torch.float64).to(DEV)
+        h = 2.0 ** -12
+        plus, minus = [list(args), list(args)]
+        plus[i], minus[i] = args[i] + h * way, args[i] - h * way
+        num = (value(*plus) - value(*minus)) / (2 * h)
+        bound = (ref[name][1] * way.abs()).sum().item()
+        assert abs(num - (got[name].double() * way).sum().item()) <= bound + 1e-4 * abs(num)
+
+
+@pytest.mark.parametrize("Lq,Lk", [(0, 5), (5, 0), (0, 0)])
+def test_attention_empty_axes(Lq, Lk):
+    q, k, v, g = make(2, Lq, Lk, 4, 2, 32, BF)
+    table = torch.randn(32, 4, device=DEV)
+    got = run(q, k, v, g, table)
+    assert got["o"].shape == q.shape and got["dk"].shape == k.shape
+    assert all(bool((x == 0).all()) for x in got.values())
+
+
+def test_attention_masked_places_may_hold_anything():
+    """NaN and infinities in K and V of masked keys, rows without a key: finite results, zeros where there is nothing"""
+    B, Lq, Lk, H, Hkv, D = 3, 40, 150, 4, 2, 64
+    q, k, v, g = make(B, Lq, Lk, H, Hkv, D, BF)
+    live, kw = make_mask("both", B, Lk)
+    live[1] = False
+    kw["key_mask"] = live.clone()
+    clean = run(q, k, v, g, **kw)
+    k, v = k.clone(), v.clone()
+    dead = ~live
+    k[dead], v[dead] = float("nan"), float("inf")
+    k[0, Lk - 1], v[0, Lk - 1] = float("-inf"), float("nan")
+    got = run(q, k, v, g, **kw)
+    for n in got:
+        assert torch.equal(got[n], clean[n]), n
+    assert bool((got["o"][1] == 0).all()) and bool((got["dq"][1] == 0).all()) and bool((got["dk"][dead] == 0).all()) and bool((got["dv"][dead] == 0).all())
+
+
+@pytest.mark.parametrize("low", [torch.finfo(torch.float32).min, float("-inf"), -1e30])
+def test_attention_bias_that_masks(low):
+    """buckets of the type's lowest value: keys of other buckets win; a row that has nothing but such keys is an ordinary softmax over
+    them (finite) or empty (-inf)"""
+    B, Lq, Lk, H, D = 1, 70, 20, 2, 32
+    q, k, v, g = make(B, Lq, Lk, H, H, D, BF)
+    table = torch.randn(8, H, device=DEV)
+    table[3] = low                           # everything from distance -16 on: later queries see nothing else
+    buckets = bucket_matrix(Lq, Lk, 8, 16, True, 0)
+    assert bool((buckets[0, -1] == 3).all()) and not bool((buckets[0, 0] == 3).any())
+    got = run(q, k, v, g, table, max_distance=16)
+    live = torch.ones(B, Lk, dtype=torch.bool, device=DEV)
+    if low == float("-inf"):
+        ref = reference(q, k, v, g, live, table, buckets, D ** -0.5)
+    else:                                    # a uniform shift of a row changes nothing: -1e30 + logit is -1e30 in fp32, logits drop out
+        t64 = table.double()
+        s = (torch.einsum("bihd,bjhd->bhij", q.double().cpu(), k.double().cpu()) * D ** -0.5).to(DEV)
+        s = torch.where((buckets == 3)[:, None], torch.full_like(s, low), s + t64[buckets].permute(0, 3, 1, 2))
+        p = torch.softmax(s, -1)
+        o = (p @ v.double().transpose(1, 2)).transpose(1, 2)
+        bound = 2.0 ** -8 * ((p @ v.double().abs().transpose(1, 2)).transpose(1, 2) + o.abs()) + E
+        within("o", got["o"], (o, bound))
+        assert all(bool(torch.isfinite(x).all()) for x in got.values())
+        return
+    for n in ("o", "dq", "dk", "dv"):
+        within(n, got[n], ref[n])
+    assert bool((got["o"][0, -1] == 0).all())
+
+
+def test_attention_reads_strided_inputs():
+    """fused projections, head-major storage, broadcast heads, offset bases and a transposed last axis: same bits as dense copies, and
+    gradients of the layouts' own leaves"""
+    B, L, H, D = 2, 75, 4, 32
+    gen = torch.Generator(device=DEV).manual_seed(5)
+    r = lambda *s: torch.randn(*s, generator=gen, device=DEV).to(BF)
+    qkv = r(B, L, 3, H, D)
+    views = [
+        (qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2]),
+        tuple(r(B, H, L, D).transpose(1, 2) for _ in range(3)),
+        (r(B, L, H, D), r(B, L, 1, D).expand(B, L, H, D), r(1, L, 1, D).expand(B, L, H, D)),
+        tuple(r(B, L, H, D + 8)[..., 1:D + 1] for _ in range(3)),
+        tuple(r(B, L, H, D + 4)[..., :D] for _ in range(3)),
+        tuple(r(B, L, D, H).transpose(2, 3) for _ in range(3)),
+        tuple(r(L, B, H, D).transpose(0, 1)[:, ::2] for _ in range(3)),
+    ]
+    for q, k, v in views:
+        g = r(*q.shape)
+        want = run(q.contiguous(), k.contiguous(), v.contiguous(), g)
+        got = run(q, k, v, g)
+        for n in want:
+            assert torch.equal(want[n], got[n])
+        g_view = g.transpose(1, 2).contiguous().transpose(1, 2)
+        got = run(q, k, v, g_view)
+        assert all(torch.equal(want[n], got[n]) for n in want)
+    # shared (broadcast) keys: the leaf's gradient is the sum over the heads
+    leaf = r(B, L, 1, D).requires_grad_(True)
+    q, v, g = r(B, L, H, D), r(B, L, H, D), r(B, L, H, D)
+    (dleaf,) = torch.autograd.grad(S.cross_attention(q, leaf.expand(B, L, H, D), v), [leaf], g)
+    dk = run(q, leaf.detach().expand(B, L, H, D).contiguous(), v, g)["dk"]
+    # (torch adds the four bf16 gradients in fp32 and rounds once)
+    assert (dleaf.double() - dk.double().sum(2, keepdim=True)).abs().max() <= 2.0 ** -8 * dk.double().abs().sum(2).max() + 1e-30
+    # a sum's gradient: every stride 0
+    x = r(B, L, H, D).requires_grad_(True)
+    S.cross_attention(x, q, v).sum().backward()
+    assert torch.equal(x.grad, run(x, q, v, torch.ones_like(x))["dq"])
+
+
+def test_attention_offsets_past_32_bits():
+    """batch items of a cache that lie further apart than 2^31 elements"""
+    B, Lq, Lk, H, D = 2, 3, 100, 2, 64
+    step = (1 << 31) + 4096
+    store = torch.empty(step + 2 * Lk * H * D, dtype=BF, device=DEV)
+    k = store.as_strided((B, Lk, H, D), (step, H * D, D, 1))
+    v = store.as_strided((B, Lk, H, D), (step, H * D, D, 1), Lk * H * D)
+    q, kd, vd, g = make(B, Lq, Lk, H, H, D, BF)
+    k.copy_(kd)
+    v.copy_(vd)
+    want, got = run(q, kd, vd, g), run(q, k, v, g)
+    assert all(torch.equal(want[n], got[n]) for n in want)
+
+
+def test_attention_partial_gradients():
+    q, k, v, g = make(1, 50, 60, 2, 2, 32, BF)
+    want = run(q, k, v, g)
+    k2 = k.clone().requires_grad_(True)
+    assert torch.equal(torch.autograd.grad(S.cross_attention(q, k2, v), k2, g)[0], want["dk"])
+    t = torch.zeros(32, 2, device=DEV, requires_grad=True)
+    (dt,) = torch.autograd.grad(S.cross_attention(q, k, v, rel_table=t), t, g)
+    assert torch.equal(dt, run(q, k, v, g, t)["dtable"])
+    with pytest.raises(RuntimeError):         # differentiable once
+        x = q.clone().requires_grad_(True)
+        (d,) = torch.autograd.grad(S.cross_attention(x, k, v), x, g, create_graph=True)
+        d.sum().backward()
+
+
+@pytest.mark.parametrize("D", [32, 64, 128])
+def test_attention_split_keys_equal_whole(D):
+    """the parts of the key axis meet to the same softmax: every cut of a call against the bounds (parts without a live key among them)"""
+    B, Lq, Lk, H, Hkv = 2, 3, 900, 4, 2
+    q, k, v, g = make(B, Lq, Lk, H, Hkv, D, BF)
+    live, kw = make_mask("lens", B, Lk)
+    ref = reference(q, k, v, g, live, None, None, D ** -0.5)
+    plan = S._parts
+    try:
+        for parts in (1, 2, 3, 7, 15, 40):
+            S._parts = lambda groups, units, n_cu, least, n=parts: n
+            got = run(q, k, v, g, **kw)
+            for n in ref:
+                within(f"{n} in {parts} parts", got[n], ref[n])
+    finally:
+        S._parts = plan
+
+
+# ---- relative position bias ---------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("H,Lq,Lk,nb,dist,both,off", [(1, 1, 1, 4, 2, True, 0), (3, 7, 5, 32, 128, True, 0), (8, 256, 256, 32, 128, True, 0), (2, 300, 1, 16, 64, True, 3),
+                                                      (5, 1, 777, 32, 128, False, 700), (4, 333, 1001, 64, 500, True, -20), (2, 1100, 1300, 17, 1024, False, 0),
+                                                      (16, 3, 2, 512, 1024, True, 1000000), (1, 2000, 2600, 32, 128, True, 0)])
+@pytest.mark.parametrize("dt", [F32, BF, HF])
+def test_bias_matrix(H, Lq, Lk, nb, dist, both, off, dt):
+    gen = torch.Generator(device=DEV).manual_seed(Lq)
+    table = torch.randn(nb, H, generator=gen, device=DEV, requires_grad=True)
+    bk = bucket_matrix(Lq, Lk, nb, dist, both, off)[0]
+    out = S.relative_position_bias(table, Lq, Lk, max_distance=dist, bidirectional=both, q_offset=off, dtype=dt)
+    assert torch.equal(out, table.detach()[bk].permute(2, 0, 1).to(dt))
+    g = torch.randn(H, Lq, Lk, generator=gen, device=DEV).to(dt)
+    (dtable,) = torch.autograd.grad(out, table, g)
+    add = lambda x: torch.zeros(H, nb, dtype=torch.float64, device=DEV).scatter_add_(1, bk.reshape(1, -1).expand(H, -1), x.reshape(H, -1).double()).t()
+    # fp32 sums: the longest chain is a thread's share of a run of rows, then the lanes, the runs
+    rows = -(-Lq // min(Lq, max(1024 // H, 1)))
+    chain = rows * Lk / 256 + rows + 64 + Lq / rows / 16 + 16
+    within("dtable", dtable, (add(g), 2.0 ** -24 * chain * add(g.abs()) + 1e-30))
+    (again,) = torch.autograd.grad(S.relative_position_bias(table, Lq, Lk, max_distance=dist, bidirectional=both, q_offset=off, dtype=dt), table, g)
+    assert torch.equal(again, dtable)
+
+
+def test_bias_empty_and_module():
+    t = torch.randn(32, 4, device=DEV, requires_grad=True)
+    for Lq, Lk in ((0, 4), (4, 0)):
+        out = S.relative_position_bias(t, Lq, Lk)
+        assert out.shape == (4, Lq, Lk)
+        assert bool((torch.autograd.grad(out, t, torch.zeros_like(out))[0] == 0).all())
+    m = S.RelativePositionBias(32, 4, max_distance=64).to(DEV)
+    torch.nn.init.normal_(m.table)
+    assert torch.equal(m(9, 11, 2), S.relative_position_bias(m.table, 9, 11, max_distance=64, q_offset=2))
+    # the gradient of a sum: strides 0
+    m(9, 11).sum().backward()
+    counts = torch.bincount(bucket_matrix(9, 11, 32, 64, True, 0).reshape(-1), minlength=32).float()
+    assert torch.equal(m.table.grad, counts[:, None].expand(32, 4).to(DEV))
+
+
+# ---- norm + rotation ------------------------------------------------------------------------------------------------------------------
+
+def rope_reference(x, w, pos, rd, base, inter, eps, g):
+    """fp64 result and gradients with the bounds of fp32 arithmetic: n * 2^-24 of the magnitudes that meet in an element.  n: products and
+    sums of an element ~ 8, the reduction's tree ~ 12, its square root and quotient ~ 3, sine and cosine 2 units and their argument's
+    rounding pi units: 32 covers the forward; the backward has two reductions and one more product: 64"""
+    x, g = x.double(), g.double()
+    w = torch.ones(x.shape[-1], dtype=torch.float64, device=DEV) if w is None else w.double()
+    i = torch.arange(rd // 2, device=DEV)
+    lo, hi = (2 * i, 2 * i + 1) if inter else (i, i + rd // 2)
+    ang = pos.double()[..., None, None] * base ** (-2.0 * i.double() / max(rd, 1))
+    c, s = torch.cos(ang), torch.sin(ang)
+
+    def turn(y, sgn):
+        z = y.clone()
+        z[..., lo], z[..., hi] = y[..., lo] * c - sgn * y[..., hi] * s, y[..., hi] * c + sgn * y[..., lo] * s
+        return z
+
+    def both(y):                            # |a| + |b| of a pair
+        z = y.abs().clone()
+        z[..., lo] = z[..., hi] = y[..., lo].abs() + y[..., hi].abs()
+        return z
+    rstd = torch.rsqrt((x * x).mean(-1, keepdim=True) + eps)
+    xh = x * rstd
+    y = turn(xh * w, 1)
+    gt = turn(g, -1)
+    gw, G = gt * w, both(g)
+    dx = rstd * (gw - xh * (gw * xh).mean(-1, keepdim=True))
+    e = 2.0 ** -24
+    dx_err = 64 * e * rstd * (G * w.abs() + xh.abs() * (G * w.abs() * xh.abs()).mean(-1, keepdim=True))
+    return (y, 32 * e * both(xh * w)), (dx, dx_err), ((gt * xh).sum((0, 1, 2)), 64 * e * (G * xh.abs()).sum((0, 1, 2)))
+
+
+@pytest.mark.parametrize("B,Lq,Lk,H,Hkv,D,rd,inter,far", [
+    (1, 1, 1, 1, 1, 8, 0, False, 10), (2, 1, 3, 8, 2, 64, 64, False, 1 << 20), (1, 17, 17, 3, 1, 32, 32, True, 5000), (3, 33, 20, 5, 5, 80, 32, False, 100),
+    (2, 130, 130, 32, 8, 128, 128, False, 1 << 20), (1, 9, 4, 2, 2, 256, 256, True, 1 << 30), (1, 257, 1, 4, 4, 40, 16, True, 3000), (2, 5, 70, 16, 1, 96, 96, False, 70),
+    (1, 3000, 3000, 8, 8, 16, 16, False, 4000)])
+@pytest.mark.parametrize("dt", [F32, BF, HF])
+def test_norm_rope(B, Lq, Lk, H, Hkv, D, rd, inter, far, dt):
+    gen = torch.Generator(device=DEV).manual_seed(D + Lq)
+    r = lambda *s: torch.randn(*s, generator=gen, device=DEV)
+    q, k = (r(B, Lq, H, D) * 2).to(dt).requires_grad_(True), (r(B, Lk, Hkv, D) * 0.3).to(dt).requires_grad_(True)
+    wq, wk = (1 + 0.2 * r(D)).requires_grad_(True), (1 + 0.2 * r(D)).requires_grad_(True)
+    gq, gk = r(B, Lq, H, D).to(dt), r(B, Lk, Hkv, D).to(dt)
+    pq = torch.randint(0, far, (B, Lq), generator=gen, device=DEV)
+    kw = dict(rotary_dim=rd, interleaved=inter, base=10000.0, eps=1e-6)
+    oq, ok = S.qk_norm_rope(q, k, wq, wk, pq, None, **kw)
+    grads = torch.autograd.grad([oq, ok], [q, k, wq, wk], [gq, gk])
+    u = torch.finfo(dt).eps / 2
+    tiny = 2.0 ** -25 if dt == HF else 1e-30
+    for x, w, pos, g, o, dx, dw in ((q, wq, pq, gq, oq, grads[0], grads[2]), (k, wk, torch.arange(Lk, device=DEV)[None], gk, ok, grads[1], grads[3])):
+        with torch.no_grad():
+            ref = rope_reference(x, w, pos, rd, 10000.0, inter, 1e-6, g)
+        for n, got, (want, err) in zip(("y", "dx"), (o.detach(), dx), ref):
+            within(n, got, (want, err + u * (want.abs() + err) + tiny))
+        # a block's share: a slot's rows one after another, at most 256 slots, then fp64
+        rows = x.numel() // D
+        within("dw", dw, (ref[2][0], ref[2][1] * (1 + (rows / 1024 + 256) / 64)))
+    again = torch.autograd.grad(S.qk_norm_rope(q, k, wq, wk, pq, None, **kw), [q, k, wq, wk], [gq, gk])
+    assert all(torch.equal(a, b) for a, b in zip(again, grads))
+
+
+def test_norm_rope_layouts_and_options():
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=gen, device=DEV).to(BF)
+    B, L, H, D = 2, 21, 4, 64
+    fused = r(B, L, 3, H, D)
+    q, k = fused[:, :, 0], fused[:, :, 1]
+    want = S.qk_norm_rope(q.contiguous(), k.contiguous())
+    for a, b in ((q, k), (r(B, H, L, D).transpose(1, 2).copy_(q), k), (q, torch.cat([k, k], -1)[..., D:]), (torch.empty(B, L, H, D + 2, device=DEV, dtype=BF)[..., 2:].copy_(q), k)):
+        got = S.qk_norm_rope(a, b)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    # one alone, shared positions, int32 positions, positions of another stride
+    assert torch.equal(S.qk_norm_rope(q, None)[0], want[0]) and S.qk_norm_rope(q, None)[1] is None
+    assert torch.equal(S.qk_norm_rope(None, k)[1], want[1])
+    pos = torch.arange(L, device=DEV)
+    for p in (pos, pos.int(), pos[None], pos[None].expand(B, L), torch.stack([pos, pos], 1)[:, 0], torch.stack([pos] * B, 1).t()):
+        assert torch.equal(S.qk_norm_rope(q, k, q_positions=p, k_positions=p)[1], want[1])
+    # empty sequences; gradients through one output only; the gradient of a sum
+    e = torch.zeros(B, 0, H, D, dtype=BF, device=DEV)
+    assert S.qk_norm_rope(e, k)[0].shape == e.shape and torch.equal(S.qk_norm_rope(e, k)[1], want[1])
+    x, w = q.detach().clone().requires_grad_(True), torch.ones(D, device=DEV, requires_grad=True)
+    y, z = S.qk_norm_rope(x, k, w, w)
+    gx, gw = torch.autograd.grad(y.float().sum(), [x, w])
+    gx2, gw2 = torch.autograd.grad(S.qk_norm_rope(x, None, w)[0], [x, w], torch.ones_like(x))
+    assert torch.equal(gx, gx2) and torch.equal(gw, gw2)
+    # a row of zeros stays zero and finite
+    zero = torch.zeros(1, 1, 1, D, dtype=BF, device=DEV, requires_grad=True)
+    y, _ = S.qk_norm_rope(zero, None)
+    assert bool((y == 0).all()) and bool(torch.isfinite(torch.autograd.grad(y, zero, torch.ones_like(y))[0]).all())
+
+
+# ---- together ---------------------------------------------------------------------------------------------------------------------------
+
+def chain(qkv, wq, wk, table, lens):
+    q, k = S.qk_norm_rope(qkv[:, :, 0], qkv[:, :, 1], wq, wk)
+    return S.cross_attention(q, k, qkv[:, :, 2], kv_lens=lens, rel_table=table)
+
+
+def test_run_of_all_on_streams_and_graphs():
+    """norm + rotation -> attention with bias -> gradients: on a side stream, and recorded into a graph that is replayed on new inputs
+    between eager calls, the same bits as the plain call"""
+    B, L, H, D = 2, 200, 4, 64
+    gen = torch.Generator(device=DEV).manual_seed(2)
+    r = lambda *s: torch.randn(*s, generator=gen, device=DEV)
+    sets = [(r(B, L, 3, H, D).to(BF), r(B, L, H, D).to(BF), torch.tensor(ls, dtype=torch.int32, device=DEV)) for ls in ([200, 150], [0, 77], [1, 200])]
+    wq, wk, table = (1 + 0.1 * r(D)), (1 + 0.1 * r(D)), r(32, H)
+
+    def step(qkv, g, lens):
+        leaves = [t.detach().requires_grad_(True) for t in (qkv, wq, wk, table)]
+        o = chain(*leaves, lens)
+        return [o.detach(), *torch.autograd.grad(o, leaves, g)]
+    want = [[t.clone() for t in step(*s)] for s in sets]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(*sets[0])
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want[0]))
+    hold = [t.clone() for t in sets[0]]
+    with torch.cuda.stream(side):
+        step(*hold)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        rec = step(*hold)
+    for turn in (1, 2, 0, 1):
+        for h, t in zip(hold, sets[turn]):
+            h.copy_(t)
+        graph.replay()
+        eager = step(*sets[turn])
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) and torch.equal(a, c) for a, b, c in zip(rec, want[turn], eager))
+
+
+def test_tokens_one_by_one_equal_the_whole():
+    """serving: the queries of a sequence one at a time, each at its own position, against the call on all of them"""
+    B, L, H, Hkv, D = 2, 70, 4, 2, 64
+    q, k, v, _ = make(B, L, L, H, Hkv, D, BF)
+    table = torch.randn(32, H, device=DEV)
+    lens = torch.tensor([70, 33], device=DEV)
+    with torch.no_grad():
+        qn, kn = S.qk_norm_rope(q, k)
+        whole = S.cross_attention(qn, kn, v, rel_table=table, kv_lens=lens)
+        for i in (0, 1, 31, 32, 69):
+            pos = torch.full((B, 1), i, device=DEV)
+            qi, _ = S.qk_norm_rope(q[:, i:i + 1], None, q_positions=pos)
+            assert torch.equal(qi, qn[:, i:i + 1])
+            for off in (i, torch.full((B,), i, device=DEV)):
+                o = S.cross_attention(qi, kn, v, rel_table=table, kv_lens=lens, q_offset=off)
+                # (another cut of the keys: two independent roundings of P and of the result)
+                assert (o.double() - whole[:, i:i + 1].double()).abs().max() <= 2 * 2.0 ** -8 * (v.abs().max().double() * 2)
+
+
+@pytest.mark.parametrize("context", [False, True])
+def test_module(context):
+    """projections, norms, rotation, bias, attention and output projection against the same formulas in fp64 with the module's roundings
+    to bf16 (weights, inputs, heads, attention output): what differs is fp32 accumulation, P's and dS's roundings and single bf16 steps that
+    fall the other way -- five roundings of 2^-8 each, at most, on a path"""
+    torch.manual_seed(0)
+    c, ckv, D, H, Hkv, B, Lq, Lk = 128, 64, 32, 4, 2, 2, 45, 83
+    m = S.CrossAttention(c, ckv if context else c, D, H, Hkv, rotary_dim=32, num_buckets=32).to(DEV)
+    torch.nn.init.normal_(m.rel_bias.table)
+    x = torch.randn(B, Lq, c, device=DEV, requires_grad=True)
+    ctx = torch.randn(B, Lk, ckv, device=DEV, requires_grad=True) if context else None
+    n = Lk if context else Lq
+    mask = torch.ones(B, n, device=DEV)
+    mask[0, n // 2:] = 0
+    out = m(x, ctx, mask=mask)
+    g = torch.randn(out.shape, device=DEV)
+    params = [x] + ([ctx] if context else []) + list(m.parameters())
+    got = torch.autograd.grad(out, params, g)
+
+    class Round(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx_, t):
+            return t.to(BF).double()
+
+        @staticmethod
+        def backward(ctx_, t):
+            return t
+    d64 = {k: p.detach().double().cpu().requires_grad_(True) for k, p in m.named_parameters()}
+    x64 = x.detach().double().cpu().requires_grad_(True)
+    c64 = ctx.detach().double().cpu().requires_grad_(True) if context else x64
+    rnd = Round.apply
+    q = rnd(rnd(x64) @ rnd(d64["linear_q.weight"]).t()).view(B, Lq, H, D)
+    kv = rnd(rnd(c64) @ rnd(d64["linear_kv.weight"]).t()).view(B, n, 2 * Hkv, D)
+
+    def nr(t, w):
+        y = t * torch.rsqrt((t * t).mean(-1, keepdim=True) + 1e-6) * w
+        ang = torch.arange(t.shape[1], dtype=torch.float64)[:, None, None] * 10000.0 ** (-torch.arange(0, D, 2, dtype=torch.float64) / D)
+        a, b = y.chunk(2, -1)
+        return rnd(torch.cat([a * ang.cos() - b * ang.sin(), b * ang.cos() + a * ang.sin()], -1))
+    q, k = nr(q, d64["q_norm"]), nr(kv[:, :, :Hkv], d64["k_norm"]).repeat_interleave(H // Hkv, 2)
+    v = kv[:, :, Hkv:].repeat_interleave(H // Hkv, 2)
+    s = torch.einsum("bihd,bjhd->bhij", q, k) * D ** -0.5 + d64["rel_bias.table"][bucket_matrix(Lq, n, 32, 128, True, 0).cpu()].permute(0, 3, 1, 2)
+    p = torch.softmax(s.masked_fill(mask.cpu()[:, None, None] == 0, -math.inf), -1)
+    o = rnd(torch.einsum("bhij,bjhd->bihd", p, v)).reshape(B, Lq, H * D)
+    ref = o @ rnd(d64["linear_o.weight"]).t() + d64["linear_o.bias"]
+    refs = torch.autograd.grad(ref, [x64] + ([c64] if context else []) + list(d64.values()), g.double().cpu())
+    rel = lambda a, b: ((a.double().cpu() - b).norm() / (b.norm() + 1e-30)).item()
+    assert out.dtype == x.dtype and rel(out.detach(), ref.detach()) <= 5 * 2.0 ** -8
+    for (name, a), b in zip([("x", got[0])] + ([("context", got[1])] if context else []) + list(zip([k for k, _ in m.named_parameters()], got[1 + context:])), refs):
+        assert rel(a, b) <= 5 * 2.0 ** -8, name
