@@ -11,12 +11,15 @@
 //   * dK, dV pass: 128 keys per workgroup, K^T and V^T operands in registers, query tiles of 64 of all heads of the group in LDS:
 //     the sum over shared heads is the accumulator's.  The bias gradient (an fp32 result) is formed here, from fp32 dS with the
 //     corrected delta.
-// Bias gradient: 32 x 32 blocks beyond the last border add to one register per side; nearer blocks add dS to a histogram over the
-// distance in LDS, one per wave and lane half.  Within one instruction the 32 lanes of a half hit 32 different distances, and a
-// wave's LDS operations stay in order: no order of additions is left open.
+// Bias gradient: 32 x 32 blocks beyond the last border add to one register per side.  A nearer block goes through LDS: rows of dS at a
+// pitch of 64 whose other half stays zero, so that lane t reads the 32 entries of diagonal t - 31 without a test, and adds its sum to
+// the wave's histogram over distances: 16 writes, 32 reads and 32 additions per block, in a fixed order.  (LDS float atomics on the
+// histogram itself: 110 -> 234 cycles per instruction of 64 lanes, the pass five times slower at 1001 x 1001.)
 #include "seq_attn.h"
 #include "seq_dtable.h"
 #include <math.h>
+
+#define SA_DIAG (32 + 32 * 64)         // floats of a wave's block of dS, a margin in front
 
 struct SaBwdParams {
   const char *q, *k, *v, *o, *d_o;
@@ -215,7 +218,7 @@ __global__ __launch_bounds__(64 * SA_WAVES, DP == 128 ? 1 : 2) void seq_attn_dkv
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* const ldsL = (float*)(smem + 4 * T::BYTES);            // [stage][log-sum | delta][SA_KT]
   float* const ldsB = ldsL + 4 * SA_KT;
-  float* const ldsH = ldsB + (REL ? 2 * p.rel.W + 1 : 0);       // [wave][lane half][distance]
+  float* const ldsH = ldsB + (REL ? 2 * p.rel.W + 1 : 0);       // [wave][distance]
   const int hn = REL ? 2 * (p.rel.W + SA_REACH) + 1 : 0;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l31 = lane & 31, h = lane >> 5;
@@ -258,14 +261,15 @@ __global__ __launch_bounds__(64 * SA_WAVES, DP == 128 ? 1 : 2) void seq_attn_dkv
 
   int off = 0, head_in = -1;
   const float* myb = ldsB + p.rel.W;
-  float* const myh = ldsH + (w * 2 + h) * hn + p.rel.W + SA_REACH;
+  float* const myh = ldsH + w * hn + p.rel.W + SA_REACH;
+  float* const diag = ldsH + SA_WAVES * hn + w * SA_DIAG + 32;   // 32 rows of 64 behind a margin of 32; columns 32 .. 63 and the margin are zero
   float accL = 0.f, accR = 0.f;
   auto table_part = [&](int head) { return p.ws_t + ((((long)b * p.H + head) * p.splits_k + sp) * nkb + kbk) * p.num_buckets; };
   // a head's histogram over distances -> its buckets; the far sums belong to the last bucket of their side
   auto flush = [&](int head) {
     accL = wave_sum(accL);
     accR = wave_sum(accR);
-    if (lane == 0) {           // (half 0's histogram: entries -W and W carry their buckets)
+    if (lane == 0) {           // (entries -W and W carry their buckets)
       myh[-p.rel.W] += accL;
       myh[p.rel.W] += accR;
     }
@@ -274,7 +278,7 @@ __global__ __launch_bounds__(64 * SA_WAVES, DP == 128 ? 1 : 2) void seq_attn_dkv
     for (int i = tid; i < hn; i += 64 * SA_WAVES) {
       float a = 0.f;
 #pragma unroll
-      for (int c = 0; c < 2 * SA_WAVES; ++c) a += ldsH[c * hn + i];
+      for (int c = 0; c < SA_WAVES; ++c) a += ldsH[c * hn + i];
       ldsH[i] = a;             // (entry i of every copy is this thread's)
     }
     __syncthreads();
@@ -283,6 +287,7 @@ __global__ __launch_bounds__(64 * SA_WAVES, DP == 128 ? 1 : 2) void seq_attn_dkv
   };
   if constexpr (REL) {
     off = sa_q_offset(p.rel, b);
+    for (int i = lane; i < SA_DIAG; i += 64) diag[i - 32] = 0.f;
     for (int g = 0; g < G; ++g)          // heads this part does not touch
       if (max(u0, g * nqt) >= min(u1, (g + 1) * nqt))
         for (int j = tid; j < p.num_buckets; j += 64 * SA_WAVES) table_part(hkv * G + g)[j] = 0.f;
@@ -310,7 +315,7 @@ __global__ __launch_bounds__(64 * SA_WAVES, DP == 128 ? 1 : 2) void seq_attn_dkv
       const int head = hkv * G + u / nqt;
       if (head != head_in) {       // (uniform)
         if (head_in >= 0) flush(head_in);      // (ends in a barrier: nobody reads the previous head's rows any more)
-        for (int i = tid; i < 2 * SA_WAVES * hn; i += 64 * SA_WAVES) ldsH[i] = 0.f;
+        for (int i = tid; i < SA_WAVES * hn; i += 64 * SA_WAVES) ldsH[i] = 0.f;
         sa_fill_bias(ldsB, p.rel, head, 1, tid);
         head_in = head;
       }
@@ -358,10 +363,20 @@ __global__ __launch_bounds__(64 * SA_WAVES, DP == 128 ? 1 : 2) void seq_attn_dkv
           for (int r = 0; r < 16; ++r) a += dp[r];
           if (far > 0) accR += a; else accL += a;
         } else {
-          const int d0 = key - qlo - 4 * h;
+          // row = query; diagonal of distance key - query = (key_w - qlo) + (column - row)
 #pragma unroll
-          for (int r = 0; r < 16; ++r)
-            __hip_atomic_fetch_add(myh + d0 - 8 * (r >> 2) - (r & 3), dp[r], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+          for (int r = 0; r < 16; ++r) diag[(8 * (r >> 2) + 4 * h + (r & 3)) * 64 + l31] = dp[r];
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+          float a = 0.f, c = 0.f;
+#pragma unroll
+          for (int k = 0; k < 32; k += 2) {      // column k + lane - 31 of row k
+            a += diag[k * 65 + lane - 31];
+            c += diag[(k + 1) * 65 + lane - 31];
+          }
+          if (lane < 63) myh[key_w - qlo + lane - 31] += a + c;
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
         }
       }
 #pragma unroll
@@ -438,7 +453,7 @@ static int sa_launch_bwd(K kernel, const SaBwdParams& p, long nwg, int lds, hipS
 }
 template <int DT, int DP, bool REL>
 static int sa_bwd_dp(const SaBwdParams& p, hipStream_t st) {
-  const int bias = REL ? (2 * p.rel.W + 1) * 4 : 0, hist = REL ? 2 * SA_WAVES * (2 * (p.rel.W + SA_REACH) + 1) * 4 : 0;
+  const int bias = REL ? (2 * p.rel.W + 1) * 4 : 0, hist = REL ? SA_WAVES * (2 * (p.rel.W + SA_REACH) + 1 + SA_DIAG) * 4 : 0;
   int rc = sa_launch_bwd(seq_attn_dq_kernel<DT, DP, REL>, p, (long)p.nrb * p.splits_q * p.H * p.B, 4 * SaTile<DP>::BYTES + bias, st);
   if (rc != DFOLD_OK) return rc;
   if (p.splits_q > 1) {

@@ -26,6 +26,7 @@ struct SaFwdParams {
 // Rescaling the accumulators costs as much as the rest of the softmax: the reference value of the exponents follows the running
 // maximum only when it has grown by more than this (P stays <= 2^8: exact in fp32 sums, harmless in 16-bit operands)
 #define SA_LAZY 8.f
+#define SA_MAX_SPLITS 1024
 
 template <int DT, int DP, bool REL>
 __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_fwd_kernel(const SaFwdParams p) {
@@ -253,6 +254,50 @@ __global__ __launch_bounds__(256) void seq_attn_combine_kernel(const SaFwdParams
   *(sa_u32x4*)(p.o + ((long)b * p.o_sb + (long)qi * p.o_sl + (long)head * p.o_sh + c * 8) * 2) = u;
 }
 
+// The same for many parts (a token over a long cache): one row per workgroup, its parts shared out over 256 / (D / 4) groups of lanes.
+// With one thread per chunk the loop over the parts is a chain of loads: 26 us for 47 parts of 544 rows, D = 64; here 5.
+template <int DT>
+__global__ __launch_bounds__(256) void seq_attn_combine_row_kernel(const SaFwdParams p) {
+  __shared__ float wgt[SA_MAX_SPLITS];
+  __shared__ f32x4 part[256];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const long nr = (long)p.B * p.Lq * p.H, r = blockIdx.x;
+  const float* const ls = p.ws + p.splits * nr * p.D + r;
+  // (every wave forms the maximum and the sum for itself)
+  float m = -INFINITY, l = 0.f;
+  for (int s = lane; s < p.splits; s += 64) m = fmaxf(m, ls[s * nr]);
+  m = wave_max(m);
+  const float mu = m == -INFINITY ? 0.f : m;
+  for (int s = lane; s < p.splits; s += 64) {
+    const float x = sa_exp2(ls[s * nr] - mu);
+    if (tid < 64) wgt[s] = x;
+    l += x;
+  }
+  l = wave_sum(l);
+  __syncthreads();
+  const int nc = p.D / 4, groups = 256 / nc, c = tid % nc, g = tid / nc;
+  f32x4 o = (f32x4){0.f, 0.f, 0.f, 0.f};
+  if (g < groups) {
+#pragma unroll 4
+    for (int s = g; s < p.splits; s += groups) {
+      const f32x4 a = *(const f32x4*)(p.ws + (s * nr + r) * p.D + c * 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[e] = __builtin_fmaf(wgt[s], a[e], o[e]);
+    }
+    part[tid] = o;
+  }
+  __syncthreads();
+  if (tid >= nc) return;
+  for (int k = 1; k < groups; ++k) o += part[k * nc + tid];
+  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  const int head = (int)(r % p.H);
+  const long bq = r / p.H;
+  const int qi = (int)(bq % p.Lq), b = (int)(bq / p.Lq);
+  if (p.lse && tid == 0) p.lse[((long)b * p.H + head) * p.Lq + qi] = l > 0.f || l != l ? m + __log2f(l) : INFINITY;
+  *(uint2*)(p.o + ((long)b * p.o_sb + (long)qi * p.o_sl + (long)head * p.o_sh + tid * 4) * 2) =
+      (uint2){sa_pack2<DT>(o[0] * inv, o[1] * inv), sa_pack2<DT>(o[2] * inv, o[3] * inv)};
+}
+
 template <int DT, int DP, bool REL>
 static int sa_launch_fwd(const SaFwdParams& p, unsigned nwg, hipStream_t st) {
   const int lds = 4 * SaTile<DP>::BYTES + (REL ? p.pack * (2 * p.rel.W + 1) * 4 : 0);
@@ -269,14 +314,18 @@ static int sa_fwd(const SaFwdParams& p, bool rel, unsigned nwg, hipStream_t st) 
   else if (p.D <= 64) rc = rel ? sa_launch_fwd<DT, 64, true>(p, nwg, st) : sa_launch_fwd<DT, 64, false>(p, nwg, st);
   else rc = rel ? sa_launch_fwd<DT, 128, true>(p, nwg, st) : sa_launch_fwd<DT, 128, false>(p, nwg, st);
   if (rc != DFOLD_OK || p.splits == 1) return rc;
-  const long n = (long)p.B * p.Lq * p.H * (p.D / 8);
+  const long rows = (long)p.B * p.Lq * p.H, n = rows * (p.D / 8);
+  if (p.splits >= 8 && rows <= 65536) {
+    DFOLD_LAUNCH(seq_attn_combine_row_kernel<DT>, dim3((unsigned)rows), dim3(256), 0, st, p);
+    return dfold_check_launch();
+  }
   DFOLD_LAUNCH(seq_attn_combine_kernel<DT>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, st, p);
   return dfold_check_launch();
 }
 
 extern "C" int dfold_seq_attn_fwd(const dfold_seq_attn_desc* d, void* stream) {
   SaFwdParams p;
-  if (!sa_desc_ok(d) || d->splits < 1 || d->splits > 4096 || (d->splits > 1 && !d->ws)) return DFOLD_EINVAL;
+  if (!sa_desc_ok(d) || d->splits < 1 || d->splits > SA_MAX_SPLITS || (d->splits > 1 && !d->ws)) return DFOLD_EINVAL;
   if (d->pack != 1 && d->pack != d->H / d->Hkv) return DFOLD_EINVAL;
   if (d->rel.table && !sa_make_rel(&d->rel, d->H, &p.rel)) return DFOLD_EINVAL;
   if (d->rel.table && (long)d->pack * (2 * p.rel.W + 1) * 4 > 32768) return DFOLD_EINVAL;

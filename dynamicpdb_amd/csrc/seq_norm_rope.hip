@@ -182,19 +182,21 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const NrParams p) {
   }
 }
 
-// dw[d] = sum of the blocks' sums, in a fixed order: 64 dimensions x 16 strided parts per workgroup
+// dw[d] = sum of the blocks' sums, in a fixed order: 16 dimensions x 64 strided parts per workgroup
 __global__ __launch_bounds__(1024) void qk_norm_rope_dw_kernel(const NrParams p) {
-  __shared__ double part[16][64];
+  __shared__ double part[64][16];
   const NrPart& q = p.part[blockIdx.y];
   if (!q.dw) return;
-  const int d = blockIdx.x * 64 + (threadIdx.x & 63), w = threadIdx.x >> 6;
+  const int d = blockIdx.x * 16 + (threadIdx.x & 15), w = threadIdx.x >> 4;
   double a = 0.;
   if (d < p.D)
-    for (int i = w; i < q.blocks; i += 16) a += (double)q.ws[(long)i * p.D + d];
-  part[w][threadIdx.x & 63] = a;
+#pragma unroll 8
+    for (int i = w; i < q.blocks; i += 64) a += (double)q.ws[(long)i * p.D + d];
+  part[w][threadIdx.x & 15] = a;
   __syncthreads();
   if (w == 0 && d < p.D) {
-    for (int k = 1; k < 16; ++k) a += part[k][threadIdx.x];
+#pragma unroll
+    for (int k = 1; k < 64; ++k) a += part[k][threadIdx.x];
     q.dw[d] = (float)a;
   }
 }
@@ -260,7 +262,7 @@ static int nr_run(const dfold_norm_rope_desc* d, bool bwd, void* stream) {
   else NR_LAUNCH(DFOLD_DT_F32);
   const int rc = dfold_check_launch();
   if (rc != DFOLD_OK || !dw) return rc;
-  DFOLD_LAUNCH(qk_norm_rope_dw_kernel, dim3((p.D + 63) / 64, 2), dim3(1024), 0, st, p);
+  DFOLD_LAUNCH(qk_norm_rope_dw_kernel, dim3((p.D + 15) / 16, 2), dim3(1024), 0, st, p);
   return dfold_check_launch();
 }
 extern "C" int dfold_qk_norm_rope_fwd(const dfold_norm_rope_desc* d, void* stream) { return nr_run(d, false, stream); }

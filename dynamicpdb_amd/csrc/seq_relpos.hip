@@ -2,9 +2,9 @@
 //
 // Bound by the one write (forward) or read (backward) of the matrix.  Forward: a workgroup holds its head's bias over the distances
 // -W .. W in LDS (beyond W it is constant) and writes 16-byte chunks of the head's matrix taken as one line; most chunks of a long
-// matrix are one constant.  Backward: a workgroup reads a run of whole rows, again as one line of 16-byte chunks; distances beyond W
-// go into two registers, the band in between is read along its diagonals, one distance per thread, so that no two threads add to
-// the same number: no atomics, and an order that does not change.
+// matrix are one constant.  Backward: a workgroup reads a run of whole rows; what lies beyond W goes into two registers, in 16-byte
+// chunks, a row per wave, four chunks in flight per lane; the band in between is read along its diagonals, one distance per thread, so
+// that no two threads add to the same number: no atomics, and an order that does not change.
 #include "seq_attn.h"
 #include "seq_dtable.h"
 
@@ -83,10 +83,40 @@ __global__ __launch_bounds__(256) void relpos_fwd_kernel(const SaMatParams p) {
   }
 }
 
+// a lane's share of the sum of row[a .. b): 16-byte chunks, single elements before the first and after the last 16-byte border
+template <int DT>
+__device__ __forceinline__ float line_sum(const typename SaElem<DT>::type* row, int a, int b, int lane) {
+  using E = typename SaElem<DT>::type;
+  constexpr int V = SaElem<DT>::VEC;
+  if (a >= b) return 0.f;
+  const int head = min((int)((-(long)(((uintptr_t)(row + a)) / sizeof(E))) & (V - 1)), b - a);
+  float s = 0.f;
+  if (lane < head) s = sa_to_f32<DT>(row[a + lane]);
+  a += head;
+  const int n = (b - a) / V;
+  if (lane < b - a - n * V) s += sa_to_f32<DT>(row[a + n * V + lane]);
+  const sa_u32x4* const c = (const sa_u32x4*)(row + a);
+  for (int k = lane; k < n; k += 256) {
+    sa_u32x4 x[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) x[u] = k + 64 * u < n ? c[k + 64 * u] : (sa_u32x4){0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      if constexpr (DT == DFOLD_DT_F32) {
+        const f32x4 y = __builtin_bit_cast(f32x4, x[u]);
+        s += (y[0] + y[1]) + (y[2] + y[3]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s += sa_lo<DT>(x[u][e]) + sa_hi<DT>(x[u][e]);
+      }
+    }
+  }
+  return s;
+}
+
 template <int DT>
 __global__ __launch_bounds__(256) void relpos_bwd_kernel(const SaMatParams p) {
   using E = typename SaElem<DT>::type;
-  constexpr int V = SaElem<DT>::VEC;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* const hist = (float*)smem;                 // [2 W + 1]
   __shared__ float side[2][4];
@@ -96,45 +126,13 @@ __global__ __launch_bounds__(256) void relpos_bwd_kernel(const SaMatParams p) {
   const E* const g = (const E*)p.g + head * n;
   float aL = 0.f, aR = 0.f;
   if (i0 < i1) {
-    // far distances: the rows as one line of aligned chunks
-    const long lo = (long)i0 * p.Lk, hi = (long)i1 * p.Lk, a = (head * n + lo) % V;
-    const long si = 256L * V / p.Lk, sj = 256L * V - si * p.Lk;
-    long e0 = lo - a + (long)tid * V, i = max(e0, lo) / p.Lk, j = e0 - i * p.Lk;     // (j < 0 where a run starts off a border)
-    auto next = [&]() {
-      e0 += 256L * V;
-      i += si;
-      j += sj;
-      if (j >= p.Lk) { j -= p.Lk; ++i; }
-      if (j < 0) { i = e0 / p.Lk; j = e0 - i * p.Lk; }
-    };
-    for (; e0 < hi; next()) {
-      const long d0 = j - i - off;
-      const bool right = d0 >= W, left = d0 + V - 1 <= -W;
-      if (e0 >= lo && e0 + V <= hi && j + V <= p.Lk) {
-        if (right || left) {
-          float s = 0.f;
-          if constexpr (DT == DFOLD_DT_F32) {
-            const f32x4 x = *(const f32x4*)(g + e0);
-            s = (x[0] + x[1]) + (x[2] + x[3]);
-          } else {
-            const sa_u32x4 x = *(const sa_u32x4*)(g + e0);
-#pragma unroll
-            for (int k = 0; k < 4; ++k) s += sa_lo<DT>(x[k]) + sa_hi<DT>(x[k]);
-          }
-          if (right) aR += s; else aL += s;
-          continue;
-        }
-        if (d0 + V - 1 < W && d0 > -W) continue;    // wholly inside the band
-      }
-      long jj = j, ii = i;                          // chunks over a border (of the run, of a row, of the band)
-      for (int e = 0; e < V; ++e) {
-        if (e0 + e >= lo && e0 + e < hi) {
-          const long d = jj - ii - off;
-          if (d >= W) aR += sa_to_f32<DT>(g[e0 + e]);
-          if (d <= -W) aL += sa_to_f32<DT>(g[e0 + e]);
-        }
-        if (++jj == p.Lk) { jj = 0; ++ii; }
-      }
+    // far distances: columns [0, jl) and [jr, Lk) of a row
+    for (int i = i0 + w; i < i1; i += 4) {
+      const long at = (long)i + off;
+      const int jl = (int)min(max(at - W + 1, 0L), (long)p.Lk), jr = (int)min(max(at + W, (long)jl), (long)p.Lk);
+      const E* const row = g + (long)i * p.Lk;
+      aL += line_sum<DT>(row, 0, jl, lane);
+      aR += line_sum<DT>(row, jr, p.Lk, lane);
     }
     // the band: distance d of every row of the run
     for (int d = tid - (W - 1); d <= W - 1; d += 256) {
@@ -142,7 +140,7 @@ __global__ __launch_bounds__(256) void relpos_bwd_kernel(const SaMatParams p) {
       const long s = (long)off + d;
       const int ilo = (int)min(max((long)i0, -s), (long)i1), ihi = (int)max(min((long)i1, p.Lk - s), (long)ilo);
       float acc = 0.f;
-#pragma unroll 8
+#pragma unroll 16
       for (int i = ilo; i < ihi; ++i) acc += sa_to_f32<DT>(g[(long)i * p.Lk + i + s]);
       hist[W + d] = acc;
     }
@@ -158,9 +156,9 @@ __global__ __launch_bounds__(256) void relpos_bwd_kernel(const SaMatParams p) {
   sa_bucket_sums(p.rel, hist, W, p.nb, p.ws + ((long)head * p.nblk + blockIdx.x) * p.nb, w, lane);
 }
 
-// row blocks of the backward: about four workgroups per CU
+// row blocks of the backward: about eight workgroups per CU
 static inline int sa_mat_blocks(int H, int Lq) {
-  const int want = 1024 / H > 1 ? 1024 / H : 1;
+  const int want = 2048 / H > 1 ? 2048 / H : 1;
   return Lq < want ? Lq : want;
 }
 extern "C" int dfold_relpos_ws(int32_t H, int32_t Lq, int32_t num_buckets) {

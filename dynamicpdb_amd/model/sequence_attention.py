@@ -10,11 +10,11 @@ on the matrix pipes with fp32 softmax statistics and accumulators, results indep
 
 Device tensors only (no CPU fallback).  Nothing is kept between calls; workspaces come from torch's allocator, so the calls may be
 recorded into a graph and run on any stream or device (the device of the tensors, its current stream)."""
-import contextlib
 import ctypes
 import functools
 import math
-from ctypes import Structure, byref, c_double, c_float, c_int16, c_int32, c_int64, c_void_p
+import struct
+from ctypes import c_double, c_float, c_int16, c_int32, c_int64, c_void_p
 
 import torch
 import torch.nn as nn
@@ -22,49 +22,68 @@ from torch.autograd import Function
 from torch.autograd.function import once_differentiable
 
 from .. import _lib, ops
-from .._lib import check, stream
+from .._lib import check
 from ..ops import BF16
 from .functional import linear
 
-DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}      # DFOLD_DT_*
+F16, F32 = torch.float16, torch.float32
+DTYPES = {BF16: 0, F16: 1, F32: 2}                                    # DFOLD_DT_*
 REL_FAR, REL_MAX_DISTANCE = 256, 1024                                 # DFOLD_REL_*
-MAX_OFFSET = 1 << 29
+MAX_OFFSET, MAX_LEN = 1 << 29, 1 << 30
 ROWS, TILE = 128, 64                                                  # softmax rows / keys of a workgroup, rows of an LDS tile
 
+# The C ABI's descriptors as struct formats: one pack per call (filling ctypes structures field by field costs as much host time as the
+# launch).  The classes give names to the same layouts.
 
-class _RelBias(Structure):
+
+class RelBias(ctypes.Structure):
     _fields_ = [("table", c_void_p), ("q_offsets", c_void_p), ("q_offset", c_int32), ("num_buckets", c_int32), ("bidirectional", c_int32),
                 ("reserved", c_int32), ("far_border", c_int16 * REL_FAR)]
 
 
-class _AttnDesc(Structure):
+class AttnDesc(ctypes.Structure):
     _fields_ = ([(n, c_void_p) for n in ("q", "k", "v", "o", "lse", "ws", "key_mask", "kv_lens")] +
                 [(n, c_int64) for n in ("q_sb", "q_sl", "q_sh", "k_sb", "k_sl", "k_sh", "v_sb", "v_sl", "v_sh", "o_sb", "o_sl", "o_sh", "mask_sb")] +
-                [(n, c_int32) for n in ("dtype", "B", "Lq", "Lk", "H", "Hkv", "D", "splits", "pack")] + [("scale", c_float), ("rel", _RelBias)])
+                [(n, c_int32) for n in ("dtype", "B", "Lq", "Lk", "H", "Hkv", "D", "splits", "pack")] + [("scale", c_float), ("rel", RelBias)])
 
 
-class _AttnGrad(Structure):
+class AttnGrad(ctypes.Structure):
     _fields_ = [("d_o", c_void_p), ("do_sb", c_int64), ("do_sl", c_int64), ("do_sh", c_int64), ("dq", c_void_p), ("dk", c_void_p),
                 ("dv", c_void_p), ("delta", c_void_p), ("dtable", c_void_p), ("ws", c_void_p), ("splits_q", c_int32), ("splits_k", c_int32)]
 
 
-class _RopePart(Structure):
+class RopePart(ctypes.Structure):
     _fields_ = ([(n, c_void_p) for n in ("x", "y", "g", "w", "dw", "pos")] +
                 [(n, c_int64) for n in ("x_sb", "x_sl", "x_sh", "g_sb", "g_sl", "g_sh", "pos_sb")] + [("L", c_int32), ("H", c_int32)])
 
 
-class _RopeDesc(Structure):
-    _fields_ = [("part", _RopePart * 2), ("ws", c_void_p), ("base", c_double), ("eps", c_float), ("dtype", c_int32), ("B", c_int32),
+class RopeDesc(ctypes.Structure):
+    _fields_ = [("part", RopePart * 2), ("ws", c_void_p), ("base", c_double), ("eps", c_float), ("dtype", c_int32), ("B", c_int32),
                 ("D", c_int32), ("rotary_dim", c_int32), ("interleaved", c_int32)]
+
+
+_REL = struct.Struct(f"@2P4i{2 * REL_FAR}s")
+_ATTN = struct.Struct("@8P13q9if")
+_GRAD = struct.Struct("@P3q6P2i")
+_PART = struct.Struct("@6P7q2i")
+_ROPE = struct.Struct("@Pdf5i")
+_NO_REL = bytes(_REL.size)
+_NO_PART = bytes(_PART.size)
 
 
 # ------------------------------------------------------------------------------------------------
 # argument helpers
 # ------------------------------------------------------------------------------------------------
 
-def _need(cond, msg):
-    if not cond:
-        raise ValueError(msg)
+def _call(name, *args, t):
+    """one C ABI call on the current stream of t's device.  Arguments: a descriptor's bytes, pointers as c_void_p, whole numbers."""
+    dev = t.get_device()
+    fn = getattr(_lib.lib(), name)
+    if dev == torch.cuda.current_device():
+        check(fn(*args, c_void_p(torch._C._cuda_getCurrentRawStream(dev))), name)
+    else:                                       # (launches go to the current device)
+        with torch.cuda.device(dev):
+            check(fn(*args, c_void_p(torch._C._cuda_getCurrentRawStream(dev))), name)
 
 
 def _require_cuda(t):
@@ -72,33 +91,32 @@ def _require_cuda(t):
         raise RuntimeError("dynamicpdb_amd sequence operators need an MI355X device tensor (no CPU fallback)")
 
 
-def _same_device(ref, **others):
-    for name, t in others.items():
-        _need(t is None or t.device == ref.device, f"{name} is on {t.device if t is not None else None}, expected {ref.device}")
-
-
-def _on(t):
-    """the launches of a call go to the device its tensors live on, whatever the current device is"""
-    return contextlib.nullcontext() if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def _same_device(dev, name, t):
+    if t is not None and t.device != dev:
+        raise ValueError(f"{name} is on {t.device}, expected {dev}")
 
 
 def _rows16(t):
     """t itself if the kernels can read it as it lies -- dense last axis, every other stride a multiple of 16 bytes, aligned base --
     else a dense copy"""
+    aligned = t.data_ptr() % 16 == 0
+    if aligned and t.is_contiguous():           # (a multiple of 16 bytes per row: the head size is checked)
+        return t
     v = 16 // t.element_size()
-    if t.numel() == 0 or (t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and
-                          all(s % v == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)):
+    if t.numel() == 0 or (aligned and t.stride(-1) == 1 and all(s % v == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
 
 def _strides(t):
-    """strides of the leading axes, 0 for axes of one entry (theirs may be anything)"""
-    return [s if n > 1 else 0 for s, n in zip(t.stride()[:-1], t.shape[:-1])]
+    """strides of the three leading axes, 0 for axes of one entry (theirs may be anything)"""
+    a, b, c, _ = t.stride()
+    n = t.shape
+    return (a if n[0] > 1 else 0, b if n[1] > 1 else 0, c if n[2] > 1 else 0)
 
 
 def _addr(t):
-    return None if t is None else t.data_ptr()
+    return 0 if t is None else t.data_ptr()
 
 
 def _mask_bytes(mask):
@@ -128,65 +146,71 @@ def far_borders(num_buckets, max_distance, bidirectional):
 
 
 @functools.lru_cache(maxsize=None)
-def _border_array(num_buckets, max_distance, bidirectional):
-    b = far_borders(num_buckets, max_distance, bidirectional)
-    return (c_int16 * REL_FAR)(*b)
+def _border_bytes(num_buckets, max_distance, bidirectional):
+    far = far_borders(num_buckets, max_distance, bidirectional)
+    return struct.pack(f"@{REL_FAR}h", *far, *([0] * (REL_FAR - len(far))))
+
+
+def _reach(num_buckets, max_distance, bidirectional):
+    """distance from which on a side's last bucket holds everything"""
+    far = far_borders(num_buckets, max_distance, bidirectional)
+    return far[-1] if far else (num_buckets // 2 if bidirectional else num_buckets) // 2
 
 
 def _check_rel(table, max_distance, bidirectional):
-    _need(table.dim() == 2 and table.dtype == torch.float32, "the bias table must be fp32 [num_buckets, heads]")
+    if table.dim() != 2 or table.dtype != F32:
+        raise ValueError("the bias table must be fp32 [num_buckets, heads]")
     nb = table.shape[0]
     half = nb // 2 if bidirectional else nb
-    _need(not bidirectional or nb % 2 == 0, "num_buckets must be even for a bidirectional bias")
-    _need(half >= 2 and half <= REL_FAR, f"num_buckets must be between 2 and {REL_FAR} per direction")
-    _need(isinstance(max_distance, int) and half // 2 < max_distance <= REL_MAX_DISTANCE,
-          f"max_distance must be a whole number above num_buckets' single distances ({half // 2}) and at most {REL_MAX_DISTANCE}")
+    if bidirectional and nb % 2:
+        raise ValueError("num_buckets must be even for a bidirectional bias")
+    if not 2 <= half <= REL_FAR:
+        raise ValueError(f"num_buckets must be between 2 and {REL_FAR} per direction")
+    if not isinstance(max_distance, int) or not half // 2 < max_distance <= REL_MAX_DISTANCE:
+        raise ValueError(f"max_distance must be a whole number above num_buckets' single distances ({half // 2}) and at most {REL_MAX_DISTANCE}")
 
 
-def _fill_rel(rel, table, max_distance, bidirectional, q_offset, q_offsets=None):
-    rel.table, rel.q_offsets, rel.q_offset = table.data_ptr(), _addr(q_offsets), q_offset
-    rel.num_buckets, rel.bidirectional = table.shape[0], int(bidirectional)
-    ctypes.memmove(rel.far_border, _border_array(table.shape[0], max_distance, bool(bidirectional)), 2 * REL_FAR)
+def _rel_desc(table, num_buckets, max_distance, bidirectional, q_offset, q_offsets=None):
+    return _REL.pack(table.data_ptr(), _addr(q_offsets), q_offset, num_buckets, bidirectional, 0, _border_bytes(num_buckets, max_distance, bidirectional))
 
 
 # ------------------------------------------------------------------------------------------------
 # relative position bias as a matrix
 # ------------------------------------------------------------------------------------------------
 
+def _bias_forward(table, q_len, k_len, max_distance, bidirectional, q_offset, dtype):
+    t = table if table.is_contiguous() else table.contiguous()
+    nb, H = t.shape
+    out = torch.empty((H, q_len, k_len), dtype=dtype, device=t.device)
+    if q_len and k_len:
+        _call("dfold_relpos_fwd", _rel_desc(t, nb, max_distance, bidirectional, q_offset), c_void_p(out.data_ptr()), DTYPES[dtype], H, q_len, k_len, t=t)
+    return out
+
+
 class RelativeBiasFn(Function):
     @staticmethod
-    def forward(ctx, table, q_len, k_len, max_distance, bidirectional, q_offset, dtype):
-        t = table.detach().contiguous()
-        H = t.shape[1]
-        ctx.args = (q_len, k_len, max_distance, bidirectional, q_offset, dtype, t.shape)
-        out = torch.empty((H, q_len, k_len), dtype=dtype, device=t.device)
-        if out.numel():
-            rel = _RelBias()
-            _fill_rel(rel, t, max_distance, bidirectional, q_offset)
-            with _on(t):
-                check(_lib.lib().dfold_relpos_fwd(byref(rel), c_void_p(out.data_ptr()), c_int32(DTYPES[dtype]), c_int32(H), c_int32(q_len),
-                                                  c_int32(k_len), stream()), "dfold_relpos_fwd")
-        return out
+    def forward(ctx, table, *args):
+        ctx.args, ctx.table_shape = args, table.shape
+        return _bias_forward(table, *args)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
-        q_len, k_len, max_distance, bidirectional, q_offset, dtype, shape = ctx.args
-        nb, H = shape
+        q_len, k_len, max_distance, bidirectional, q_offset, dtype = ctx.args
+        nb, H = ctx.table_shape
+        dev = g.device
         if g.numel() == 0:
-            return (torch.zeros(shape, dtype=torch.float32, device=g.device),) + (None,) * 6
+            return (torch.zeros((nb, H), dtype=F32, device=dev),) + (None,) * 6
         if not g.is_contiguous() or g.data_ptr() % 16:
             g = g.clone(memory_format=torch.contiguous_format)
-        dtable = torch.empty(shape, dtype=torch.float32, device=g.device)
-        with _on(g):
-            L = _lib.lib()
-            n = L.dfold_relpos_ws(c_int32(H), c_int32(q_len), c_int32(nb))
-            _need(n > 0, "relative_position_bias: too many heads x buckets")
-            ws = torch.empty(n, dtype=torch.float32, device=g.device)
-            rel = _RelBias()
-            _fill_rel(rel, dtable, max_distance, bidirectional, q_offset)      # (the backward reads the borders, not the entries)
-            check(L.dfold_relpos_bwd(byref(rel), c_void_p(g.data_ptr()), c_int32(DTYPES[dtype]), c_int32(H), c_int32(q_len), c_int32(k_len),
-                                     c_void_p(dtable.data_ptr()), c_void_p(ws.data_ptr()), stream()), "dfold_relpos_bwd")
+        dtable = torch.empty((nb, H), dtype=F32, device=dev)
+        n = _lib.lib().dfold_relpos_ws(H, q_len, nb)
+        if n <= 0:
+            raise ValueError("relative_position_bias: too many heads x buckets")
+        ws = torch.empty(n, dtype=F32, device=dev)
+        # (the backward reads the borders, not the entries)
+        _call("dfold_relpos_bwd", _rel_desc(dtable, nb, max_distance, bidirectional, q_offset), c_void_p(g.data_ptr()), DTYPES[dtype], H, q_len, k_len,
+              c_void_p(dtable.data_ptr()), c_void_p(ws.data_ptr()), t=g)
         return (dtable,) + (None,) * 6
 
 
@@ -197,12 +221,19 @@ def relative_position_bias(table, q_len, k_len, *, max_distance=128, bidirection
     half; else half = num_buckets and keys behind the query count as distance 0) the first half // 2 hold one distance each, the others
     grow logarithmically up to max_distance, beyond which everything shares the last.  dtype: fp32, bf16 or fp16 of the result."""
     _check_rel(table, max_distance, bidirectional)
-    _need(isinstance(q_len, int) and isinstance(k_len, int) and 0 <= q_len <= 1 << 30 and 0 <= k_len <= 1 << 30, "q_len, k_len must be whole numbers >= 0")
-    _need(isinstance(q_offset, int) and abs(q_offset) <= MAX_OFFSET, f"q_offset must be a whole number, at most {MAX_OFFSET}")
-    _need(dtype in DTYPES, "dtype must be float32, bfloat16 or float16")
-    _need(1 <= table.shape[1] <= 65535, "the table needs between 1 and 65535 heads")
+    if not (isinstance(q_len, int) and isinstance(k_len, int) and 0 <= q_len <= MAX_LEN and 0 <= k_len <= MAX_LEN):
+        raise ValueError("q_len, k_len must be whole numbers >= 0")
+    if not isinstance(q_offset, int) or abs(q_offset) > MAX_OFFSET:
+        raise ValueError(f"q_offset must be a whole number, at most {MAX_OFFSET}")
+    if dtype not in DTYPES:
+        raise ValueError("dtype must be float32, bfloat16 or float16")
+    if not 1 <= table.shape[1] <= 65535:
+        raise ValueError("the table needs between 1 and 65535 heads")
     _require_cuda(table)
-    return RelativeBiasFn.apply(table, q_len, k_len, max_distance, bool(bidirectional), q_offset, dtype)
+    args = (table, q_len, k_len, max_distance, bool(bidirectional), q_offset, dtype)
+    if table.requires_grad and torch.is_grad_enabled():
+        return RelativeBiasFn.apply(*args)
+    return _bias_forward(*args)
 
 
 class RelativePositionBias(nn.Module):
@@ -224,74 +255,74 @@ class RelativePositionBias(nn.Module):
 # norm + rotation of query and key heads
 # ------------------------------------------------------------------------------------------------
 
+def _rope_part(x, y, w, pos, g=None, dw=None):
+    if x is None or x.numel() == 0:
+        return _NO_PART
+    pos_sb = 0 if pos is None or pos.shape[0] == 1 else pos.stride(0)
+    return _PART.pack(x.data_ptr(), y.data_ptr(), _addr(g), _addr(w), _addr(dw), _addr(pos), *_strides(x), *(_strides(g) if g is not None else (0, 0, 0)),
+                      pos_sb, x.shape[1], x.shape[2])
+
+
+def _rope_desc(parts, ref, opts, ws=None):
+    rotary_dim, base, interleaved, eps = opts
+    return parts[0] + parts[1] + _ROPE.pack(_addr(ws), base, eps, DTYPES[ref.dtype], ref.shape[0], ref.shape[3], rotary_dim, interleaved)
+
+
+def _rope_forward(q, k, w_q, w_k, q_pos, k_pos, *opts):
+    """results and the (readable) inputs they were computed from"""
+    q, k = (None if t is None else _rows16(t) for t in (q, k))
+    w_q, w_k = (None if t is None else t.contiguous() for t in (w_q, w_k))
+    oq, ok = (None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
+    parts = _rope_part(q, oq, w_q, q_pos), _rope_part(k, ok, w_k, k_pos)
+    if parts != (_NO_PART, _NO_PART):
+        ref = q if q is not None else k
+        _call("dfold_qk_norm_rope_fwd", _rope_desc(parts, ref, opts), t=ref)
+    return oq, ok, (q, k, w_q, w_k, q_pos, k_pos)
+
+
 class QKNormRopeFn(Function):
     @staticmethod
-    def forward(ctx, q, k, w_q, w_k, q_pos, k_pos, rotary_dim, base, interleaved, eps):
-        q, k = (None if t is None else _rows16(t.detach()) for t in (q, k))
-        w_q, w_k = (None if t is None else t.detach().contiguous() for t in (w_q, w_k))
-        ctx.opts = (rotary_dim, base, interleaved, eps)
-        ctx.save_for_backward(q, k, w_q, w_k, q_pos, k_pos)
-        outs = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k)]
-        d = QKNormRopeFn._desc(ctx.opts, (q, k), outs, (w_q, w_k), (q_pos, k_pos))
-        if d is not None:
-            with _on(outs[0] if outs[0] is not None else outs[1]):
-                check(_lib.lib().dfold_qk_norm_rope_fwd(byref(d), stream()), "dfold_qk_norm_rope_fwd")
-        return tuple(outs)
-
-    @staticmethod
-    def _desc(opts, xs, ys, ws, poss, gs=(None, None)):
-        d = _RopeDesc()
-        d.rotary_dim, d.base, d.interleaved, d.eps = opts[0], opts[1], int(opts[2]), opts[3]
-        any_part = False
-        for part, x, y, w, pos, g in zip(d.part, xs, ys, ws, poss, gs):
-            if x is None or x.numel() == 0:
-                continue
-            any_part = True
-            d.dtype, d.B, d.D = DTYPES[x.dtype], x.shape[0], x.shape[3]
-            part.x, part.y, part.w, part.pos = _addr(x), _addr(y), _addr(w), _addr(pos)
-            part.x_sb, part.x_sl, part.x_sh = _strides(x)
-            part.L, part.H = x.shape[1], x.shape[2]
-            if pos is not None:
-                part.pos_sb = pos.stride(0) if pos.shape[0] > 1 else 0
-            if g is not None:
-                part.g = _addr(g)
-                part.g_sb, part.g_sl, part.g_sh = _strides(g)
-        return d if any_part else None
+    def forward(ctx, *args):
+        oq, ok, saved = _rope_forward(*args)
+        ctx.opts = args[6:]
+        ctx.save_for_backward(*saved)
+        return oq, ok
 
     @staticmethod
     @once_differentiable
     def backward(ctx, gq, gk):
         q, k, w_q, w_k, q_pos, k_pos = ctx.saved_tensors
-        gs = [None if x is None else _rows16(g) for x, g in ((q, gq), (k, gk))]
-        dxs = [None if x is None else torch.empty(x.shape, dtype=x.dtype, device=x.device) for x in (q, k)]
         ref = q if q is not None else k
-        dws = [None, None]
-        d = QKNormRopeFn._desc(ctx.opts, (q, k), dxs, (w_q, w_k), (q_pos, k_pos), gs)
-        with _on(ref):
-            L = _lib.lib()
-            for i, (x, w) in enumerate(((q, w_q), (k, w_k))):
-                if w is not None and ctx.needs_input_grad[2 + i]:
-                    empty = x is None or x.numel() == 0
-                    dws[i] = (torch.zeros if empty else torch.empty)(w.shape, dtype=torch.float32, device=w.device)
-                    if not empty:
-                        d.part[i].dw = dws[i].data_ptr()
-            if d is not None:
-                if dws[0] is not None or dws[1] is not None:
-                    ws = torch.empty(L.dfold_qk_norm_rope_ws(), dtype=torch.float32, device=ref.device)
-                    d.ws = ws.data_ptr()
-                check(L.dfold_qk_norm_rope_bwd(byref(d), stream()), "dfold_qk_norm_rope_bwd")
-        return dxs[0], dxs[1], dws[0], dws[1], None, None, None, None, None, None
+        grads, parts, ws = [None] * 4, [], None
+        for i, (x, w, pos, g) in enumerate(((q, w_q, q_pos, gq), (k, w_k, k_pos, gk))):
+            if x is None:
+                parts.append(_NO_PART)
+                continue
+            dx = grads[i] = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            dw = None
+            if w is not None and ctx.needs_input_grad[2 + i]:
+                dw = grads[2 + i] = torch.empty(w.shape, dtype=F32, device=w.device) if x.numel() else torch.zeros(w.shape, dtype=F32, device=w.device)
+                if ws is None:
+                    ws = torch.empty(_lib.lib().dfold_qk_norm_rope_ws(), dtype=F32, device=ref.device)
+            parts.append(_rope_part(x, dx, w, pos, _rows16(g), dw))
+        if parts != [_NO_PART, _NO_PART]:
+            _call("dfold_qk_norm_rope_bwd", _rope_desc(parts, ref, ctx.opts, ws), t=ref)
+        return (*grads, None, None, None, None, None, None)
 
 
 def _positions(pos, x, name):
     if pos is None or x is None:
         return None
-    _need(pos.dtype in (torch.int64, torch.int32), f"{name} must be int64 or int32")
+    _same_device(x.device, name, pos)
+    if pos.dtype != torch.int64:
+        if pos.dtype != torch.int32:
+            raise ValueError(f"{name} must be int64 or int32")
+        pos = pos.long()
     if pos.dim() == 1:
         pos = pos[None]
-    _need(pos.dim() == 2 and pos.shape[0] in (1, x.shape[0]) and pos.shape[1] == x.shape[1], f"{name} must be [{x.shape[1]}] or [{x.shape[0]}, {x.shape[1]}]")
-    pos = pos.long()
-    return pos if pos.shape[1] <= 1 or pos.stride(1) == 1 else pos.contiguous()
+    if pos.dim() != 2 or pos.shape[0] not in (1, x.shape[0]) or pos.shape[1] != x.shape[1]:
+        raise ValueError(f"{name} must be [{x.shape[1]}] or [{x.shape[0]}, {x.shape[1]}]")
+    return pos if pos.stride(1) == 1 or pos.shape[1] <= 1 else pos.contiguous()
 
 
 def qk_norm_rope(q, k, w_q=None, w_k=None, q_positions=None, k_positions=None, *, rotary_dim=None, base=10000.0, interleaved=False, eps=1e-6):
@@ -299,25 +330,41 @@ def qk_norm_rope(q, k, w_q=None, w_k=None, q_positions=None, k_positions=None, *
     rotary_dim dimensions (default: all; a multiple of 16; 0: none) rotated by position * base^(-2 i / rotary_dim): pairs
     (i, i + rotary_dim / 2), or (2 i, 2 i + 1) if interleaved.  k may be None (keys that are rotated already).  Positions: int64 / int32
     [L] or [B, L], default 0, 1, ...; any size (angles are reduced in fp64).  bf16, fp16 or fp32; one launch for q and k; differentiable
-    in q, k, w_q, w_k."""
+    (once) in q, k, w_q, w_k."""
     ref = q if q is not None else k
-    _need(ref is not None, "qk_norm_rope needs q or k")
-    _same_device(ref, q=q, k=k, w_q=w_q, w_k=w_k, q_positions=q_positions, k_positions=k_positions)
-    _need(ref.dtype in DTYPES, "q, k must be bfloat16, float16 or float32")
+    if ref is None:
+        raise ValueError("qk_norm_rope needs q or k")
+    if ref.dtype not in DTYPES:
+        raise ValueError("q, k must be bfloat16, float16 or float32")
     for name, t in (("q", q), ("k", k)):
-        _need(t is None or (t.dim() == 4 and t.dtype == ref.dtype), f"{name} must be [B, L, heads, D], q and k of one type")
-    _need(q is None or k is None or (q.shape[0] == k.shape[0] and q.shape[3] == k.shape[3]), "q and k differ in batch or head size")
-    D = ref.shape[3]
-    _need(D % 8 == 0 and 8 <= D <= 256, "the head size must be a multiple of 8, at most 256")
-    rd = (D // 16 * 16 if D % 16 else D) if rotary_dim is None else rotary_dim
-    _need(rotary_dim is not None or rd == D, "this head size is not a multiple of 16: give rotary_dim")
-    _need(isinstance(rd, int) and 0 <= rd <= D and rd % 16 == 0, "rotary_dim must be a multiple of 16, at most the head size")
-    _need(base > 0 and math.isfinite(base) and eps >= 0, "base must be positive and eps not negative")
+        if t is not None and (t.dim() != 4 or t.dtype != ref.dtype):
+            raise ValueError(f"{name} must be [B, L, heads, D], q and k of one type")
+    D, dev = ref.shape[3], ref.device
+    if q is not None and k is not None:
+        _same_device(dev, "k", k)
+        if q.shape[0] != k.shape[0] or k.shape[3] != D:
+            raise ValueError("q and k differ in batch or head size")
+    if D % 8 or not 8 <= D <= 256:
+        raise ValueError("the head size must be a multiple of 8, at most 256")
+    if rotary_dim is None:
+        if D % 16:
+            raise ValueError("this head size is not a multiple of 16: give rotary_dim")
+        rotary_dim = D
+    if not isinstance(rotary_dim, int) or not 0 <= rotary_dim <= D or rotary_dim % 16:
+        raise ValueError("rotary_dim must be a multiple of 16, at most the head size")
+    if not (base > 0 and math.isfinite(base) and eps >= 0):
+        raise ValueError("base must be positive and eps not negative")
     for name, w in (("w_q", w_q), ("w_k", w_k)):
-        _need(w is None or (w.dtype == torch.float32 and w.shape == (D,)), f"{name} must be fp32 [{D}]")
+        if w is not None:
+            _same_device(dev, name, w)
+            if w.dtype != F32 or w.dim() != 1 or w.shape[0] != D:
+                raise ValueError(f"{name} must be fp32 [{D}]")
     q_positions, k_positions = _positions(q_positions, q, "q_positions"), _positions(k_positions, k, "k_positions")
     _require_cuda(ref)
-    return QKNormRopeFn.apply(q, k, w_q, w_k, q_positions, k_positions, rd, float(base), bool(interleaved), float(eps))
+    args = (q, k, w_q, w_k, q_positions, k_positions, rotary_dim, float(base), bool(interleaved), float(eps))
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+        return QKNormRopeFn.apply(*args)
+    return _rope_forward(*args)[:2]
 
 
 # ------------------------------------------------------------------------------------------------
@@ -327,7 +374,7 @@ def qk_norm_rope(q, k, w_q=None, w_k=None, q_positions=None, k_positions=None, *
 def _parts(groups, units, n_cu, least):
     """Cut factor of a launch of `groups` workgroups that each walk `units` tiles: as many parts as bring the launch to two workgroups
     per CU, each of at least `least` tiles (below that, writing and adding the parts costs more than the idle CUs)."""
-    return max(1, min(2 * n_cu // max(groups, 1), units // least))
+    return max(1, min(1024, 2 * n_cu // max(groups, 1), units // least))
 
 
 def _attn_plan(B, Lq, Lk, H, Hkv, rel_width, n_cu):
@@ -340,92 +387,72 @@ def _attn_plan(B, Lq, Lk, H, Hkv, rel_width, n_cu):
     return pack, _parts(groups, -(-Lk // TILE), n_cu, 2)
 
 
+def _attn_desc(q, k, v, o, lse, ws, key_mask, kv_lens, rel, scale, pack=1, splits=1):
+    B, Lq, H, D = q.shape
+    mask_sb = 0 if key_mask is None or B == 1 else key_mask.stride(0)
+    return _ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _addr(lse), _addr(ws), _addr(key_mask), _addr(kv_lens), *_strides(q),
+                      *_strides(k), *_strides(v), *_strides(o), mask_sb, DTYPES[q.dtype], B, Lq, k.shape[1], H, k.shape[2], D, splits, pack, scale) + rel
+
+
+def _attn_forward(train, q, k, v, table, key_mask, kv_lens, q_offsets, q_offset, max_distance, bidirectional, scale):
+    """the result and what a backward pass needs"""
+    q, k, v = _rows16(q), _rows16(k), _rows16(v)
+    B, Lq, H, D = q.shape
+    Lk, Hkv = k.shape[1], k.shape[2]
+    dev = q.device
+    o = torch.empty((B, Lq, H, D), dtype=q.dtype, device=dev)
+    lse = torch.empty((B, H, Lq), dtype=F32, device=dev) if train else None
+    if table is not None and not table.is_contiguous():
+        table = table.contiguous()
+    if B and Lq:
+        rel, width = _NO_REL, 0
+        if table is not None:
+            nb = table.shape[0]
+            rel = _rel_desc(table, nb, max_distance, bidirectional, q_offset, q_offsets)
+            width = 2 * _reach(nb, max_distance, bidirectional) + 1
+        pack, splits = _attn_plan(B, Lq, Lk, H, Hkv, width, ops.cu_count(dev))
+        ws = torch.empty(splits * B * H * Lq * (D + 1), dtype=F32, device=dev) if splits > 1 else None
+        _call("dfold_seq_attn_fwd", _attn_desc(q, k, v, o, lse, ws, key_mask, kv_lens, rel, scale, pack, splits), t=q)
+    return o, (q, k, v, table, key_mask, kv_lens, q_offsets, o, lse)
+
+
 class CrossAttentionFn(Function):
     @staticmethod
-    def forward(ctx, q, k, v, table, key_mask, kv_lens, q_offsets, q_offset, max_distance, bidirectional, scale, train):
-        q, k, v = (_rows16(t.detach()) for t in (q, k, v))
-        B, Lq, H, D = q.shape
-        Lk, Hkv = k.shape[1], k.shape[2]
-        dev = q.device
-        if table is not None:
-            table = table.detach().contiguous()
-        o = torch.empty((B, Lq, H, D), dtype=q.dtype, device=dev)
-        lse = torch.empty((B, H, Lq), dtype=torch.float32, device=dev) if train else None
-        ctx.opts = (q_offset, max_distance, bidirectional, scale)
-        ctx.save_for_backward(q, k, v, table, key_mask, kv_lens, q_offsets, o, lse)
-        if o.numel():
-            d = CrossAttentionFn._desc(ctx.opts, q, k, v, table, key_mask, kv_lens, q_offsets, o, lse)
-            width = 0
-            if table is not None:
-                nb = table.shape[0]
-                far = far_borders(nb, max_distance, bidirectional)
-                width = 2 * (far[-1] if far else (nb // 2 if bidirectional else nb) // 2) + 1
-            with _on(q):
-                d.pack, d.splits = _attn_plan(B, Lq, Lk, H, Hkv, width, ops.cu_count(dev))
-                if d.splits > 1:
-                    ws = torch.empty(d.splits * B * H * Lq * (D + 1), dtype=torch.float32, device=dev)
-                    d.ws = ws.data_ptr()
-                check(_lib.lib().dfold_seq_attn_fwd(byref(d), stream()), "dfold_seq_attn_fwd")
+    def forward(ctx, *args):
+        o, saved = _attn_forward(True, *args)
+        ctx.opts = args[7:]
+        ctx.save_for_backward(*saved)
         return o
-
-    @staticmethod
-    def _desc(opts, q, k, v, table, key_mask, kv_lens, q_offsets, o, lse):
-        q_offset, max_distance, bidirectional, scale = opts
-        d = _AttnDesc()
-        d.q, d.k, d.v, d.o, d.lse = (_addr(t) for t in (q, k, v, o, lse))
-        d.key_mask, d.kv_lens = _addr(key_mask), _addr(kv_lens)
-        d.q_sb, d.q_sl, d.q_sh = _strides(q)
-        d.k_sb, d.k_sl, d.k_sh = _strides(k)
-        d.v_sb, d.v_sl, d.v_sh = _strides(v)
-        d.o_sb, d.o_sl, d.o_sh = _strides(o)
-        if key_mask is not None:
-            d.mask_sb = key_mask.stride(0) if key_mask.shape[0] > 1 else 0
-        d.dtype, d.scale = DTYPES[q.dtype], scale
-        d.B, d.Lq, d.H, d.D = q.shape
-        d.Lk, d.Hkv = k.shape[1], k.shape[2]
-        if table is not None:
-            _fill_rel(d.rel, table, max_distance, bidirectional, q_offset, q_offsets)
-        return d
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g):
         q, k, v, table, key_mask, kv_lens, q_offsets, o, lse = ctx.saved_tensors
+        q_offset, max_distance, bidirectional, scale = ctx.opts
         B, Lq, H, D = q.shape
         Lk, Hkv = k.shape[1], k.shape[2]
-        dev = q.device
-        dq, dk, dv = (torch.empty(t.shape, dtype=t.dtype, device=dev) for t in (q, k, v))
-        dtable = None
-        if o.numel() == 0 or k.numel() == 0:
-            for t in (dq, dk, dv):
-                t.zero_()
-            dtable = None if table is None else torch.zeros_like(table)
-        else:
+        dev, dt = q.device, q.dtype
+        new = torch.zeros if o.numel() == 0 or k.numel() == 0 else torch.empty
+        dq, dk, dv = new(q.shape, dtype=dt, device=dev), new(k.shape, dtype=dt, device=dev), new(k.shape, dtype=dt, device=dev)
+        dtable = None if table is None else new(table.shape, dtype=F32, device=dev)
+        if new is torch.empty:
             g = _rows16(g)
-            a = CrossAttentionFn._desc(ctx.opts, q, k, v, table, key_mask, kv_lens, q_offsets, o, lse)
-            b = _AttnGrad()
-            b.d_o, b.dq, b.dk, b.dv = (_addr(t) for t in (g, dq, dk, dv))
-            b.do_sb, b.do_sl, b.do_sh = _strides(g)
-            with _on(q):
-                n_cu = ops.cu_count(dev)
-                nrb, nkb = -(-Lq // ROWS), -(-Lk // ROWS)
-                b.splits_q = _parts(B * H * nrb, -(-Lk // TILE), n_cu, 4)
-                b.splits_k = _parts(B * Hkv * nkb, (H // Hkv) * -(-Lq // TILE), n_cu, 4)
-                up4 = lambda x: (x + 3) // 4 * 4
-                n = up4(b.splits_q * dq.numel()) if b.splits_q > 1 else 0
-                n += up4(2 * b.splits_k * dk.numel()) if b.splits_k > 1 else 0
-                if table is not None:
-                    dtable = torch.empty_like(table)
-                    b.dtable = dtable.data_ptr()
-                    n += up4(b.splits_k * B * H * nkb * table.shape[0])
-                delta = torch.empty((1 + b.splits_q if b.splits_q > 1 else 1, B, H, Lq), dtype=torch.float32, device=dev)
-                b.delta = delta.data_ptr()
-                if n:
-                    ws = torch.empty(n, dtype=torch.float32, device=dev)
-                    b.ws = ws.data_ptr()
-                check(_lib.lib().dfold_seq_attn_bwd(byref(a), byref(b), stream()), "dfold_seq_attn_bwd")
+            n_cu = ops.cu_count(dev)
+            nrb, nkb = -(-Lq // ROWS), -(-Lk // ROWS)
+            splits_q = _parts(B * H * nrb, -(-Lk // TILE), n_cu, 4)
+            splits_k = _parts(B * Hkv * nkb, (H // Hkv) * -(-Lq // TILE), n_cu, 4)
+            n = (splits_q * q.numel() if splits_q > 1 else 0) + (2 * splits_k * k.numel() if splits_k > 1 else 0)    # (multiples of 8)
+            rel = _NO_REL
+            if table is not None:
+                rel = _rel_desc(table, table.shape[0], max_distance, bidirectional, q_offset, q_offsets)
+                n += splits_k * B * H * nkb * table.shape[0]
+            delta = torch.empty((1 + splits_q if splits_q > 1 else 1, B, H, Lq), dtype=F32, device=dev)
+            ws = torch.empty(n, dtype=F32, device=dev) if n else None
+            grad = _GRAD.pack(g.data_ptr(), *_strides(g), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(), _addr(dtable), _addr(ws),
+                              splits_q, splits_k)
+            _call("dfold_seq_attn_bwd", _attn_desc(q, k, v, o, lse, None, key_mask, kv_lens, rel, scale), grad, t=q)
         need = ctx.needs_input_grad
-        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dtable if need[3] else None) + (None,) * 8
+        return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dtable if need[3] else None) + (None,) * 7
 
 
 def cross_attention(q, k, v, *, key_mask=None, kv_lens=None, rel_table=None, max_distance=128, bidirectional=True, q_offset=0, scale=None):
@@ -437,39 +464,59 @@ def cross_attention(q, k, v, *, key_mask=None, kv_lens=None, rel_table=None, max
     [num_buckets, H] adds the bias of relative_position_bias without forming it; q_offset: position of query 0 minus position of key 0, a
     whole number or an int32 / int64 tensor [B] (one token at its own position per sequence).  scale defaults to D^-1/2.
     Differentiable (once) in q, k, v and rel_table; repeated calls give the same bits."""
-    _need(q.dim() == 4 and k.dim() == 4 and v.dim() == 4, "q must be [B, Lq, H, D], k and v [B, Lk, Hkv, D]")
-    _need(q.dtype in (torch.bfloat16, torch.float16) and k.dtype == q.dtype and v.dtype == q.dtype, "q, k, v must all be bfloat16 or all float16")
+    dt, dev = q.dtype, q.device
+    if q.dim() != 4 or k.dim() != 4:
+        raise ValueError("q must be [B, Lq, H, D], k and v [B, Lk, Hkv, D]")
+    if (dt is not BF16 and dt is not F16) or k.dtype != dt or v.dtype != dt:
+        raise ValueError("q, k, v must all be bfloat16 or all float16")
     B, Lq, H, D = q.shape
-    _need(k.shape == v.shape and k.shape[0] == B and k.shape[3] == D, "k and v must be [B, Lk, Hkv, D] with q's B and D")
-    Lk, Hkv = k.shape[1], k.shape[2]
-    _need(H > 0 and Hkv > 0 and H % Hkv == 0, "the query heads must be a multiple of the key heads")
-    _need(8 <= D <= 128 and D % 8 == 0, "the head size must be a multiple of 8, at most 128")
-    _need(Lq <= 1 << 30 and Lk <= 1 << 30, "sequences are at most 2^30 long")
-    _same_device(q, k=k, v=v, key_mask=key_mask, kv_lens=kv_lens, rel_table=rel_table)
+    Bk, Lk, Hkv, Dk = k.shape
+    if k.shape != v.shape or Bk != B or Dk != D:
+        raise ValueError("k and v must be [B, Lk, Hkv, D] with q's B and D")
+    if not (H > 0 and Hkv > 0) or H % Hkv:
+        raise ValueError("the query heads must be a multiple of the key heads")
+    if D % 8 or not 8 <= D <= 128:
+        raise ValueError("the head size must be a multiple of 8, at most 128")
+    if Lq > MAX_LEN or Lk > MAX_LEN:
+        raise ValueError("sequences are at most 2^30 long")
+    _same_device(dev, "k", k)
+    _same_device(dev, "v", v)
     if key_mask is not None:
-        _need(key_mask.shape == (B, Lk), f"key_mask must be [{B}, {Lk}]")
+        _same_device(dev, "key_mask", key_mask)
+        if key_mask.shape != (B, Lk):
+            raise ValueError(f"key_mask must be [{B}, {Lk}]")
         key_mask = _mask_bytes(key_mask)
     if kv_lens is not None:
-        _need(kv_lens.shape == (B,) and kv_lens.dtype in (torch.int32, torch.int64), f"kv_lens must be int32 or int64 [{B}]")
-        kv_lens = kv_lens.clamp(max=Lk).int().contiguous() if kv_lens.dtype == torch.int64 else kv_lens.contiguous()
+        _same_device(dev, "kv_lens", kv_lens)
+        if kv_lens.shape != (B,) or kv_lens.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"kv_lens must be int32 or int64 [{B}]")
+        if kv_lens.dtype == torch.int64:
+            kv_lens = kv_lens.clamp(0, Lk).int()
+        kv_lens = kv_lens.contiguous()
     q_offsets = None
     if rel_table is not None:
+        _same_device(dev, "rel_table", rel_table)
         _check_rel(rel_table, max_distance, bidirectional)
-        _need(rel_table.shape[1] == H, f"rel_table must have {H} columns, one per query head")
+        if rel_table.shape[1] != H:
+            raise ValueError(f"rel_table must have {H} columns, one per query head")
         if torch.is_tensor(q_offset):
-            _same_device(q, q_offset=q_offset)
-            _need(q_offset.shape == (B,) and q_offset.dtype in (torch.int32, torch.int64), f"q_offset must be a whole number or int32 / int64 [{B}]")
+            _same_device(dev, "q_offset", q_offset)
+            if q_offset.shape != (B,) or q_offset.dtype not in (torch.int32, torch.int64):
+                raise ValueError(f"q_offset must be a whole number or int32 / int64 [{B}]")
             q_offsets = (q_offset.clamp(-MAX_OFFSET, MAX_OFFSET).int() if q_offset.dtype == torch.int64 else q_offset).contiguous()
             q_offset = 0
-        else:
-            _need(isinstance(q_offset, int) and abs(q_offset) <= MAX_OFFSET, f"q_offset must be a whole number, at most {MAX_OFFSET}")
+        elif not isinstance(q_offset, int) or abs(q_offset) > MAX_OFFSET:
+            raise ValueError(f"q_offset must be a whole number, at most {MAX_OFFSET}")
     else:
         q_offset = 0
     scale = D ** -0.5 if scale is None else float(scale)
-    _need(math.isfinite(scale), "scale must be finite")
+    if not math.isfinite(scale):
+        raise ValueError("scale must be finite")
     _require_cuda(q)
-    train = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (q, k, v, rel_table))
-    return CrossAttentionFn.apply(q, k, v, rel_table, key_mask, kv_lens, q_offsets, q_offset, max_distance, bool(bidirectional), scale, train)
+    args = (q, k, v, rel_table, key_mask, kv_lens, q_offsets, q_offset, max_distance, bool(bidirectional), scale)
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (rel_table is not None and rel_table.requires_grad)):
+        return CrossAttentionFn.apply(*args)
+    return _attn_forward(False, *args)[0]
 
 
 class CrossAttention(nn.Module):

@@ -1,7 +1,7 @@
 """Sequence-track operators, what needs no GPU: bucket borders against whole-number arithmetic, refusals of the Python entry points and
 of the C ABI (argument checks come before any launch), launch plans, no CPU fallback."""
 import math
-from ctypes import byref, c_int32, c_void_p
+from ctypes import byref, c_int32, c_void_p, sizeof
 from fractions import Fraction
 
 import pytest
@@ -110,13 +110,31 @@ def test_launch_plans():
         assert 1 <= s <= nt and s <= 4096
 
 
+def rel_of(table, dist, both):
+    return S.RelBias.from_buffer_copy(S._rel_desc(table, table.shape[0], dist, both, 0))
+
+
+def test_packed_descriptors_have_the_layout_of_the_structures():
+    assert S._REL.size == sizeof(S.RelBias) and S._ATTN.size + S._REL.size == sizeof(S.AttnDesc) and S._GRAD.size == sizeof(S.AttnGrad)
+    assert S._PART.size == sizeof(S.RopePart) and 2 * S._PART.size + S._ROPE.size == sizeof(S.RopeDesc)
+    d = S.AttnDesc.from_buffer_copy(S._ATTN.pack(*range(1, 31), 0.5) + S._NO_REL)
+    assert [getattr(d, n) for n, _ in S.AttnDesc._fields_[:30]] == list(range(1, 31)) and d.scale == 0.5
+    g = S.AttnGrad.from_buffer_copy(S._GRAD.pack(*range(1, 13)))
+    assert [getattr(g, n) for n, _ in S.AttnGrad._fields_] == list(range(1, 13))
+    r = S.RopeDesc.from_buffer_copy(S._PART.pack(*range(1, 16)) + S._PART.pack(*range(21, 36)) + S._ROPE.pack(51, 2.5, 0.25, *range(52, 57)))
+    assert [getattr(r.part[1], n) for n, _ in S.RopePart._fields_] == list(range(21, 36))
+    assert [getattr(r, n) for n, _ in S.RopeDesc._fields_[1:]] == [51, 2.5, 0.25, 52, 53, 54, 55, 56]
+    rel = rel_of(torch.zeros(32, 4), 128, True)
+    assert list(rel.far_border[:7]) == list(S.far_borders(32, 128, True)) and rel.num_buckets == 32 and rel.bidirectional == 1
+
+
 def test_cabi_refuses_bad_descriptors():
     from dynamicpdb_amd import _lib
     L = _lib.lib()
     tok = 16
 
     def attn(**kw):
-        d = S._AttnDesc()
+        d = S.AttnDesc()
         for n in ("q", "k", "v", "o"):
             setattr(d, n, tok)
         d.B, d.Lq, d.Lk, d.H, d.Hkv, d.D, d.splits, d.pack, d.scale = 1, 4, 4, 4, 2, 64, 1, 1, 0.1
@@ -125,24 +143,24 @@ def test_cabi_refuses_bad_descriptors():
         return d
     assert L.dfold_seq_attn_fwd(None, c_void_p(0)) == -1
     for kw in (dict(q=None), dict(k=None), dict(o=None), dict(dtype=2), dict(D=60), dict(D=136), dict(D=0), dict(H=3), dict(Hkv=0), dict(B=0), dict(Lq=0),
-               dict(Lk=-1), dict(splits=0), dict(splits=2), dict(splits=5000, ws=tok), dict(pack=3), dict(q_sl=4), dict(k_sh=-8), dict(q=tok + 2), dict(mask_sb=-1)):
+               dict(Lk=-1), dict(splits=0), dict(splits=2), dict(splits=1025, ws=tok), dict(pack=3), dict(q_sl=4), dict(k_sh=-8), dict(q=tok + 2), dict(mask_sb=-1)):
         assert L.dfold_seq_attn_fwd(byref(attn(**kw)), c_void_p(0)) == -1, kw
     for nb, dist, both, breakage in ((32, 128, True, lambda r: setattr(r, "num_buckets", 33)), (32, 128, True, lambda r: setattr(r, "num_buckets", 1)),
                                      (32, 128, True, lambda r: r.far_border.__setitem__(0, 3)), (32, 128, True, lambda r: r.far_border.__setitem__(6, 1025)),
                                      (32, 128, False, lambda r: setattr(r, "num_buckets", 600))):
         d = attn()
         table = torch.zeros(nb, 4)
-        S._fill_rel(d.rel, table, dist, both, 0)
+        d.rel = rel_of(table, dist, both)
         breakage(d.rel)
         assert L.dfold_seq_attn_fwd(byref(d), c_void_p(0)) == -1
         assert L.dfold_relpos_fwd(byref(d.rel), c_void_p(tok), c_int32(0), c_int32(4), c_int32(4), c_int32(4), c_void_p(0)) == -1
     d = attn(pack=2)                                   # bias rows of the packed heads over 32 KB
     d.H, d.pack = 16, 8
-    S._fill_rel(d.rel, torch.zeros(32, 16), 1024, True, 0)
+    d.rel = rel_of(torch.zeros(32, 16), 1024, True)
     assert L.dfold_seq_attn_fwd(byref(d), c_void_p(0)) == -1
 
     def grad(**kw):
-        g = S._AttnGrad()
+        g = S.AttnGrad()
         for n in ("d_o", "dq", "dk", "dv", "delta"):
             setattr(g, n, tok)
         g.splits_q = g.splits_k = 1
@@ -153,19 +171,18 @@ def test_cabi_refuses_bad_descriptors():
     for kw in (dict(d_o=None), dict(dq=None), dict(dk=None), dict(delta=None), dict(splits_q=0), dict(splits_q=2), dict(splits_k=2), dict(do_sl=3), dict(dv=tok + 8)):
         assert L.dfold_seq_attn_bwd(byref(attn(lse=tok)), byref(grad(**kw)), c_void_p(0)) == -1, kw
 
-    rel = S._RelBias()
-    S._fill_rel(rel, torch.zeros(32, 4), 128, True, 0)
+    rel = rel_of(torch.zeros(32, 4), 128, True)
     one, st = c_void_p(tok), c_void_p(0)
     for args in ((None, 0, 4, 4, 4), (tok + 2, 0, 4, 4, 4), (tok, 3, 4, 4, 4), (tok, 0, 0, 4, 4), (tok, 0, 4, 0, 4), (tok, 0, 4, 4, 0), (tok, 0, 70000, 4, 4)):
         a = (byref(rel), c_void_p(args[0])) + tuple(c_int32(x) for x in args[1:])
         assert L.dfold_relpos_fwd(*a, st) == -1
         assert L.dfold_relpos_bwd(*a, one, one, st) == -1
     assert L.dfold_relpos_ws(c_int32(0), c_int32(1), c_int32(1)) == -1 and L.dfold_relpos_ws(c_int32(1 << 20), c_int32(1 << 20), c_int32(1 << 20)) == -1
-    for blocks_of in ((1, 1, 32), (16, 4097, 64), (2000, 5, 2)):
-        assert L.dfold_relpos_ws(*(c_int32(x) for x in blocks_of)) == blocks_of[0] * min(blocks_of[1], max(1024 // blocks_of[0], 1)) * blocks_of[2]
+    for blocks_of in ((1, 1, 32), (16, 4097, 64), (3000, 5, 2)):
+        assert L.dfold_relpos_ws(*(c_int32(x) for x in blocks_of)) == blocks_of[0] * min(blocks_of[1], max(2048 // blocks_of[0], 1)) * blocks_of[2]
 
     def rope(**kw):
-        d = S._RopeDesc()
+        d = S.RopeDesc()
         d.B, d.D, d.rotary_dim, d.base, d.eps = 1, 64, 64, 10000.0, 1e-6
         p = d.part[0]
         p.x = p.y = tok
