@@ -69,61 +69,84 @@ __device__ __forceinline__ unsigned sa_work_id() {
 
 // ---- LDS tiles: SA_KT rows of DP 16-bit values, 16-byte chunks XOR-permuted within a row.  The key makes both kinds of read
 //      conflict-free: 16 consecutive rows at one chunk (operand rows) and 4 consecutive rows at 4 consecutive chunks (transpose
-//      reads; rows 0 .. 3 of a quadruple must land in different 64-byte groups of the 256-byte bank line) ----
+//      reads; rows 0 .. 3 of a quadruple must land in different 64-byte groups of the 256-byte bank line).  It depends on row % 16
+//      only, so every address is one of a lane's few offsets plus a constant that fits the instruction ----
 template <int DP>
 struct SaTile {
   static constexpr int CPR = DP / 8;                       // chunks per row: 4, 8, 16
-  static constexpr int BYTES = SA_KT * DP * 2;
+  static constexpr int PITCH = DP * 2;
+  static constexpr int BYTES = SA_KT * PITCH;
+  static constexpr int KS = DP / 16, NT = DP / 32;         // 16-deep steps, 32-wide column tiles
   static constexpr int NCH = SA_KT * CPR / (64 * SA_WAVES);  // chunks per thread of a staged tile
   static __device__ __forceinline__ int key(int row) {
     if constexpr (CPR == 16) return ((row & 3) << 2) | ((row >> 2) & 3);
     if constexpr (CPR == 8) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
     return (row >> 2) & 3;
   }
-  static __device__ __forceinline__ int off(int row, int chunk) { return row * (DP * 2) + ((chunk ^ key(row)) << 4); }
-  // operand rows: lane holds row `row`, elements 16 ks + 8 h .. + 8
-  static __device__ __forceinline__ sa_u32x4 rows(const char* t, int row, int ks, int h) {
-    return *(const sa_u32x4*)(t + off(row, 2 * ks + h));
+  static __device__ __forceinline__ int off(int row, int chunk) { return row * PITCH + ((chunk ^ key(row)) << 4); }
+};
+
+// A lane's offsets into a tile.  rows(r0, ks): lane holds row r0 + (lane & 31), elements 16 ks + 8 h .. + 8.  cols(r0, dt): lane holds
+// column 32 dt + (lane & 31), rows r0 + 4 h + 0 .. 3 and r0 + 8 + 4 h + 0 .. 3.  r0 a multiple of 16, a constant at every use.
+template <int DP>
+struct SaAddr {
+  using T = SaTile<DP>;
+  int row[T::KS], col[T::NT][2];
+  __device__ __forceinline__ SaAddr(int lane) {
+    const int h = lane >> 5, i = lane & 15;
+#pragma unroll
+    for (int ks = 0; ks < T::KS; ++ks) row[ks] = T::off(lane & 31, 2 * ks + h);
+#pragma unroll
+    for (int dt = 0; dt < T::NT; ++dt)
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        col[dt][x] = T::off(8 * x + 4 * h + (i >> 2), 4 * dt + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) + (i & 1) * 8;
   }
-  // transposed operand: lane holds column 32 dt + (lane & 31), rows r0 + 4 h + 0 .. 3 and r0 + 8 + 4 h + 0 .. 3
-  static __device__ __forceinline__ sa_u32x4 cols(const char* t, int r0, int dt, int lane) {
-    const int i = lane & 15, row = r0 + 4 * (lane >> 5) + (i >> 2);
-    const int chunk = 4 * dt + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1), sub = (i & 1) * 8;
+  __device__ __forceinline__ sa_u32x4 rows(const char* t, int r0, int ks) const { return *(const sa_u32x4*)(t + row[ks] + r0 * T::PITCH); }
+  __device__ __forceinline__ sa_u32x4 cols(const char* t, int r0, int dt) const {
     sa_lchar* b = (sa_lchar*)t;
-    const sa_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((sa_ls16x4*)(b + off(row, chunk) + sub));
-    const sa_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((sa_ls16x4*)(b + off(row + 8, chunk) + sub));
+    const sa_s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((sa_ls16x4*)(b + col[dt][0] + r0 * T::PITCH));
+    const sa_s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((sa_ls16x4*)(b + col[dt][1] + r0 * T::PITCH));
     return __builtin_bit_cast(sa_u32x4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   }
 };
 
-// registers of a tile on its way to LDS: rows row0 .. row0 + SA_KT of a [rows][D] matrix with row stride `rs` elements.  Rows at or
-// past `end` and columns at or past D read as zeros; `live` (one bit per row) zeroes rows whose content must not be used.
+// Registers of a tile on its way to LDS: SA_KT rows of a [rows][D] matrix with row stride `rs` elements (< SA_MAX_ROW).  The loads go
+// through a buffer descriptor that ends with the last row there is: a tile costs no address arithmetic on the vector unit and rows past
+// the end (and columns past D) come back as zeros.  mask(): one bit per row, zeroes rows whose content must not be used.
+#define SA_MAX_ROW (1 << 24)
 template <int DP>
 struct SaStage {
   using T = SaTile<DP>;
   sa_u32x4 v[T::NCH];
-  __device__ __forceinline__ void load(const char* base, long rs, int row0, int end, int D, int tid) {
+  unsigned voff[T::NCH];
+  int lds;
+  __device__ __forceinline__ void init(long rs, int D, int tid) {
+    const int cc = tid % T::CPR;
 #pragma unroll
-    for (int i = 0; i < T::NCH; ++i) {
-      const int c = tid + i * 64 * SA_WAVES, row = row0 + c / T::CPR, cc = c % T::CPR;
-      v[i] = (sa_u32x4){0u, 0u, 0u, 0u};
-      if (row < end && cc * 8 < D) v[i] = *(const sa_u32x4*)(base + ((long)row * rs + cc * 8) * 2);
-    }
+    for (int i = 0; i < T::NCH; ++i) voff[i] = cc * 8 < D ? (unsigned)((tid / T::CPR + i * (64 * SA_WAVES / T::CPR)) * rs + cc * 8) * 2u : 0x80000000u;
+    lds = T::off(tid / T::CPR, cc);
+  }
+  // rows row0 .. of a matrix of `end` > row0 rows
+  __device__ __forceinline__ void load(const char* base, long rs, int row0, int end, int D) {
+    const unsigned bytes = (unsigned)(((long)(min(end - row0, SA_KT) - 1) * rs + D) * 2);
+    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(base + (long)row0 * rs * 2), 0, bytes, 0x00020000);
+#pragma unroll
+    for (int i = 0; i < T::NCH; ++i) v[i] = __builtin_amdgcn_raw_buffer_load_b128(r, voff[i], 0, 0);
   }
   __device__ __forceinline__ void mask(unsigned long live, int tid) {
 #pragma unroll
-    for (int i = 0; i < T::NCH; ++i) {
-      const int row = (tid + i * 64 * SA_WAVES) / T::CPR;
-      if (!((live >> row) & 1)) v[i] = (sa_u32x4){0u, 0u, 0u, 0u};
-    }
+    for (int i = 0; i < T::NCH; ++i)
+      if (!((live >> (tid / T::CPR + i * (64 * SA_WAVES / T::CPR))) & 1)) v[i] = (sa_u32x4){0u, 0u, 0u, 0u};
   }
-  __device__ __forceinline__ void store(char* t, int tid) const {
+  __device__ __forceinline__ void store(char* t) const {
 #pragma unroll
-    for (int i = 0; i < T::NCH; ++i) {
-      const int c = tid + i * 64 * SA_WAVES;
-      *(sa_u32x4*)(t + T::off(c / T::CPR, c % T::CPR)) = v[i];
-    }
+    for (int i = 0; i < T::NCH; ++i) *(sa_u32x4*)(t + lds + i * (64 * SA_WAVES / T::CPR) * T::PITCH) = v[i];
   }
+};
+template <int I>
+struct SaInt {
+  static constexpr int value = I;
 };
 
 // ---- bucketed relative position bias ----
@@ -209,5 +232,6 @@ static inline bool sa_desc_ok(const dfold_seq_attn_desc* d) {
   const int64_t st[12] = {d->q_sb, d->q_sl, d->q_sh, d->k_sb, d->k_sl, d->k_sh, d->v_sb, d->v_sl, d->v_sh, d->o_sb, d->o_sl, d->o_sh};
   for (int i = 0; i < 12; ++i)
     if (st[i] % 8 || st[i] < 0) return false;
+  if (d->q_sl >= SA_MAX_ROW || d->k_sl >= SA_MAX_ROW || d->v_sl >= SA_MAX_ROW || !(d->scale != 0.f)) return false;
   return d->mask_sb >= 0;
 }

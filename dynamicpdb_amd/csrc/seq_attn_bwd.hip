@@ -34,30 +34,31 @@ struct SaBwdParams {
   SaRel rel;
 };
 
-// logits x log2 e of a block held with columns `c` and rows 8 (r / 4) + 4 h + r % 4; sgn = +1: rows are keys, -1: rows are queries
+// logits x log2 e minus the row's log-sum of a block whose columns are softmax rows (rows: keys d0 + 8 (r / 4) + r % 4)
 template <bool REL>
-__device__ __forceinline__ void sa_logits(f32x16& s, float sl2, const float* myb, int W, int far, float farv, int d0, int sgn) {
+__device__ __forceinline__ void sa_logits(f32x16& s, float sl2, float nlse, const float* myb, int W, int far, float farv, int d0) {
   if constexpr (REL) {
     if (far) {
+      const float c = farv + nlse;
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], sl2, farv);
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], sl2, c);
     } else {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        const int d = d0 + sgn * (8 * (r >> 2) + (r & 3));
-        s[r] = __builtin_fmaf(s[r], sl2, myb[min(max(d, -W), W)]);
+        const int d = d0 + 8 * (r >> 2) + (r & 3);
+        s[r] = __builtin_fmaf(s[r], sl2, myb[min(max(d, -W), W)] + nlse);
       }
     }
   } else {
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] *= sl2;
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], sl2, nlse);
   }
 }
 
 template <int DT, int DP, bool REL>
 __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_dq_kernel(const SaBwdParams p) {
   using T = SaTile<DP>;
-  constexpr int KS = DP / 16, NT = DP / 32;
+  constexpr int KS = T::KS, NT = T::NT;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* const ldsB = (float*)(smem + 4 * T::BYTES);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -125,28 +126,30 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_dq_kernel(const SaB
     for (int r = 0; r < 16; ++r) dq[i][r] = 0.f;
 
   float left = 0.f;          // row sum of dS
+  const SaAddr<DP> ad(lane);
   SaStage<DP> sk, sv;
+  sk.init(p.k_sl, p.D, tid);
+  sv.init(p.v_sl, p.D, tid);
   int kmask = 0;
   auto fetch = [&](int t) {
-    sk.load(kb_, p.k_sl, t * SA_KT, kv_end, p.D, tid);
-    sv.load(vb_, p.v_sl, t * SA_KT, kv_end, p.D, tid);
+    sk.load(kb_, p.k_sl, t * SA_KT, kv_end, p.D);
+    sv.load(vb_, p.v_sl, t * SA_KT, kv_end, p.D);
     const int key = t * SA_KT + lane;
     kmask = key < kv_end ? (mb_ ? mb_[key] : 1) : 0;
   };
-  if (t0 < t1) fetch(t0);
-  for (int t = t0; t < t1; ++t) {
-    char* const lk = smem + (t & 1) * 2 * T::BYTES;
+  auto step = [&](int t, auto stage) {
+    char* const lk = smem + decltype(stage)::value * 2 * T::BYTES;
     char* const lv = lk + T::BYTES;
     const unsigned long live = __ballot(kmask != 0);
-    if (mb_ && live != ~0ul) {
+    if (live != ~0ul) {
       sk.mask(live, tid);
       sv.mask(live, tid);
     }
-    sk.store(lk, tid);
-    sv.store(lv, tid);
+    sk.store(lk);
+    sv.store(lv);
     __syncthreads();
     if (t + 1 < t1) fetch(t + 1);
-    if (live == 0 || !wave_on) continue;
+    if (live == 0 || !wave_on) return;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       f32x16 s, dp;
@@ -154,13 +157,12 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_dq_kernel(const SaB
       for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        s = sa_mfma<DT>(T::rows(lk, kb * 32 + l31, ks, h), qf[ks], s);
-        dp = sa_mfma<DT>(T::rows(lv, kb * 32 + l31, ks, h), of[ks], dp);
+        s = sa_mfma<DT>(ad.rows(lk, kb * 32, ks), qf[ks], s);
+        dp = sa_mfma<DT>(ad.rows(lv, kb * 32, ks), of[ks], dp);
       }
       const int k0 = t * SA_KT + kb * 32;
       const int far = !REL ? 0 : k0 - qhi >= p.rel.W ? 1 : k0 + 31 - qlo <= -p.rel.W ? -1 : 0;
-      const int d0 = k0 + 4 * h - qpos;
-      sa_logits<REL>(s, p.sl2, myb, p.rel.W, far, far > 0 ? bR : bL, d0, 1);
+      sa_logits<REL>(s, p.sl2, -lse, myb, p.rel.W, far, far > 0 ? bR : bL, k0 + 4 * h - qpos);
       if (live != ~0ul) {
         const unsigned bits = (unsigned)(live >> (kb * 32)) >> (4 * h);
 #pragma unroll
@@ -169,7 +171,7 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_dq_kernel(const SaB
       }
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[r] = sa_exp2(s[r] - lse) * (dp[r] - dl);
+        s[r] = sa_exp2(s[r]) * (dp[r] - dl);
         left += s[r];
       }
 #pragma unroll
@@ -178,9 +180,14 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_dq_kernel(const SaB
 #pragma unroll
         for (int e = 0; e < 4; ++e) df[e] = sa_pack2<DT>(s[8 * c + 2 * e], s[8 * c + 2 * e + 1]);
 #pragma unroll
-        for (int i = 0; i < NT; ++i) dq[i] = sa_mfma<DT>(T::cols(lk, kb * 32 + c * 16, i, lane), df, dq[i]);
+        for (int i = 0; i < NT; ++i) dq[i] = sa_mfma<DT>(ad.cols(lk, kb * 32 + c * 16, i), df, dq[i]);
       }
     }
+  };
+  if (t0 < t1) fetch(t0);
+  for (int t = t0; t < t1; t += 2) {
+    step(t, SaInt<0>());
+    if (t + 1 < t1) step(t + 1, SaInt<1>());
   }
 
   left = sa_xsum(left);
@@ -214,7 +221,7 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_dq_kernel(const SaB
 template <int DT, int DP, bool REL>
 __global__ __launch_bounds__(64 * SA_WAVES, DP == 128 ? 1 : 2) void seq_attn_dkv_kernel(const SaBwdParams p) {
   using T = SaTile<DP>;
-  constexpr int KS = DP / 16, NT = DP / 32;
+  constexpr int KS = T::KS, NT = T::NT;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* const ldsL = (float*)(smem + 4 * T::BYTES);            // [stage][log-sum | delta][SA_KT]
   float* const ldsB = ldsL + 4 * SA_KT;
@@ -293,26 +300,32 @@ __global__ __launch_bounds__(64 * SA_WAVES, DP == 128 ? 1 : 2) void seq_attn_dkv
         for (int j = tid; j < p.num_buckets; j += 64 * SA_WAVES) table_part(hkv * G + g)[j] = 0.f;
   }
 
+  const SaAddr<DP> ad(lane);
   SaStage<DP> sq, sg;
+  sq.init(p.q_sl, p.D, tid);
+  sg.init(p.do_sl, p.D, tid);
   float lse_r = 0.f, del_r = 0.f;
-  auto fetch = [&](int u) {
-    const int head = hkv * G + u / nqt, q0 = (u % nqt) * SA_KT;
-    sq.load(p.q + ((long)b * p.q_sb + (long)head * p.q_sh) * 2, p.q_sl, q0, p.Lq, p.D, tid);
-    sg.load(p.d_o + ((long)b * p.do_sb + (long)head * p.do_sh) * 2, p.do_sl, q0, p.Lq, p.D, tid);
+  // position in the walk of the unit that is fetched next, and of the one that is worked on
+  int fg = u0 / nqt, fq = (u0 - fg * nqt) * SA_KT, wg = fg, wq = fq;
+  auto fetch = [&]() {
+    const int head = hkv * G + fg;
+    sq.load(p.q + ((long)b * p.q_sb + (long)head * p.q_sh) * 2, p.q_sl, fq, p.Lq, p.D);
+    sg.load(p.d_o + ((long)b * p.do_sb + (long)head * p.do_sh) * 2, p.do_sl, fq, p.Lq, p.D);
     if (tid < SA_KT) {
-      const int qi = q0 + tid;
+      const int qi = fq + tid;
       const long r = ((long)b * p.H + head) * p.Lq + qi;
-      lse_r = qi < p.Lq ? p.lse[r] : INFINITY;       // rows past the end: P = 0
+      lse_r = qi < p.Lq ? -p.lse[r] : -INFINITY;       // rows past the end: P = 0
       del_r = qi < p.Lq ? p.delta[r] : 0.f;
     }
+    if ((fq += SA_KT) >= p.Lq) { fq = 0; ++fg; }
   };
-  if (u0 < u1) fetch(u0);
-  for (int u = u0; u < u1; ++u) {
-    char* const lq = smem + (u & 1) * 2 * T::BYTES;
+  auto step = [&](bool more, auto stage) {
+    char* const lq = smem + decltype(stage)::value * 2 * T::BYTES;
     char* const lg = lq + T::BYTES;
-    float* const ll = ldsL + (u & 1) * 2 * SA_KT;
+    float* const ll = ldsL + decltype(stage)::value * 2 * SA_KT;
+    const int q0 = wq;
     if constexpr (REL) {
-      const int head = hkv * G + u / nqt;
+      const int head = hkv * G + wg;
       if (head != head_in) {       // (uniform)
         if (head_in >= 0) flush(head_in);      // (ends in a barrier: nobody reads the previous head's rows any more)
         for (int i = tid; i < SA_WAVES * hn; i += 64 * SA_WAVES) ldsH[i] = 0.f;
@@ -320,16 +333,16 @@ __global__ __launch_bounds__(64 * SA_WAVES, DP == 128 ? 1 : 2) void seq_attn_dkv
         head_in = head;
       }
     }
-    sq.store(lq, tid);
-    sg.store(lg, tid);
+    if ((wq += SA_KT) >= p.Lq) { wq = 0; ++wg; }
+    sq.store(lq);
+    sg.store(lg);
     if (tid < SA_KT) {
       ll[tid] = lse_r;
       ll[SA_KT + tid] = del_r;
     }
     __syncthreads();
-    if (u + 1 < u1) fetch(u + 1);
-    if (!wave_on) continue;
-    const int q0 = (u % nqt) * SA_KT;
+    if (more) fetch();
+    if (!wave_on) return;
 #pragma unroll
     for (int qb = 0; qb < 2; ++qb) {
       if (q0 + qb * 32 >= p.Lq) continue;
@@ -338,23 +351,33 @@ __global__ __launch_bounds__(64 * SA_WAVES, DP == 128 ? 1 : 2) void seq_attn_dkv
       for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
-        s = sa_mfma<DT>(T::rows(lq, qb * 32 + l31, ks, h), kf[ks], s);
-        dp = sa_mfma<DT>(T::rows(lg, qb * 32 + l31, ks, h), vf[ks], dp);
+        s = sa_mfma<DT>(ad.rows(lq, qb * 32, ks), kf[ks], s);
+        dp = sa_mfma<DT>(ad.rows(lg, qb * 32, ks), vf[ks], dp);
       }
       const int qlo = q0 + qb * 32 + off, qhi = qlo + 31;
       const int far = !REL ? 0 : key_w - qhi >= p.rel.W ? 1 : key_w + 31 - qlo <= -p.rel.W ? -1 : 0;
-      const float farv = REL ? myb[far > 0 ? p.rel.W : -p.rel.W] : 0.f;
-      sa_logits<REL>(s, p.sl2, myb, p.rel.W, far, farv, key - qlo - 4 * h, -1);
-      f32x4 rl[4], rd[4];
+      if constexpr (REL) {
+        if (far) {
+          const float c = myb[far > 0 ? p.rel.W : -p.rel.W];
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        rl[g] = *(const f32x4*)(ll + qb * 32 + g * 8 + h * 4);
-        rd[g] = *(const f32x4*)(ll + SA_KT + qb * 32 + g * 8 + h * 4);
+          for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], p.sl2, c);
+        } else {
+          const int d0 = key - qlo - 4 * h;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], p.sl2, myb[min(max(d0 - 8 * (r >> 2) - (r & 3), -p.rel.W), p.rel.W)]);
+        }
       }
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        s[r] = key_on ? sa_exp2(s[r] - rl[r >> 2][r & 3]) : 0.f;
-        dp[r] = s[r] * (dp[r] - rd[r >> 2][r & 3]);
+      for (int g = 0; g < 4; ++g) {
+        const f32x4 rl = *(const f32x4*)(ll + qb * 32 + g * 8 + h * 4);
+        const f32x4 rd = *(const f32x4*)(ll + SA_KT + qb * 32 + g * 8 + h * 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = g * 4 + e;
+          const float x = REL ? s[r] + rl[e] : __builtin_fmaf(s[r], p.sl2, rl[e]);
+          s[r] = key_on ? sa_exp2(x) : 0.f;
+          dp[r] = s[r] * (dp[r] - rd[e]);
+        }
       }
       if constexpr (REL) {
         if (far) {
@@ -389,11 +412,16 @@ __global__ __launch_bounds__(64 * SA_WAVES, DP == 128 ? 1 : 2) void seq_attn_dkv
         }
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
-          dv[i] = sa_mfma<DT>(T::cols(lg, qb * 32 + c * 16, i, lane), pf, dv[i]);
-          dk[i] = sa_mfma<DT>(T::cols(lq, qb * 32 + c * 16, i, lane), df, dk[i]);
+          dv[i] = sa_mfma<DT>(ad.cols(lg, qb * 32 + c * 16, i), pf, dv[i]);
+          dk[i] = sa_mfma<DT>(ad.cols(lq, qb * 32 + c * 16, i), df, dk[i]);
         }
       }
     }
+  };
+  if (u0 < u1) fetch();
+  for (int u = u0; u < u1; u += 2) {
+    step(u + 1 < u1, SaInt<0>());
+    if (u + 1 < u1) step(u + 2 < u1, SaInt<1>());
   }
 
   if constexpr (REL)
@@ -493,7 +521,7 @@ extern "C" int dfold_seq_attn_bwd(const dfold_seq_attn_desc* d, const dfold_seq_
   if (!sa_desc_ok(d) || d->Lk == 0 || !g || !d->lse || !g->d_o || !g->dq || !g->delta || !g->dk || !g->dv) return DFOLD_EINVAL;
   if (g->splits_q < 1 || g->splits_q > 4096 || g->splits_k < 1 || g->splits_k > 4096) return DFOLD_EINVAL;
   if (((uintptr_t)g->d_o | (uintptr_t)g->dq | (uintptr_t)g->dk | (uintptr_t)g->dv | (uintptr_t)g->ws) & 15) return DFOLD_EINVAL;
-  if ((g->do_sb | g->do_sl | g->do_sh) % 8 || g->do_sb < 0 || g->do_sl < 0 || g->do_sh < 0) return DFOLD_EINVAL;
+  if ((g->do_sb | g->do_sl | g->do_sh) % 8 || g->do_sl >= SA_MAX_ROW || g->do_sb < 0 || g->do_sl < 0 || g->do_sh < 0) return DFOLD_EINVAL;
   const bool rel = d->rel.table != nullptr;
   if (rel && (!g->dtable || !sa_make_rel(&d->rel, d->H, &p.rel))) return DFOLD_EINVAL;
   if ((rel || g->splits_q > 1 || g->splits_k > 1) && !g->ws) return DFOLD_EINVAL;

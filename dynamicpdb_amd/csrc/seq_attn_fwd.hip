@@ -31,7 +31,7 @@ struct SaFwdParams {
 template <int DT, int DP, bool REL>
 __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_fwd_kernel(const SaFwdParams p) {
   using T = SaTile<DP>;
-  constexpr int KS = DP / 16, NT = DP / 32;
+  constexpr int KS = T::KS, NT = T::NT;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* const ldsB = (float*)(smem + 4 * T::BYTES);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -67,17 +67,22 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_fwd_kernel(const Sa
     bR = myb[p.rel.W];
   }
 
-  // Q^T operand of the lane's row
+  // Q^T operand of the lane's row; a negative scale turns its sign, so that the softmax can take its maximum over unscaled products
   sa_u32x4 qf[KS];
   {
     const char* src = p.q + ((long)b * p.q_sb + (long)qi * p.q_sl + (long)(head0 + hl) * p.q_sh) * 2;
+    const unsigned flip = p.sl2 < 0.f ? 0x80008000u : 0u;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const int d = ks * 16 + h * 8;
       qf[ks] = (sa_u32x4){0u, 0u, 0u, 0u};
       if (d < p.D) qf[ks] = *(const sa_u32x4*)(src + d * 2);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) qf[ks][e] ^= flip;
     }
   }
+  const float sl2 = fabsf(p.sl2);
+  const float us = REL ? 1.f : sl2, lazy = SA_LAZY / us;       // units of the logits below: log2 with a bias, else unscaled products
   const char* const kb_ = p.k + ((long)b * p.k_sb + (long)hkv * p.k_sh) * 2;
   const char* const vb_ = p.v + ((long)b * p.v_sb + (long)hkv * p.v_sh) * 2;
   const uint8_t* const mb_ = p.key_mask ? p.key_mask + (long)b * p.mask_sb : nullptr;
@@ -89,28 +94,30 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_fwd_kernel(const Sa
     for (int r = 0; r < 16; ++r) O[i][r] = 0.f;
   float m = -INFINITY, l = 0.f;
 
+  const SaAddr<DP> ad(lane);
   SaStage<DP> sk, sv;
+  sk.init(p.k_sl, p.D, tid);
+  sv.init(p.v_sl, p.D, tid);
   int kmask = 0;
   auto fetch = [&](int t) {
-    sk.load(kb_, p.k_sl, t * SA_KT, kv_end, p.D, tid);
-    sv.load(vb_, p.v_sl, t * SA_KT, kv_end, p.D, tid);
+    sk.load(kb_, p.k_sl, t * SA_KT, kv_end, p.D);
+    sv.load(vb_, p.v_sl, t * SA_KT, kv_end, p.D);
     const int key = t * SA_KT + lane;
     kmask = key < kv_end ? (mb_ ? mb_[key] : 1) : 0;
   };
-  if (t0 < t1) fetch(t0);
-  for (int t = t0; t < t1; ++t) {
-    char* const lk = smem + (t & 1) * 2 * T::BYTES;
+  auto step = [&](int t, auto stage) {
+    char* const lk = smem + decltype(stage)::value * 2 * T::BYTES;
     char* const lv = lk + T::BYTES;
     const unsigned long live = __ballot(kmask != 0);
-    if (mb_ && live != ~0ul) {
+    if (live != ~0ul) {
       sk.mask(live, tid);
       sv.mask(live, tid);
     }
-    sk.store(lk, tid);
-    sv.store(lv, tid);
+    sk.store(lk);
+    sv.store(lv);
     __syncthreads();
     if (t + 1 < t1) fetch(t + 1);
-    if (live == 0 || !wave_on) continue;
+    if (live == 0 || !wave_on) return;
 
     // S^T: keys x rows
     f32x16 s[2];
@@ -119,7 +126,7 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_fwd_kernel(const Sa
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < KS; ++ks) s[kb] = sa_mfma<DT>(T::rows(lk, kb * 32 + l31, ks, h), qf[ks], s[kb]);
+      for (int ks = 0; ks < KS; ++ks) s[kb] = sa_mfma<DT>(ad.rows(lk, kb * 32, ks), qf[ks], s[kb]);
     }
     if constexpr (REL) {
 #pragma unroll
@@ -128,21 +135,16 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_fwd_kernel(const Sa
         if (k0 - qhi >= p.rel.W || k0 + 31 - qlo <= -p.rel.W) {       // the whole block lies in the last bucket of a side
           const float c = k0 - qhi >= p.rel.W ? bR : bL;
 #pragma unroll
-          for (int r = 0; r < 16; ++r) s[kb][r] = __builtin_fmaf(s[kb][r], p.sl2, c);
+          for (int r = 0; r < 16; ++r) s[kb][r] = __builtin_fmaf(s[kb][r], sl2, c);
         } else {
           const int d0 = k0 + 4 * h - qpos;
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
             const int d = d0 + 8 * (r >> 2) + (r & 3);
-            s[kb][r] = __builtin_fmaf(s[kb][r], p.sl2, myb[min(max(d, -p.rel.W), p.rel.W)]);
+            s[kb][r] = __builtin_fmaf(s[kb][r], sl2, myb[min(max(d, -p.rel.W), p.rel.W)]);
           }
         }
       }
-    } else {
-#pragma unroll
-      for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[kb][r] *= p.sl2;
     }
     if (live != ~0ul) {
 #pragma unroll
@@ -153,14 +155,12 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_fwd_kernel(const Sa
           if (!((bits >> (8 * (r >> 2) + (r & 3))) & 1)) s[kb][r] = -INFINITY;
       }
     }
-    float mt = -INFINITY;
+    float mt = fmaxf(s[0][0], s[1][0]);
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) mt = fmaxf(mt, s[kb][r]);
+    for (int r = 1; r < 16; ++r) mt = fmaxf(fmaxf(mt, s[0][r]), s[1][r]);
     mt = sa_xmax(mt);
-    if (__ballot(mt > m + SA_LAZY)) {
-      const float mn = fmaxf(m, mt), a = m == mn ? 1.f : sa_exp2(m - mn);     // (m == mn also for rows without keys so far)
+    if (__ballot(mt > m + lazy)) {
+      const float mn = fmaxf(m, mt), a = m == mn ? 1.f : sa_exp2((m - mn) * us);     // (m == mn also for rows without keys so far)
       m = mn;
       l *= a;
 #pragma unroll
@@ -168,13 +168,13 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_fwd_kernel(const Sa
 #pragma unroll
         for (int r = 0; r < 16; ++r) O[i][r] *= a;
     }
-    const float mu = m == -INFINITY ? 0.f : m;
+    const float nm = m == -INFINITY ? 0.f : -m * us;
     sa_u32x4 pf[4];
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[kb][r] = sa_exp2(s[kb][r] - mu);
+        s[kb][r] = sa_exp2(REL ? s[kb][r] + nm : __builtin_fmaf(s[kb][r], sl2, nm));
         l += s[kb][r];
       }
 #pragma unroll
@@ -185,7 +185,12 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_fwd_kernel(const Sa
 #pragma unroll
     for (int c = 0; c < 4; ++c)
 #pragma unroll
-      for (int i = 0; i < NT; ++i) O[i] = sa_mfma<DT>(T::cols(lv, c * 16, i, lane), pf[c], O[i]);
+      for (int i = 0; i < NT; ++i) O[i] = sa_mfma<DT>(ad.cols(lv, c * 16, i), pf[c], O[i]);
+  };
+  if (t0 < t1) fetch(t0);
+  for (int t = t0; t < t1; t += 2) {
+    step(t, SaInt<0>());
+    if (t + 1 < t1) step(t + 1, SaInt<1>());
   }
 
   if (!wave_on) return;
@@ -194,7 +199,7 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_fwd_kernel(const Sa
   if (!on) return;
   const int head = head0 + hl;
   if (p.splits == 1) {
-    if (p.lse && h == 0) p.lse[((long)b * p.H + head) * p.Lq + qi] = l > 0.f || l != l ? m + __log2f(l) : INFINITY;
+    if (p.lse && h == 0) p.lse[((long)b * p.H + head) * p.Lq + qi] = l > 0.f || l != l ? m * us + __log2f(l) : INFINITY;
     char* const dst = p.o + ((long)b * p.o_sb + (long)qi * p.o_sl + (long)head * p.o_sh) * 2;
 #pragma unroll
     for (int i = 0; i < NT; ++i)
@@ -208,7 +213,7 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_fwd_kernel(const Sa
     // partial result: normalised O and the log2 of the part's sum (-inf: no keys), [split][b][query][head][D], [split][b][query][head]
     const long r1 = ((long)b * p.Lq + qi) * p.H + head, nr = (long)p.B * p.Lq * p.H;
     float* const dst = p.ws + ((long)sp * nr + r1) * p.D;
-    if (h == 0) p.ws[p.splits * nr * p.D + sp * nr + r1] = l > 0.f || l != l ? m + __log2f(l) : -INFINITY;
+    if (h == 0) p.ws[p.splits * nr * p.D + sp * nr + r1] = l > 0.f || l != l ? m * us + __log2f(l) : -INFINITY;
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll

@@ -83,36 +83,53 @@ __global__ __launch_bounds__(256) void relpos_fwd_kernel(const SaMatParams p) {
   }
 }
 
-// a lane's share of the sum of row[a .. b): 16-byte chunks, single elements before the first and after the last 16-byte border
+// A lane's share of row[a .. b): 16-byte chunks, single elements before the first and after the last 16-byte border.  fetch() requests the
+// first 256 chunks of a wave (and the single elements), sum() adds them up and walks the rest: a caller fetches several before it sums.
 template <int DT>
-__device__ __forceinline__ float line_sum(const typename SaElem<DT>::type* row, int a, int b, int lane) {
+struct SaLine {
   using E = typename SaElem<DT>::type;
-  constexpr int V = SaElem<DT>::VEC;
-  if (a >= b) return 0.f;
-  const int head = min((int)((-(long)(((uintptr_t)(row + a)) / sizeof(E))) & (V - 1)), b - a);
-  float s = 0.f;
-  if (lane < head) s = sa_to_f32<DT>(row[a + lane]);
-  a += head;
-  const int n = (b - a) / V;
-  if (lane < b - a - n * V) s += sa_to_f32<DT>(row[a + n * V + lane]);
-  const sa_u32x4* const c = (const sa_u32x4*)(row + a);
-  for (int k = lane; k < n; k += 256) {
-    sa_u32x4 x[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) x[u] = k + 64 * u < n ? c[k + 64 * u] : (sa_u32x4){0u, 0u, 0u, 0u};
+  static constexpr int V = SaElem<DT>::VEC;
+  const sa_u32x4* c;
+  int n, k;
+  E one[2];
+  sa_u32x4 x[4];
+  __device__ __forceinline__ void more() {
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      if constexpr (DT == DFOLD_DT_F32) {
-        const f32x4 y = __builtin_bit_cast(f32x4, x[u]);
-        s += (y[0] + y[1]) + (y[2] + y[3]);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) s += sa_lo<DT>(x[u][e]) + sa_hi<DT>(x[u][e]);
-      }
+      x[u] = (sa_u32x4){0u, 0u, 0u, 0u};
+      if (k + 64 * u < n) x[u] = c[k + 64 * u];
     }
   }
-  return s;
-}
+  __device__ __forceinline__ void fetch(const E* row, int a, int b, int lane) {
+    const int head = min((int)((-(long)(((uintptr_t)(row + a)) / sizeof(E))) & (V - 1)), b - a);
+    one[0] = one[1] = 0;
+    if (lane < head) one[0] = row[a + lane];
+    a += head;
+    n = (b - a) / V;
+    k = lane;
+    if (lane < b - a - n * V) one[1] = row[a + n * V + lane];
+    c = (const sa_u32x4*)(row + a);
+    more();
+  }
+  __device__ __forceinline__ float sum() {
+    float s = sa_to_f32<DT>(one[0]) + sa_to_f32<DT>(one[1]);
+    while (true) {
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        if constexpr (DT == DFOLD_DT_F32) {
+          const f32x4 y = __builtin_bit_cast(f32x4, x[u]);
+          s += (y[0] + y[1]) + (y[2] + y[3]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s += sa_lo<DT>(x[u][e]) + sa_hi<DT>(x[u][e]);
+        }
+      }
+      k += 256;
+      if (k >= n) return s;
+      more();
+    }
+  }
+};
 
 template <int DT>
 __global__ __launch_bounds__(256) void relpos_bwd_kernel(const SaMatParams p) {
@@ -131,8 +148,11 @@ __global__ __launch_bounds__(256) void relpos_bwd_kernel(const SaMatParams p) {
       const long at = (long)i + off;
       const int jl = (int)min(max(at - W + 1, 0L), (long)p.Lk), jr = (int)min(max(at + W, (long)jl), (long)p.Lk);
       const E* const row = g + (long)i * p.Lk;
-      aL += line_sum<DT>(row, 0, jl, lane);
-      aR += line_sum<DT>(row, jr, p.Lk, lane);
+      SaLine<DT> left, right;
+      left.fetch(row, 0, jl, lane);
+      right.fetch(row, jr, p.Lk, lane);
+      aL += left.sum();
+      aR += right.sum();
     }
     // the band: distance d of every row of the run
     for (int d = tid - (W - 1); d <= W - 1; d += 256) {

@@ -29,7 +29,7 @@ from .functional import linear
 F16, F32 = torch.float16, torch.float32
 DTYPES = {BF16: 0, F16: 1, F32: 2}                                    # DFOLD_DT_*
 REL_FAR, REL_MAX_DISTANCE = 256, 1024                                 # DFOLD_REL_*
-MAX_OFFSET, MAX_LEN = 1 << 29, 1 << 30
+MAX_OFFSET, MAX_LEN, MAX_ROW = 1 << 29, 1 << 30, 1 << 24
 ROWS, TILE = 128, 64                                                  # softmax rows / keys of a workgroup, rows of an LDS tile
 
 # The C ABI's descriptors as struct formats: one pack per call (filling ctypes structures field by field costs as much host time as the
@@ -79,7 +79,7 @@ def _call(name, *args, t):
     """one C ABI call on the current stream of t's device.  Arguments: a descriptor's bytes, pointers as c_void_p, whole numbers."""
     dev = t.get_device()
     fn = getattr(_lib.lib(), name)
-    if dev == torch.cuda.current_device():
+    if dev == torch._C._cuda_getDevice():
         check(fn(*args, c_void_p(torch._C._cuda_getCurrentRawStream(dev))), name)
     else:                                       # (launches go to the current device)
         with torch.cuda.device(dev):
@@ -97,13 +97,14 @@ def _same_device(dev, name, t):
 
 
 def _rows16(t):
-    """t itself if the kernels can read it as it lies -- dense last axis, every other stride a multiple of 16 bytes, aligned base --
-    else a dense copy"""
+    """t itself if the kernels can read it as it lies -- dense last axis, every other stride a multiple of 16 bytes, rows less than
+    2^24 elements apart, aligned base -- else a dense copy"""
     aligned = t.data_ptr() % 16 == 0
     if aligned and t.is_contiguous():           # (a multiple of 16 bytes per row: the head size is checked)
         return t
     v = 16 // t.element_size()
-    if t.numel() == 0 or (aligned and t.stride(-1) == 1 and all(s % v == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1)):
+    if t.numel() == 0 or (aligned and t.stride(-1) == 1 and all(s % v == 0 for s, n in zip(t.stride()[:-1], t.shape[:-1]) if n > 1) and
+                          (t.shape[1] == 1 or t.stride(1) < MAX_ROW)):
         return t
     return t.clone(memory_format=torch.contiguous_format)
 
@@ -111,8 +112,14 @@ def _rows16(t):
 def _strides(t):
     """strides of the three leading axes, 0 for axes of one entry (theirs may be anything)"""
     a, b, c, _ = t.stride()
+    if t.is_contiguous():
+        return a, b, c
     n = t.shape
     return (a if n[0] > 1 else 0, b if n[1] > 1 else 0, c if n[2] > 1 else 0)
+
+
+def _dense_like(t):
+    return torch.empty_like(t) if t.is_contiguous() else torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def _addr(t):
@@ -272,7 +279,7 @@ def _rope_forward(q, k, w_q, w_k, q_pos, k_pos, *opts):
     """results and the (readable) inputs they were computed from"""
     q, k = (None if t is None else _rows16(t) for t in (q, k))
     w_q, w_k = (None if t is None else t.contiguous() for t in (w_q, w_k))
-    oq, ok = (None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device) for t in (q, k))
+    oq, ok = (None if t is None else _dense_like(t) for t in (q, k))
     parts = _rope_part(q, oq, w_q, q_pos), _rope_part(k, ok, w_k, k_pos)
     if parts != (_NO_PART, _NO_PART):
         ref = q if q is not None else k
@@ -298,10 +305,10 @@ class QKNormRopeFn(Function):
             if x is None:
                 parts.append(_NO_PART)
                 continue
-            dx = grads[i] = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+            dx = grads[i] = _dense_like(x)
             dw = None
             if w is not None and ctx.needs_input_grad[2 + i]:
-                dw = grads[2 + i] = torch.empty(w.shape, dtype=F32, device=w.device) if x.numel() else torch.zeros(w.shape, dtype=F32, device=w.device)
+                dw = grads[2 + i] = torch.empty_like(w) if x.numel() else torch.zeros_like(w)
                 if ws is None:
                     ws = torch.empty(_lib.lib().dfold_qk_norm_rope_ws(), dtype=F32, device=ref.device)
             parts.append(_rope_part(x, dx, w, pos, _rows16(g), dw))
@@ -371,20 +378,45 @@ def qk_norm_rope(q, k, w_q=None, w_k=None, q_positions=None, k_positions=None, *
 # attention of one sequence over another
 # ------------------------------------------------------------------------------------------------
 
-def _parts(groups, units, n_cu, least):
-    """Cut factor of a launch of `groups` workgroups that each walk `units` tiles: as many parts as bring the launch to two workgroups
-    per CU, each of at least `least` tiles (below that, writing and adding the parts costs more than the idle CUs)."""
-    return max(1, min(1024, 2 * n_cu // max(groups, 1), units // least))
+_PARTS = (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256, 384, 512, 768, 1024)
 
 
+def _parts(groups, units, n_cu, join, alone=False):
+    """Cut factor of a launch of `groups` workgroups that each walk `units` tiles.  Estimated in tile times: the longest part, times the
+    rounds that w = workgroups per CU make (two share a CU, each at two thirds of its speed; `alone`: a workgroup fills its CU), plus
+    `join` for writing and adding the parts.  Measured against it, us: 94 tiles of 8 groups: 102 whole, 14.4 in 24 parts, 13.9 in 32,
+    15.4 in 47; 16 tiles of 256 groups: 24 whole, 28 in 2; 256 tiles of 128 groups, ragged: 161 in 4, 178 in 6."""
+    best, best_cost = 1, None
+    for parts in _PARTS:
+        if parts > max(units, 1):
+            break
+        w = groups * parts / n_cu
+        rounds = math.ceil(w) if alone else 1.5 * (w // 2) + (0.0 if w % 2 == 0 else 1.0 if w % 2 <= 1 else 1.5)
+        cost = -(-units // parts) * max(rounds, 1.0) + (join if parts > 1 else 0)
+        if best_cost is None or cost * 1.05 < best_cost:
+            best, best_cost = parts, cost
+    return best
+
+
+@functools.lru_cache(maxsize=4096)
 def _attn_plan(B, Lq, Lk, H, Hkv, rel_width, n_cu):
     """(pack, splits) of the forward.  pack: the query heads of a group share tiles if that at least halves the number of row blocks
     (their bias rows have to fit 32 KB of LDS); K and V are then read once per group."""
     G = H // Hkv
     blocks, packed = -(-Lq // ROWS) * G, -(-(Lq * G) // ROWS)
     pack = G if 2 * packed <= blocks and G * rel_width * 4 <= 32768 else 1
-    groups = B * (H // pack) * -(-(Lq * pack) // ROWS)
-    return pack, _parts(groups, -(-Lk // TILE), n_cu, 2)
+    return pack, _parts(B * (H // pack) * -(-(Lq * pack) // ROWS), -(-Lk // TILE), n_cu, 5)
+
+
+@functools.lru_cache(maxsize=4096)
+def _grad_plan(B, Lq, Lk, H, Hkv, D, num_buckets, n_cu):
+    """(splits_q, splits_k, floats of delta, floats of delta and workspace) of the backward"""
+    nrb, nkb = -(-Lq // ROWS), -(-Lk // ROWS)
+    splits_q = _parts(B * H * nrb, -(-Lk // TILE), n_cu, 6)
+    splits_k = _parts(B * Hkv * nkb, (H // Hkv) * -(-Lq // TILE), n_cu, 6, alone=D > 64)
+    delta = (B * H * Lq * (1 + splits_q if splits_q > 1 else 1) + 3) // 4 * 4
+    ws = (splits_q * B * Lq * H * D if splits_q > 1 else 0) + (2 * splits_k * B * Lk * Hkv * D if splits_k > 1 else 0)
+    return splits_q, splits_k, delta, delta + ws + splits_k * B * H * nkb * num_buckets
 
 
 def _attn_desc(q, k, v, o, lse, ws, key_mask, kv_lens, rel, scale, pack=1, splits=1):
@@ -400,7 +432,7 @@ def _attn_forward(train, q, k, v, table, key_mask, kv_lens, q_offsets, q_offset,
     B, Lq, H, D = q.shape
     Lk, Hkv = k.shape[1], k.shape[2]
     dev = q.device
-    o = torch.empty((B, Lq, H, D), dtype=q.dtype, device=dev)
+    o = _dense_like(q)
     lse = torch.empty((B, H, Lq), dtype=F32, device=dev) if train else None
     if table is not None and not table.is_contiguous():
         table = table.contiguous()
@@ -431,24 +463,22 @@ class CrossAttentionFn(Function):
         q_offset, max_distance, bidirectional, scale = ctx.opts
         B, Lq, H, D = q.shape
         Lk, Hkv = k.shape[1], k.shape[2]
-        dev, dt = q.device, q.dtype
-        new = torch.zeros if o.numel() == 0 or k.numel() == 0 else torch.empty
-        dq, dk, dv = new(q.shape, dtype=dt, device=dev), new(k.shape, dtype=dt, device=dev), new(k.shape, dtype=dt, device=dev)
-        dtable = None if table is None else new(table.shape, dtype=F32, device=dev)
-        if new is torch.empty:
-            g = _rows16(g)
-            n_cu = ops.cu_count(dev)
-            nrb, nkb = -(-Lq // ROWS), -(-Lk // ROWS)
-            splits_q = _parts(B * H * nrb, -(-Lk // TILE), n_cu, 4)
-            splits_k = _parts(B * Hkv * nkb, (H // Hkv) * -(-Lq // TILE), n_cu, 4)
-            n = (splits_q * q.numel() if splits_q > 1 else 0) + (2 * splits_k * k.numel() if splits_k > 1 else 0)    # (multiples of 8)
-            rel = _NO_REL
+        dtable = None
+        if o.numel() == 0 or k.numel() == 0:
+            dq, dk, dv = torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v)
             if table is not None:
-                rel = _rel_desc(table, table.shape[0], max_distance, bidirectional, q_offset, q_offsets)
-                n += splits_k * B * H * nkb * table.shape[0]
-            delta = torch.empty((1 + splits_q if splits_q > 1 else 1, B, H, Lq), dtype=F32, device=dev)
-            ws = torch.empty(n, dtype=F32, device=dev) if n else None
-            grad = _GRAD.pack(g.data_ptr(), *_strides(g), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta.data_ptr(), _addr(dtable), _addr(ws),
+                dtable = torch.zeros_like(table)
+        else:
+            g = _rows16(g)
+            dq, dk, dv = _dense_like(q), _dense_like(k), _dense_like(v)
+            rel, nb = _NO_REL, 0
+            if table is not None:
+                dtable, nb = torch.empty_like(table), table.shape[0]
+                rel = _rel_desc(table, nb, max_distance, bidirectional, q_offset, q_offsets)
+            splits_q, splits_k, n_delta, n = _grad_plan(B, Lq, Lk, H, Hkv, D, nb, ops.cu_count(q.device))
+            ws = torch.empty(n, dtype=F32, device=q.device)          # delta, then the workspace
+            delta = ws.data_ptr()
+            grad = _GRAD.pack(g.data_ptr(), *_strides(g), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta, _addr(dtable), delta + 4 * n_delta,
                               splits_q, splits_k)
             _call("dfold_seq_attn_bwd", _attn_desc(q, k, v, o, lse, None, key_mask, kv_lens, rel, scale), grad, t=q)
         need = ctx.needs_input_grad
@@ -477,8 +507,8 @@ def cross_attention(q, k, v, *, key_mask=None, kv_lens=None, rel_table=None, max
         raise ValueError("the query heads must be a multiple of the key heads")
     if D % 8 or not 8 <= D <= 128:
         raise ValueError("the head size must be a multiple of 8, at most 128")
-    if Lq > MAX_LEN or Lk > MAX_LEN:
-        raise ValueError("sequences are at most 2^30 long")
+    if Lq > MAX_LEN or Lk > MAX_LEN or H * D >= MAX_ROW:
+        raise ValueError("sequences are at most 2^30 long, rows (heads x head size) below 2^24")
     _same_device(dev, "k", k)
     _same_device(dev, "v", v)
     if key_mask is not None:
@@ -510,8 +540,8 @@ def cross_attention(q, k, v, *, key_mask=None, kv_lens=None, rel_table=None, max
     else:
         q_offset = 0
     scale = D ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale):
-        raise ValueError("scale must be finite")
+    if not math.isfinite(scale) or scale == 0:
+        raise ValueError("scale must be finite and not 0")
     _require_cuda(q)
     args = (q, k, v, rel_table, key_mask, kv_lens, q_offsets, q_offset, max_distance, bool(bidirectional), scale)
     if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (rel_table is not None and rel_table.requires_grad)):

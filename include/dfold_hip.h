@@ -634,7 +634,7 @@ int dfold_relpos_bwd(const dfold_rel_bias* rel, const void* g, int32_t dtype, in
 int dfold_relpos_ws(int32_t H, int32_t Lq, int32_t num_buckets);
 
 /* o = softmax(scale q k^T + bias) v.  q [B][Lq][H][D], k, v [B][Lk][Hkv][D], o like q: bf16 or f16, the last axis dense, other
- * strides in elements, multiples of 8, base pointers 16-byte aligned; D a multiple of 8, <= 128; H a multiple of Hkv (query head h
+ * strides in elements, multiples of 8, row strides (*_sl) below 2^24, base pointers 16-byte aligned; D a multiple of 8, <= 128; H a multiple of Hkv (query head h
  * reads key head h / (H / Hkv)).  Keys j >= kv_lens[b] and keys with key_mask[b * mask_sb + j] == 0 do not exist: their K and V
  * are never used (they may hold NaN); a row without any key gives zeros.
  *   lse [B][H][Lq] fp32 (optional): log2 of the row's sum of exp2 (logits x log2 e); +inf for a row without keys.

@@ -326,12 +326,14 @@ def test_attention_split_keys_equal_whole(D):
     plan = S._parts
     try:
         for parts in (1, 2, 3, 7, 15, 40):
-            S._parts = lambda groups, units, n_cu, least, n=parts: n
+            S._parts = lambda *a, n=parts, **kw: n
+            S._attn_plan.cache_clear(), S._grad_plan.cache_clear()
             got = run(q, k, v, g, **kw)
             for n in ref:
                 within(f"{n} in {parts} parts", got[n], ref[n])
     finally:
         S._parts = plan
+        S._attn_plan.cache_clear(), S._grad_plan.cache_clear()
 
 
 # ---- relative position bias ---------------------------------------------------------------------------------------------------------
