@@ -77,7 +77,6 @@ struct SaTile {
   static constexpr int PITCH = DP * 2;
   static constexpr int BYTES = SA_KT * PITCH;
   static constexpr int KS = DP / 16, NT = DP / 32;         // 16-deep steps, 32-wide column tiles
-  static constexpr int NCH = SA_KT * CPR / (64 * SA_WAVES);  // chunks per thread of a staged tile
   static __device__ __forceinline__ int key(int row) {
     if constexpr (CPR == 16) return ((row & 3) << 2) | ((row >> 2) & 3);
     if constexpr (CPR == 8) return (((row >> 1) & 1) << 2) | ((row >> 2) & 3);
@@ -92,15 +91,16 @@ template <int DP>
 struct SaAddr {
   using T = SaTile<DP>;
   int row[T::KS], col[T::NT][2];
-  __device__ __forceinline__ SaAddr(int lane) {
+  // shift: rows added to every r0 (a multiple of 16, the same for the wave)
+  __device__ __forceinline__ SaAddr(int lane, int shift = 0) {
     const int h = lane >> 5, i = lane & 15;
 #pragma unroll
-    for (int ks = 0; ks < T::KS; ++ks) row[ks] = T::off(lane & 31, 2 * ks + h);
+    for (int ks = 0; ks < T::KS; ++ks) row[ks] = T::off(lane & 31, 2 * ks + h) + shift * T::PITCH;
 #pragma unroll
     for (int dt = 0; dt < T::NT; ++dt)
 #pragma unroll
       for (int x = 0; x < 2; ++x)
-        col[dt][x] = T::off(8 * x + 4 * h + (i >> 2), 4 * dt + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) + (i & 1) * 8;
+        col[dt][x] = T::off(8 * x + 4 * h + (i >> 2), 4 * dt + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) + (i & 1) * 8 + shift * T::PITCH;
   }
   __device__ __forceinline__ sa_u32x4 rows(const char* t, int r0, int ks) const { return *(const sa_u32x4*)(t + row[ks] + r0 * T::PITCH); }
   __device__ __forceinline__ sa_u32x4 cols(const char* t, int r0, int dt) const {
@@ -111,39 +111,53 @@ struct SaAddr {
   }
 };
 
-// Registers of a tile on its way to LDS: SA_KT rows of a [rows][D] matrix with row stride `rs` elements (< SA_MAX_ROW).  The loads go
-// through a buffer descriptor that ends with the last row there is: a tile costs no address arithmetic on the vector unit and rows past
-// the end (and columns past D) come back as zeros.  mask(): one bit per row, zeroes rows whose content must not be used.
+// SA_KT (or ROWS) rows of a [rows][D] matrix with row stride `rs` elements (< SA_MAX_ROW) into an LDS tile, by LDS-DMA: no registers and
+// no LDS write instructions.  A wave's instruction fills 1 KB of the tile in lane order, so the chunk permutation is applied to the
+// source.  Rows past the last one repeat it (never out of range; their content is masked by the caller), columns past D repeat
+// column 0 (they meet zeros of the other operand, or results that are not stored).
 #define SA_MAX_ROW (1 << 24)
-template <int DP>
-struct SaStage {
+typedef __attribute__((address_space(3))) void* sa_lds_ptr;
+template <int DP, int NW = SA_WAVES, int ROWS = SA_KT>
+struct SaDma {
   using T = SaTile<DP>;
-  sa_u32x4 v[T::NCH];
-  unsigned voff[T::NCH];
-  int lds;
-  __device__ __forceinline__ void init(long rs, int D, int tid) {
-    const int cc = tid % T::CPR;
-#pragma unroll
-    for (int i = 0; i < T::NCH; ++i) voff[i] = cc * 8 < D ? (unsigned)((tid / T::CPR + i * (64 * SA_WAVES / T::CPR)) * rs + cc * 8) * 2u : 0x80000000u;
-    lds = T::off(tid / T::CPR, cc);
+  static constexpr int NCH = ROWS * T::CPR / (64 * NW);    // instructions per wave
+  static constexpr int STEP = 64 * NW / T::CPR;            // rows between a lane's chunks (a multiple of 16: one permutation key)
+  static_assert(NCH >= 1 && STEP % 16 == 0, "whole instructions, one key per lane");
+  int row, col;
+  unsigned rs2, voff;      // bytes of a row, of this lane's first chunk
+  __device__ __forceinline__ SaDma(long rs, int D, int tid) {
+    row = tid / T::CPR;
+    const int cc = (tid % T::CPR) ^ T::key(row);
+    col = cc * 8 < D ? cc * 16 : 0;
+    rs2 = (unsigned)rs * 2u;
+    voff = row * rs2 + col;
   }
-  // rows row0 .. of a matrix of `end` > row0 rows
-  __device__ __forceinline__ void load(const char* base, long rs, int row0, int end, int D) {
-    const unsigned bytes = (unsigned)(((long)(min(end - row0, SA_KT) - 1) * rs + D) * 2);
-    const __amdgpu_buffer_rsrc_t r = __builtin_amdgcn_make_buffer_rsrc((void*)(base + (long)row0 * rs * 2), 0, bytes, 0x00020000);
+  // rows row0 .. of a matrix of `end` > row0 rows -> tile; w: the wave's number in the workgroup
+  __device__ __forceinline__ void load(const char* base, int row0, int end, char* tile, int w) const {
+    const char* const src = base + (long)row0 * rs2;
+    const int last = end - 1 - row0;
+    if (last >= ROWS - 1) {
 #pragma unroll
-    for (int i = 0; i < T::NCH; ++i) v[i] = __builtin_amdgcn_raw_buffer_load_b128(r, voff[i], 0, 0);
+      for (int i = 0; i < NCH; ++i)
+        __builtin_amdgcn_global_load_lds((const void*)(src + (long)(i * STEP) * rs2 + voff), (sa_lds_ptr)(tile + (i * NW + w) * 1024), 16, 0, 0);
+    } else {
+#pragma unroll
+      for (int i = 0; i < NCH; ++i)
+        __builtin_amdgcn_global_load_lds((const void*)(src + (min(row + i * STEP, last) * rs2 + col)), (sa_lds_ptr)(tile + (i * NW + w) * 1024), 16, 0, 0);
+    }
   }
-  __device__ __forceinline__ void mask(unsigned long live, int tid) {
+  // rows whose bit is 0 become zeros (this thread's share; between two barriers)
+  __device__ __forceinline__ void zero(unsigned long live, char* tile, int tid) const {
 #pragma unroll
-    for (int i = 0; i < T::NCH; ++i)
-      if (!((live >> (tid / T::CPR + i * (64 * SA_WAVES / T::CPR))) & 1)) v[i] = (sa_u32x4){0u, 0u, 0u, 0u};
-  }
-  __device__ __forceinline__ void store(char* t) const {
-#pragma unroll
-    for (int i = 0; i < T::NCH; ++i) *(sa_u32x4*)(t + lds + i * (64 * SA_WAVES / T::CPR) * T::PITCH) = v[i];
+    for (int i = 0; i < NCH; ++i)
+      if (!((live >> (row + i * STEP)) & 1)) *(sa_u32x4*)(tile + (i * 64 * NW + tid) * 16) = (sa_u32x4){0u, 0u, 0u, 0u};
   }
 };
+// every DMA of this wave has landed, then everybody's
+__device__ __forceinline__ void sa_landed() {
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+}
 template <int I>
 struct SaInt {
   static constexpr int value = I;

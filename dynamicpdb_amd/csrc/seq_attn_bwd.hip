@@ -127,29 +127,27 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_dq_kernel(const SaB
 
   float left = 0.f;          // row sum of dS
   const SaAddr<DP> ad(lane);
-  SaStage<DP> sk, sv;
-  sk.init(p.k_sl, p.D, tid);
-  sv.init(p.v_sl, p.D, tid);
+  const SaDma<DP> ldk(p.k_sl, p.D, tid), ldv(p.v_sl, p.D, tid);
   int kmask = 0;
-  auto fetch = [&](int t) {
-    sk.load(kb_, p.k_sl, t * SA_KT, kv_end, p.D);
-    sv.load(vb_, p.v_sl, t * SA_KT, kv_end, p.D);
+  auto fetch = [&](int t, char* tile) {
+    ldk.load(kb_, t * SA_KT, kv_end, tile, w);
+    ldv.load(vb_, t * SA_KT, kv_end, tile + T::BYTES, w);
     const int key = t * SA_KT + lane;
     kmask = key < kv_end ? (mb_ ? mb_[key] : 1) : 0;
   };
   auto step = [&](int t, auto stage) {
     char* const lk = smem + decltype(stage)::value * 2 * T::BYTES;
     char* const lv = lk + T::BYTES;
+    sa_landed();
     const unsigned long live = __ballot(kmask != 0);
+    if (t + 1 < t1) fetch(t + 1, smem + (1 - decltype(stage)::value) * 2 * T::BYTES);
     if (live != ~0ul) {
-      sk.mask(live, tid);
-      sv.mask(live, tid);
+      if (live == 0) return;
+      ldk.zero(live, lk, tid);
+      ldv.zero(live, lv, tid);
+      __syncthreads();
     }
-    sk.store(lk);
-    sv.store(lv);
-    __syncthreads();
-    if (t + 1 < t1) fetch(t + 1);
-    if (live == 0 || !wave_on) return;
+    if (!wave_on) return;
 #pragma unroll
     for (int kb = 0; kb < 2; ++kb) {
       f32x16 s, dp;
@@ -184,7 +182,7 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_dq_kernel(const SaB
       }
     }
   };
-  if (t0 < t1) fetch(t0);
+  if (t0 < t1) fetch(t0, smem);
   for (int t = t0; t < t1; t += 2) {
     step(t, SaInt<0>());
     if (t + 1 < t1) step(t + 1, SaInt<1>());
@@ -218,12 +216,24 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_dq_kernel(const SaB
   }
 }
 
+// Four waves of 32 keys each, K^T and V^T operands in registers.  At D = 128 that takes more than 256 registers: one wave per SIMD, and
+// nothing runs under its products.  PAIR: eight waves, two for the same 32 keys, one per 32-query half of a tile, V^T operands from LDS;
+// the two sums meet in LDS at the end.
+template <int DP, bool REL>
+struct SaDkvCfg {
+  static constexpr bool PAIR = DP == 128 && !REL;      // (with a bias the eight waves' blocks of dS would not fit LDS)
+  static constexpr int WAVES = PAIR ? 2 * SA_WAVES : SA_WAVES;
+  static constexpr int LDS = 4 * SaTile<DP>::BYTES + 4 * SA_KT * 4 + (PAIR ? SA_ROWS * SaTile<DP>::PITCH : 0);
+};
 template <int DT, int DP, bool REL>
-__global__ __launch_bounds__(64 * SA_WAVES, DP == 128 ? 1 : 2) void seq_attn_dkv_kernel(const SaBwdParams p) {
+__global__ __launch_bounds__((64 * SaDkvCfg<DP, REL>::WAVES), (DP == 128 && REL ? 1 : 2)) void seq_attn_dkv_kernel(const SaBwdParams p) {
   using T = SaTile<DP>;
   constexpr int KS = T::KS, NT = T::NT;
+  constexpr bool PAIR = SaDkvCfg<DP, REL>::PAIR;
+  constexpr int NW = SaDkvCfg<DP, REL>::WAVES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* const ldsL = (float*)(smem + 4 * T::BYTES);            // [stage][log-sum | delta][SA_KT]
+  char* const ldsV = smem + 4 * T::BYTES + 4 * SA_KT * 4;
   float* const ldsB = ldsL + 4 * SA_KT;
   float* const ldsH = ldsB + (REL ? 2 * p.rel.W + 1 : 0);       // [wave][distance]
   const int hn = REL ? 2 * (p.rel.W + SA_REACH) + 1 : 0;
@@ -234,7 +244,8 @@ __global__ __launch_bounds__(64 * SA_WAVES, DP == 128 ? 1 : 2) void seq_attn_dkv
   const int kbk = id % nkb; id /= nkb;
   const int sp = id % p.splits_k; id /= p.splits_k;
   const int hkv = id % p.Hkv, b = id / p.Hkv;
-  const int key_w = kbk * SA_ROWS + w * 32, key = key_w + l31;
+  const int wk = w & (SA_WAVES - 1), half = w / SA_WAVES;
+  const int key_w = kbk * SA_ROWS + wk * 32, key = key_w + l31;
 
   int kv_end = p.Lk;
   if (p.kv_lens) kv_end = min(max(p.kv_lens[b], 0), p.Lk);
@@ -246,20 +257,26 @@ __global__ __launch_bounds__(64 * SA_WAVES, DP == 128 ? 1 : 2) void seq_attn_dkv
   const int nqt = (p.Lq + SA_KT - 1) / SA_KT, nu = G * nqt, per = (nu + p.splits_k - 1) / p.splits_k;
   const int u0 = sp * per, u1 = wg_on ? min(nu, u0 + per) : 0;
 
-  sa_u32x4 kf[KS], vf[KS];
+  sa_u32x4 kf[KS], vf[PAIR ? 1 : KS];
   {
     const char* sk = p.k + ((long)b * p.k_sb + (long)key * p.k_sl + (long)hkv * p.k_sh) * 2;
     const char* sv = p.v + ((long)b * p.v_sb + (long)key * p.v_sl + (long)hkv * p.v_sh) * 2;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
       const int d = ks * 16 + h * 8;
-      kf[ks] = vf[ks] = (sa_u32x4){0u, 0u, 0u, 0u};
-      if (key_on && d < p.D) {
-        kf[ks] = *(const sa_u32x4*)(sk + d * 2);
-        vf[ks] = *(const sa_u32x4*)(sv + d * 2);
+      kf[ks] = (sa_u32x4){0u, 0u, 0u, 0u};
+      if (key_on && d < p.D) kf[ks] = *(const sa_u32x4*)(sk + d * 2);
+      if constexpr (!PAIR) {
+        vf[ks] = (sa_u32x4){0u, 0u, 0u, 0u};
+        if (key_on && d < p.D) vf[ks] = *(const sa_u32x4*)(sv + d * 2);
       }
     }
   }
+  if constexpr (PAIR)
+    if (u0 < u1) {
+      const SaDma<DP, NW, SA_ROWS> ldv(p.v_sl, p.D, tid);
+      ldv.load(p.v + ((long)b * p.v_sb + (long)hkv * p.v_sh) * 2, kbk * SA_ROWS, kv_end, ldsV, w);
+    }
   f32x16 dk[NT], dv[NT];
 #pragma unroll
   for (int i = 0; i < NT; ++i)
@@ -300,17 +317,16 @@ __global__ __launch_bounds__(64 * SA_WAVES, DP == 128 ? 1 : 2) void seq_attn_dkv
         for (int j = tid; j < p.num_buckets; j += 64 * SA_WAVES) table_part(hkv * G + g)[j] = 0.f;
   }
 
-  const SaAddr<DP> ad(lane);
-  SaStage<DP> sq, sg;
-  sq.init(p.q_sl, p.D, tid);
-  sg.init(p.do_sl, p.D, tid);
+  const SaAddr<DP> ad(lane, half * 32);
+  const SaDma<DP, NW> ldq(p.q_sl, p.D, tid), ldg(p.do_sl, p.D, tid);
+  const char* const lv = ldsV + (wk - half) * 32 * T::PITCH;
   float lse_r = 0.f, del_r = 0.f;
   // position in the walk of the unit that is fetched next, and of the one that is worked on
   int fg = u0 / nqt, fq = (u0 - fg * nqt) * SA_KT, wg = fg, wq = fq;
-  auto fetch = [&]() {
+  auto fetch = [&](char* tile) {
     const int head = hkv * G + fg;
-    sq.load(p.q + ((long)b * p.q_sb + (long)head * p.q_sh) * 2, p.q_sl, fq, p.Lq, p.D);
-    sg.load(p.d_o + ((long)b * p.do_sb + (long)head * p.do_sh) * 2, p.do_sl, fq, p.Lq, p.D);
+    ldq.load(p.q + ((long)b * p.q_sb + (long)head * p.q_sh) * 2, fq, p.Lq, tile, w);
+    ldg.load(p.d_o + ((long)b * p.do_sb + (long)head * p.do_sh) * 2, fq, p.Lq, tile + T::BYTES, w);
     if (tid < SA_KT) {
       const int qi = fq + tid;
       const long r = ((long)b * p.H + head) * p.Lq + qi;
@@ -334,27 +350,26 @@ __global__ __launch_bounds__(64 * SA_WAVES, DP == 128 ? 1 : 2) void seq_attn_dkv
       }
     }
     if ((wq += SA_KT) >= p.Lq) { wq = 0; ++wg; }
-    sq.store(lq);
-    sg.store(lg);
     if (tid < SA_KT) {
       ll[tid] = lse_r;
       ll[SA_KT + tid] = del_r;
     }
-    __syncthreads();
-    if (more) fetch();
+    sa_landed();
+    if (more) fetch(smem + (1 - decltype(stage)::value) * 2 * T::BYTES);
     if (!wave_on) return;
 #pragma unroll
-    for (int qb = 0; qb < 2; ++qb) {
-      if (q0 + qb * 32 >= p.Lq) continue;
+    for (int qb = 0; qb < (PAIR ? 1 : 2); ++qb) {
+      const int qs = (PAIR ? half : qb) * 32;
+      if (q0 + qs >= p.Lq) continue;
       f32x16 s, dp;
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         s = sa_mfma<DT>(ad.rows(lq, qb * 32, ks), kf[ks], s);
-        dp = sa_mfma<DT>(ad.rows(lg, qb * 32, ks), vf[ks], dp);
+        dp = sa_mfma<DT>(ad.rows(lg, qb * 32, ks), PAIR ? ad.rows(lv, 0, ks) : vf[PAIR ? 0 : ks], dp);
       }
-      const int qlo = q0 + qb * 32 + off, qhi = qlo + 31;
+      const int qlo = q0 + qs + off, qhi = qlo + 31;
       const int far = !REL ? 0 : key_w - qhi >= p.rel.W ? 1 : key_w + 31 - qlo <= -p.rel.W ? -1 : 0;
       if constexpr (REL) {
         if (far) {
@@ -369,13 +384,15 @@ __global__ __launch_bounds__(64 * SA_WAVES, DP == 128 ? 1 : 2) void seq_attn_dkv
       }
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
-        const f32x4 rl = *(const f32x4*)(ll + qb * 32 + g * 8 + h * 4);
-        const f32x4 rd = *(const f32x4*)(ll + SA_KT + qb * 32 + g * 8 + h * 4);
+        const f32x4 rl = *(const f32x4*)(ll + qs + g * 8 + h * 4);
+        const f32x4 rd = *(const f32x4*)(ll + SA_KT + qs + g * 8 + h * 4);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = g * 4 + e;
-          const float x = REL ? s[r] + rl[e] : __builtin_fmaf(s[r], p.sl2, rl[e]);
-          s[r] = key_on ? sa_exp2(x) : 0.f;
+          // a masked key's column holds products with zeros: whatever comes of them stays in that column, which is not stored (only the
+          // bias gradient sums over columns)
+          const float x = sa_exp2(REL ? s[r] + rl[e] : __builtin_fmaf(s[r], p.sl2, rl[e]));
+          s[r] = REL ? (key_on ? x : 0.f) : x;
           dp[r] = s[r] * (dp[r] - rd[e]);
         }
       }
@@ -418,7 +435,7 @@ __global__ __launch_bounds__(64 * SA_WAVES, DP == 128 ? 1 : 2) void seq_attn_dkv
       }
     }
   };
-  if (u0 < u1) fetch();
+  if (u0 < u1) fetch(smem);
   for (int u = u0; u < u1; u += 2) {
     step(u + 1 < u1, SaInt<0>());
     if (u + 1 < u1) step(u + 2 < u1, SaInt<1>());
@@ -426,6 +443,23 @@ __global__ __launch_bounds__(64 * SA_WAVES, DP == 128 ? 1 : 2) void seq_attn_dkv
 
   if constexpr (REL)
     if (head_in >= 0) flush(head_in);
+  if constexpr (PAIR) {
+    // the second wave of a pair hands its sums over, 64 KB at a time through the tiles' memory
+    f32x16* const acc = (f32x16*)smem + (wk * NT) * 64 + lane;
+    auto join = [&](f32x16(&x)[NT]) {
+      __syncthreads();
+      if (half)
+#pragma unroll
+        for (int i = 0; i < NT; ++i) acc[i * 64] = x[i];
+      __syncthreads();
+      if (!half)
+#pragma unroll
+        for (int i = 0; i < NT; ++i) x[i] += acc[i * 64];
+    };
+    join(dk);
+    join(dv);
+    if (half) return;
+  }
   if (key >= p.Lk) return;
   const long r1 = ((long)b * p.Lk + key) * p.Hkv + hkv, n = (long)p.B * p.Lk * p.Hkv;
 #pragma unroll
@@ -437,8 +471,8 @@ __global__ __launch_bounds__(64 * SA_WAVES, DP == 128 ? 1 : 2) void seq_attn_dkv
       f32x4 a, c;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        a[e] = dk[i][g * 4 + e] * p.scale;
-        c[e] = dv[i][g * 4 + e];
+        a[e] = key_on ? dk[i][g * 4 + e] * p.scale : 0.f;
+        c[e] = key_on ? dv[i][g * 4 + e] : 0.f;
       }
       if (p.splits_k == 1) {
         *(uint2*)(p.dk + (r1 * p.D + d) * 2) = (uint2){sa_pack2<DT>(a[0], a[1]), sa_pack2<DT>(a[2], a[3])};
@@ -473,16 +507,17 @@ __global__ __launch_bounds__(256) void seq_attn_delta_kernel(float* __restrict__
 }
 
 template <typename K>
-static int sa_launch_bwd(K kernel, const SaBwdParams& p, long nwg, int lds, hipStream_t st) {
+static int sa_launch_bwd(K kernel, const SaBwdParams& p, long nwg, int waves, int lds, hipStream_t st) {
   if (lds > 65536 && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
     return DFOLD_ELAUNCH;
-  DFOLD_LAUNCH(kernel, dim3((unsigned)nwg), dim3(64 * SA_WAVES), lds, st, p);
+  DFOLD_LAUNCH(kernel, dim3((unsigned)nwg), dim3(64 * waves), lds, st, p);
   return dfold_check_launch();
 }
 template <int DT, int DP, bool REL>
 static int sa_bwd_dp(const SaBwdParams& p, hipStream_t st) {
   const int bias = REL ? (2 * p.rel.W + 1) * 4 : 0, hist = REL ? SA_WAVES * (2 * (p.rel.W + SA_REACH) + 1 + SA_DIAG) * 4 : 0;
-  int rc = sa_launch_bwd(seq_attn_dq_kernel<DT, DP, REL>, p, (long)p.nrb * p.splits_q * p.H * p.B, 4 * SaTile<DP>::BYTES + bias, st);
+  int rc = sa_launch_bwd(seq_attn_dq_kernel<DT, DP, REL>, p, (long)p.nrb * p.splits_q * p.H * p.B, SA_WAVES,
+                         4 * SaTile<DP>::BYTES + bias, st);
   if (rc != DFOLD_OK) return rc;
   if (p.splits_q > 1) {
     const long n8 = (long)p.B * p.Lq * p.H * p.D / 8;
@@ -493,7 +528,8 @@ static int sa_bwd_dp(const SaBwdParams& p, hipStream_t st) {
     if ((rc = dfold_check_launch()) != DFOLD_OK) return rc;
   }
   const long nkb = (p.Lk + SA_ROWS - 1) / SA_ROWS;
-  rc = sa_launch_bwd(seq_attn_dkv_kernel<DT, DP, REL>, p, nkb * p.splits_k * p.Hkv * p.B, 4 * SaTile<DP>::BYTES + 4 * SA_KT * 4 + bias + hist, st);
+  rc = sa_launch_bwd(seq_attn_dkv_kernel<DT, DP, REL>, p, nkb * p.splits_k * p.Hkv * p.B, SaDkvCfg<DP, REL>::WAVES,
+                     SaDkvCfg<DP, REL>::LDS + bias + hist, st);
   if (rc != DFOLD_OK) return rc;
   if (REL) {
     DFOLD_LAUNCH(seq_dtable_kernel, dim3(p.H, (p.num_buckets + 63) / 64), dim3(1024), 0, st, (const float*)p.ws_t, p.dtable, p.num_buckets,

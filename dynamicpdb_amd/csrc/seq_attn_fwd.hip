@@ -3,9 +3,9 @@
 //
 // A workgroup owns 128 softmax rows of one key head (4 waves x 32 rows; with pack > 1 the rows of the query heads of a group are
 // interleaved, head fastest, so that one token of a grouped layer fills its tile), walks its part of the keys in tiles of 64 and
-// keeps S, P and O in registers; K and V tiles go registers -> LDS one tile ahead of the arithmetic, two LDS stages, one barrier
-// per tile.  Key masks are one ballot per tile: an empty tile is skipped, a full one takes no mask arithmetic, K / V rows of masked
-// keys are zeroed on the way into LDS (0 * NaN would not stay 0).
+// keeps S, P and O in registers; K and V tiles go to LDS by DMA one tile ahead of the arithmetic, two stages, one barrier per tile.
+// Key masks are one ballot per tile: an empty tile is skipped, a full one takes no mask arithmetic, K / V rows of masked keys are
+// zeroed in LDS behind one more barrier (0 * NaN would not stay 0).
 // Few rows and many keys: the key axis is cut over workgroups (splits), partial results meet in seq_attn_combine_kernel in split
 // order (deterministic).
 #include "seq_attn.h"
@@ -95,29 +95,27 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_fwd_kernel(const Sa
   float m = -INFINITY, l = 0.f;
 
   const SaAddr<DP> ad(lane);
-  SaStage<DP> sk, sv;
-  sk.init(p.k_sl, p.D, tid);
-  sv.init(p.v_sl, p.D, tid);
+  const SaDma<DP> ldk(p.k_sl, p.D, tid), ldv(p.v_sl, p.D, tid);
   int kmask = 0;
-  auto fetch = [&](int t) {
-    sk.load(kb_, p.k_sl, t * SA_KT, kv_end, p.D);
-    sv.load(vb_, p.v_sl, t * SA_KT, kv_end, p.D);
+  auto fetch = [&](int t, char* tile) {
+    ldk.load(kb_, t * SA_KT, kv_end, tile, w);
+    ldv.load(vb_, t * SA_KT, kv_end, tile + T::BYTES, w);
     const int key = t * SA_KT + lane;
     kmask = key < kv_end ? (mb_ ? mb_[key] : 1) : 0;
   };
   auto step = [&](int t, auto stage) {
     char* const lk = smem + decltype(stage)::value * 2 * T::BYTES;
     char* const lv = lk + T::BYTES;
+    sa_landed();
     const unsigned long live = __ballot(kmask != 0);
+    if (t + 1 < t1) fetch(t + 1, smem + (1 - decltype(stage)::value) * 2 * T::BYTES);
     if (live != ~0ul) {
-      sk.mask(live, tid);
-      sv.mask(live, tid);
+      if (live == 0) return;
+      ldk.zero(live, lk, tid);
+      ldv.zero(live, lv, tid);
+      __syncthreads();
     }
-    sk.store(lk);
-    sv.store(lv);
-    __syncthreads();
-    if (t + 1 < t1) fetch(t + 1);
-    if (live == 0 || !wave_on) return;
+    if (!wave_on) return;
 
     // S^T: keys x rows
     f32x16 s[2];
@@ -187,7 +185,7 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_fwd_kernel(const Sa
 #pragma unroll
       for (int i = 0; i < NT; ++i) O[i] = sa_mfma<DT>(ad.cols(lv, c * 16, i), pf[c], O[i]);
   };
-  if (t0 < t1) fetch(t0);
+  if (t0 < t1) fetch(t0, smem);
   for (int t = t0; t < t1; t += 2) {
     step(t, SaInt<0>());
     if (t + 1 < t1) step(t + 1, SaInt<1>());
