@@ -3,7 +3,7 @@
 // Bound by the one write (forward) or read (backward) of the matrix.  Forward: a workgroup holds its head's bias over the distances
 // -W .. W in LDS (beyond W it is constant) and writes 16-byte chunks of the head's matrix taken as one line; most chunks of a long
 // matrix are one constant.  Backward: a workgroup reads a run of whole rows; what lies beyond W goes into two registers, in 16-byte
-// chunks, a row per wave, four chunks in flight per lane; the band in between is read along its diagonals, one distance per thread, so
+// chunks, a row per wave, eight chunks in flight per lane; the band in between is read along its diagonals, one distance per thread, so
 // that no two threads add to the same number: no atomics, and an order that does not change.
 #include "seq_attn.h"
 #include "seq_dtable.h"
@@ -83,76 +83,66 @@ __global__ __launch_bounds__(256) void relpos_fwd_kernel(const SaMatParams p) {
   }
 }
 
-// A lane's share of row[a .. b): 16-byte chunks, single elements before the first and after the last 16-byte border.  fetch() requests the
-// first 256 chunks of a wave (and the single elements), sum() adds them up and walks the rest: a caller fetches several before it sums.
 template <int DT>
-struct SaLine {
+__global__ __launch_bounds__(256, 5) void relpos_bwd_kernel(const SaMatParams p) {
   using E = typename SaElem<DT>::type;
-  static constexpr int V = SaElem<DT>::VEC;
-  const sa_u32x4* c;
-  int n, k;
-  E one[2];
-  sa_u32x4 x[4];
-  __device__ __forceinline__ void more() {
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      x[u] = (sa_u32x4){0u, 0u, 0u, 0u};
-      if (k + 64 * u < n) x[u] = c[k + 64 * u];
-    }
-  }
-  __device__ __forceinline__ void fetch(const E* row, int a, int b, int lane) {
-    const int head = min((int)((-(long)(((uintptr_t)(row + a)) / sizeof(E))) & (V - 1)), b - a);
-    one[0] = one[1] = 0;
-    if (lane < head) one[0] = row[a + lane];
-    a += head;
-    n = (b - a) / V;
-    k = lane;
-    if (lane < b - a - n * V) one[1] = row[a + n * V + lane];
-    c = (const sa_u32x4*)(row + a);
-    more();
-  }
-  __device__ __forceinline__ float sum() {
-    float s = sa_to_f32<DT>(one[0]) + sa_to_f32<DT>(one[1]);
-    while (true) {
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        if constexpr (DT == DFOLD_DT_F32) {
-          const f32x4 y = __builtin_bit_cast(f32x4, x[u]);
-          s += (y[0] + y[1]) + (y[2] + y[3]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s += sa_lo<DT>(x[u][e]) + sa_hi<DT>(x[u][e]);
-        }
-      }
-      k += 256;
-      if (k >= n) return s;
-      more();
-    }
-  }
-};
-
-template <int DT>
-__global__ __launch_bounds__(256) void relpos_bwd_kernel(const SaMatParams p) {
-  using E = typename SaElem<DT>::type;
+  constexpr int V = SaElem<DT>::VEC;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* const hist = (float*)smem;                 // [2 W + 1]
   __shared__ float side[2][4];
-  const int tid = threadIdx.x, lane = tid & 63, w = tid >> 6, head = blockIdx.y, W = p.rel.W, off = p.rel.q_offset;
+  const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), head = blockIdx.y, W = p.rel.W, off = p.rel.q_offset;
   const long n = (long)p.Lq * p.Lk;
   const int i0 = blockIdx.x * p.rows, i1 = min(p.Lq, i0 + p.rows);
   const E* const g = (const E*)p.g + head * n;
   float aL = 0.f, aR = 0.f;
   if (i0 < i1) {
-    // far distances: columns [0, jl) and [jr, Lk) of a row
+    // far distances: columns [0, jl) and [jr, Lk) of a row, as the aligned chunks that hold them -- a lane's loads are all issued before the
+    // first sum; a chunk over a border counts by element.  (The loads go through a buffer descriptor that ends with the tensor: nothing
+    // to test.  Single elements in front of the first and behind the last border, each loaded under a test, cost an L2 round trip each.)
     for (int i = i0 + w; i < i1; i += 4) {
       const long at = (long)i + off;
       const int jl = (int)min(max(at - W + 1, 0L), (long)p.Lk), jr = (int)min(max(at + W, (long)jl), (long)p.Lk);
-      const E* const row = g + (long)i * p.Lk;
-      SaLine<DT> left, right;
-      left.fetch(row, 0, jl, lane);
-      right.fetch(row, jr, p.Lk, lane);
-      aL += left.sum();
-      aR += right.sum();
+      const long row = head * n + (long)i * p.Lk, base = row / V * V;
+      const int shift = (int)(row - base);
+      const unsigned bytes = (unsigned)min(((long)p.H * n - base) * (long)sizeof(E), 0x7fffffffL);
+      const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)((const E*)p.g + base), 0, bytes, 0x00020000);
+      const int nl = jl > 0 ? (jl + shift + V - 1) / V : 0;                                  // chunks on the left: 0 .. nl
+      const int r0 = (jr + shift) / V, nr = jr < p.Lk ? (p.Lk + shift + V - 1) / V - r0 : 0;  // and on the right: r0 .. r0 + nr
+      for (int k0 = lane; k0 < nl + nr; k0 += 512) {
+        sa_u32x4 x[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int k = k0 + 64 * u, c = k < nl ? k : r0 + k - nl;
+          x[u] = __builtin_amdgcn_raw_buffer_load_b128(rsrc, k < nl + nr ? c * 16 : (int)0x80000000, 0, 0);
+        }
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const int k = k0 + 64 * u;
+          const bool left = k < nl;
+          const int j0 = (left ? k : r0 + k - nl) * V - shift, lo = left ? 0 : jr, hi = left ? jl : p.Lk;
+          float v[V], a = 0.f;
+          if constexpr (DT == DFOLD_DT_F32) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = __uint_as_float(x[u][e]);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              v[2 * e] = sa_lo<DT>(x[u][e]);
+              v[2 * e + 1] = sa_hi<DT>(x[u][e]);
+            }
+          }
+          if (k < nl + nr) {
+            if (j0 >= lo && j0 + V <= hi) {
+#pragma unroll
+              for (int e = 0; e < V; ++e) a += v[e];
+            } else {
+#pragma unroll
+              for (int e = 0; e < V; ++e) a += j0 + e >= lo && j0 + e < hi ? v[e] : 0.f;
+            }
+            if (left) aL += a; else aR += a;
+          }
+        }
+      }
     }
     // the band: distance d of every row of the run
     for (int d = tid - (W - 1); d <= W - 1; d += 256) {
@@ -176,9 +166,10 @@ __global__ __launch_bounds__(256) void relpos_bwd_kernel(const SaMatParams p) {
   sa_bucket_sums(p.rel, hist, W, p.nb, p.ws + ((long)head * p.nblk + blockIdx.x) * p.nb, w, lane);
 }
 
-// row blocks of the backward: about eight workgroups per CU
+// row blocks of the backward: five workgroups per CU, one round of what fits (2048 of them: a second round of three, 170 -> 167 us at
+// 16 x 4097 x 4100, 12.0 -> 8.2 at 8 x 256 x 256)
 static inline int sa_mat_blocks(int H, int Lq) {
-  const int want = 2048 / H > 1 ? 2048 / H : 1;
+  const int want = 1280 / H > 1 ? 1280 / H : 1;
   return Lq < want ? Lq : want;
 }
 extern "C" int dfold_relpos_ws(int32_t H, int32_t Lq, int32_t num_buckets) {
@@ -187,7 +178,7 @@ extern "C" int dfold_relpos_ws(int32_t H, int32_t Lq, int32_t num_buckets) {
   return f > 0x7fffffffL ? DFOLD_EINVAL : (int)f;
 }
 static bool sa_mat_params(const dfold_rel_bias* rel, int dtype, int H, int Lq, int Lk, SaMatParams* p) {
-  if (!rel || dtype < DFOLD_DT_BF16 || dtype > DFOLD_DT_F32 || H <= 0 || H > 65535 || Lq <= 0 || Lk <= 0 || Lq > (1 << 30) || Lk > (1 << 30)) return false;
+  if (!rel || dtype < DFOLD_DT_BF16 || dtype > DFOLD_DT_F32 || H <= 0 || H > 65535 || Lq <= 0 || Lk <= 0 || Lq > (1 << 30) || Lk > (1 << 28)) return false;
   if (!sa_make_rel(rel, H, &p->rel)) return false;
   if (rel->q_offset > (1 << 29) || rel->q_offset < -(1 << 29)) return false;
   p->H = H; p->Lq = Lq; p->Lk = Lk; p->nb = rel->num_buckets;

@@ -228,8 +228,8 @@ def relative_position_bias(table, q_len, k_len, *, max_distance=128, bidirection
     half; else half = num_buckets and keys behind the query count as distance 0) the first half // 2 hold one distance each, the others
     grow logarithmically up to max_distance, beyond which everything shares the last.  dtype: fp32, bf16 or fp16 of the result."""
     _check_rel(table, max_distance, bidirectional)
-    if not (isinstance(q_len, int) and isinstance(k_len, int) and 0 <= q_len <= MAX_LEN and 0 <= k_len <= MAX_LEN):
-        raise ValueError("q_len, k_len must be whole numbers >= 0")
+    if not (isinstance(q_len, int) and isinstance(k_len, int) and 0 <= q_len <= MAX_LEN and 0 <= k_len <= 1 << 28):
+        raise ValueError("q_len, k_len must be whole numbers >= 0, k_len at most 2^28")
     if not isinstance(q_offset, int) or abs(q_offset) > MAX_OFFSET:
         raise ValueError(f"q_offset must be a whole number, at most {MAX_OFFSET}")
     if dtype not in DTYPES:

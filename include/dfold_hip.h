@@ -626,7 +626,7 @@ typedef struct {
   int16_t far_border[DFOLD_REL_FAR];
 } dfold_rel_bias;
 
-/* out [H][Lq][Lk] of type dtype = the bias matrix; backward: g of type dtype -> dtable [num_buckets][H] fp32 (overwritten;
+/* out [H][Lq][Lk] (Lk <= 2^28) of type dtype = the bias matrix; backward: g of type dtype -> dtable [num_buckets][H] fp32 (overwritten;
  * deterministic; ws: dfold_relpos_ws(H, Lq, num_buckets) floats). */
 int dfold_relpos_fwd(const dfold_rel_bias* rel, void* out, int32_t dtype, int32_t H, int32_t Lq, int32_t Lk, void* stream);
 int dfold_relpos_bwd(const dfold_rel_bias* rel, const void* g, int32_t dtype, int32_t H, int32_t Lq, int32_t Lk, float* dtable, float* ws,

@@ -180,7 +180,7 @@ def test_cabi_refuses_bad_descriptors():
         assert L.dfold_relpos_bwd(*a, one, one, st) == -1
     assert L.dfold_relpos_ws(c_int32(0), c_int32(1), c_int32(1)) == -1 and L.dfold_relpos_ws(c_int32(1 << 20), c_int32(1 << 20), c_int32(1 << 20)) == -1
     for blocks_of in ((1, 1, 32), (16, 4097, 64), (3000, 5, 2)):
-        assert L.dfold_relpos_ws(*(c_int32(x) for x in blocks_of)) == blocks_of[0] * min(blocks_of[1], max(2048 // blocks_of[0], 1)) * blocks_of[2]
+        assert L.dfold_relpos_ws(*(c_int32(x) for x in blocks_of)) == blocks_of[0] * min(blocks_of[1], max(1280 // blocks_of[0], 1)) * blocks_of[2]
 
     def rope(**kw):
         d = S.RopeDesc()

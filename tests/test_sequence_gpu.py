@@ -352,7 +352,7 @@ def test_bias_matrix(H, Lq, Lk, nb, dist, both, off, dt):
     (dtable,) = torch.autograd.grad(out, table, g)
     add = lambda x: torch.zeros(H, nb, dtype=torch.float64, device=DEV).scatter_add_(1, bk.reshape(1, -1).expand(H, -1), x.reshape(H, -1).double()).t()
     # fp32 sums: the longest chain is a thread's share of a run of rows, then the lanes, the runs
-    rows = -(-Lq // min(Lq, max(2048 // H, 1)))
+    rows = -(-Lq // min(Lq, max(1280 // H, 1)))
     chain = rows * Lk / 256 + rows + 64 + Lq / rows / 16 + 16
     within("dtable", dtable, (add(g), 2.0 ** -24 * chain * add(g.abs()) + 1e-30))
     (again,) = torch.autograd.grad(S.relative_position_bias(table, Lq, Lk, max_distance=dist, bidirectional=both, q_offset=off, dtype=dt), table, g)
