@@ -10,9 +10,11 @@
 #pragma once
 #include "dfold_common.h"
 #include "../../include/dfold_hip.h"
+#include <atomic>
 
 #define SA_LOG2E 1.44269504088896341f
 #define SA_KT 64                       // rows of an LDS tile
+#define SA_MAX_LDS (160 * 1024)
 #define SA_WAVES 4
 #define SA_REACH 64                    // distances a 32 x 32 block can lie beyond W and still not be uniform
 #define SA_ROWS (32 * SA_WAVES)        // softmax rows (forward, dQ) or keys (dK, dV) of a workgroup
@@ -233,6 +235,20 @@ static inline bool sa_make_rel(const dfold_rel_bias* d, int H, SaRel* r) {
     r->far[i] = (int16_t)(prev = d->far_border[i]);
   }
   r->W = nfar ? prev : exact;
+  return true;
+}
+
+// Launches with more than 64 KB of dynamic LDS need the kernel's limit raised, once per device and kernel (F: a type of the caller's own
+// per kernel, so that each has its flags; setting it twice does no harm).
+template <typename F, typename K>
+static inline bool sa_raise_lds(K kernel, int lds) {
+  static std::atomic<bool> done[64];
+  int dev = 0;
+  if (lds <= 65536) return true;
+  if (hipGetDevice(&dev) != hipSuccess) return false;
+  if (dev < 64 && done[dev].load(std::memory_order_relaxed)) return true;
+  if (hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, SA_MAX_LDS) != hipSuccess) return false;
+  if (dev < 64) done[dev].store(true, std::memory_order_relaxed);
   return true;
 }
 

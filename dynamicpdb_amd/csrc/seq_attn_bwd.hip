@@ -506,17 +506,19 @@ __global__ __launch_bounds__(256) void seq_attn_delta_kernel(float* __restrict__
   delta[i] += a;
 }
 
-template <typename K>
+template <typename F, typename K>
 static int sa_launch_bwd(K kernel, const SaBwdParams& p, long nwg, int waves, int lds, hipStream_t st) {
-  if (lds > 65536 && hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, lds) != hipSuccess)
-    return DFOLD_ELAUNCH;
+  if (lds > SA_MAX_LDS) return DFOLD_EINVAL;
+  if (!sa_raise_lds<F>(kernel, lds)) return DFOLD_ELAUNCH;
   DFOLD_LAUNCH(kernel, dim3((unsigned)nwg), dim3(64 * waves), lds, st, p);
   return dfold_check_launch();
 }
 template <int DT, int DP, bool REL>
 static int sa_bwd_dp(const SaBwdParams& p, hipStream_t st) {
   const int bias = REL ? (2 * p.rel.W + 1) * 4 : 0, hist = REL ? SA_WAVES * (2 * (p.rel.W + SA_REACH) + 1 + SA_DIAG) * 4 : 0;
-  int rc = sa_launch_bwd(seq_attn_dq_kernel<DT, DP, REL>, p, (long)p.nrb * p.splits_q * p.H * p.B, SA_WAVES,
+  struct Dq;
+  struct Dkv;
+  int rc = sa_launch_bwd<Dq>(seq_attn_dq_kernel<DT, DP, REL>, p, (long)p.nrb * p.splits_q * p.H * p.B, SA_WAVES,
                          4 * SaTile<DP>::BYTES + bias, st);
   if (rc != DFOLD_OK) return rc;
   if (p.splits_q > 1) {
@@ -528,7 +530,7 @@ static int sa_bwd_dp(const SaBwdParams& p, hipStream_t st) {
     if ((rc = dfold_check_launch()) != DFOLD_OK) return rc;
   }
   const long nkb = (p.Lk + SA_ROWS - 1) / SA_ROWS;
-  rc = sa_launch_bwd(seq_attn_dkv_kernel<DT, DP, REL>, p, nkb * p.splits_k * p.Hkv * p.B, SaDkvCfg<DP, REL>::WAVES,
+  rc = sa_launch_bwd<Dkv>(seq_attn_dkv_kernel<DT, DP, REL>, p, nkb * p.splits_k * p.Hkv * p.B, SaDkvCfg<DP, REL>::WAVES,
                      SaDkvCfg<DP, REL>::LDS + bias + hist, st);
   if (rc != DFOLD_OK) return rc;
   if (REL) {

@@ -304,9 +304,9 @@ __global__ __launch_bounds__(256) void seq_attn_combine_row_kernel(const SaFwdPa
 template <int DT, int DP, bool REL>
 static int sa_launch_fwd(const SaFwdParams& p, unsigned nwg, hipStream_t st) {
   const int lds = 4 * SaTile<DP>::BYTES + (REL ? p.pack * (2 * p.rel.W + 1) * 4 : 0);
-  if (lds > 65536 && hipFuncSetAttribute((const void*)seq_attn_fwd_kernel<DT, DP, REL>, hipFuncAttributeMaxDynamicSharedMemorySize, lds) !=
-                         hipSuccess)
-    return DFOLD_ELAUNCH;
+  struct Mine;
+  if (lds > SA_MAX_LDS) return DFOLD_EINVAL;
+  if (!sa_raise_lds<Mine>(seq_attn_fwd_kernel<DT, DP, REL>, lds)) return DFOLD_ELAUNCH;
   DFOLD_LAUNCH((seq_attn_fwd_kernel<DT, DP, REL>), dim3(nwg), dim3(64 * SA_WAVES), lds, st, p);
   return dfold_check_launch();
 }

@@ -69,8 +69,8 @@ def reference(q, k, v, g, live, table, buckets, scale):
     p_err = (u + E) * p + sub * lvf
     fold = lambda x: x.unflatten(1, (Hkv, G)).sum(2)                                # heads of a group
     back = lambda x: x.transpose(1, 2)
-    outs = dict(o=(o, p_err @ v64.abs()), dq=(ds @ k64 * scale, (ds_err + p * q_delta) @ k64.abs() * scale),
-                dk=(fold(ds.transpose(-1, -2) @ q64 * scale), fold(ds_err.transpose(-1, -2) @ q64.abs() * scale)),
+    outs = dict(o=(o, p_err @ v64.abs()), dq=(ds @ k64 * scale, (ds_err + p * q_delta) @ k64.abs() * abs(scale)),
+                dk=(fold(ds.transpose(-1, -2) @ q64 * scale), fold(ds_err.transpose(-1, -2) @ q64.abs() * abs(scale))),
                 dv=(fold(p.transpose(-1, -2) @ g64), fold(p_err.transpose(-1, -2) @ g64.abs())))
     outs = {n: (back(x), back(e) + u * back(x).abs() + 2.0 ** -24 * (1 if q.dtype == HF else 0) + 1e-30) for n, (x, e) in outs.items()}
     if table is not None:
@@ -322,7 +322,9 @@ def test_attention_split_keys_equal_whole(D):
     B, Lq, Lk, H, Hkv = 2, 3, 900, 4, 2
     q, k, v, g = make(B, Lq, Lk, H, Hkv, D, BF)
     live, kw = make_mask("lens", B, Lk)
+    table = torch.randn(32, H, device=DEV)
     ref = reference(q, k, v, g, live, None, None, D ** -0.5)
+    with_table = reference(q, k, v, g, live, table, bucket_matrix(Lq, Lk, 32, 128, True, 0), D ** -0.5)
     plan = S._parts
     try:
         for parts in (1, 2, 3, 7, 15, 40):
@@ -331,9 +333,58 @@ def test_attention_split_keys_equal_whole(D):
             got = run(q, k, v, g, **kw)
             for n in ref:
                 within(f"{n} in {parts} parts", got[n], ref[n])
+            got = run(q, k, v, g, table, **kw)
+            for n in with_table:
+                within(f"{n} with bias in {parts} parts", got[n], with_table[n])
     finally:
         S._parts = plan
         S._attn_plan.cache_clear(), S._grad_plan.cache_clear()
+
+
+@pytest.mark.parametrize("scale", [-0.3, 1.0, 1e-4])
+@pytest.mark.parametrize("rel", [False, True])
+def test_attention_scale(scale, rel):
+    B, Lq, Lk, H, Hkv, D = 1, 70, 90, 4, 2, 32
+    q, k, v, g = make(B, Lq, Lk, H, Hkv, D, BF, seed=4)
+    live, kw = make_mask("keys", B, Lk)
+    table = torch.randn(32, H, device=DEV) if rel else None
+    buckets = bucket_matrix(Lq, Lk, 32, 128, True, 0) if rel else None
+    got = run(q, k, v, g, table, scale=scale, **kw)
+    ref = reference(q, k, v, g, live, table, buckets, scale)
+    for n in ref:
+        within(n, got[n], ref[n])
+
+
+def test_attention_rows_far_apart():
+    """rows of a cache 2^23 elements apart (the sequence spans more than 2^31 elements), and too far apart for the kernels' row offsets
+    (a copy is made)"""
+    B, Lq, Lk, H, D = 1, 40, 300, 1, 64
+    q, kd, vd, g = make(B, Lq, Lk, H, H, D, BF)
+    want = run(q, kd, vd, g)
+    store = torch.empty((Lk - 1) * (1 << 23) + 2 * D, dtype=BF, device=DEV)
+    k = store.as_strided((B, Lk, H, D), (0, 1 << 23, D, 1))
+    v = store.as_strided((B, Lk, H, D), (0, 1 << 23, D, 1), D)
+    k.copy_(kd)
+    v.copy_(vd)
+    got = run(q, k, v, g)
+    assert all(torch.equal(want[n], got[n]) for n in want)
+    got = run(k[:, :Lq], kd, vd, g)
+    assert torch.equal(got["dq"], run(kd[:, :Lq].contiguous(), kd, vd, g)["dq"])
+    far = store.as_strided((B, 100, H, D), (0, 1 << 24, D, 1))
+    far.copy_(kd[:, :100])
+    assert torch.equal(run(q, far, vd[:, :100], g)["dk"], run(q, kd[:, :100].contiguous(), vd[:, :100].contiguous(), g)["dk"])
+
+
+def test_attention_saved_tensors_may_move():
+    """a backward pass whose saved tensors come back at other addresses with other strides"""
+    B, L, H, D = 2, 75, 4, 32
+    qkv = torch.randn(B, L, 3, H, D, device=DEV).to(BF)
+    g, table = torch.randn(B, L, H, D, device=DEV).to(BF), torch.randn(32, H, device=DEV)
+    keep = torch.rand(B, L, device=DEV) < 0.8
+    want = run(qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2], g, table, key_mask=keep)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: t.to(DEV)):
+        got = run(qkv[:, :, 0], qkv[:, :, 1], qkv[:, :, 2], g, table, key_mask=keep)
+    assert all(torch.equal(want[n], got[n]) for n in want)
 
 
 # ---- relative position bias ---------------------------------------------------------------------------------------------------------
@@ -468,23 +519,24 @@ def test_norm_rope_layouts_and_options():
 
 # ---- together ---------------------------------------------------------------------------------------------------------------------------
 
-def chain(qkv, wq, wk, table, lens):
+def chain(qkv, wq, wk, table, lens, dist):
     q, k = S.qk_norm_rope(qkv[:, :, 0], qkv[:, :, 1], wq, wk)
-    return S.cross_attention(q, k, qkv[:, :, 2], kv_lens=lens, rel_table=table)
+    return S.cross_attention(q, k, qkv[:, :, 2], kv_lens=lens, rel_table=table, max_distance=dist)
 
 
-def test_run_of_all_on_streams_and_graphs():
+@pytest.mark.parametrize("D,dist", [(64, 128), (128, 1024), (128, 0)])
+def test_run_of_all_on_streams_and_graphs(D, dist):
     """norm + rotation -> attention with bias -> gradients: on a side stream, and recorded into a graph that is replayed on new inputs
     between eager calls, the same bits as the plain call"""
-    B, L, H, D = 2, 200, 4, 64
+    B, L, H = 2, 200, 4
     gen = torch.Generator(device=DEV).manual_seed(2)
     r = lambda *s: torch.randn(*s, generator=gen, device=DEV)
     sets = [(r(B, L, 3, H, D).to(BF), r(B, L, H, D).to(BF), torch.tensor(ls, dtype=torch.int32, device=DEV)) for ls in ([200, 150], [0, 77], [1, 200])]
     wq, wk, table = (1 + 0.1 * r(D)), (1 + 0.1 * r(D)), r(32, H)
 
     def step(qkv, g, lens):
-        leaves = [t.detach().requires_grad_(True) for t in (qkv, wq, wk, table)]
-        o = chain(*leaves, lens)
+        leaves = [t.detach().requires_grad_(True) for t in (qkv, wq, wk) + ((table,) if dist else ())]
+        o = chain(*(leaves if dist else leaves + [None]), lens, dist or 128)
         return [o.detach(), *torch.autograd.grad(o, leaves, g)]
     want = [[t.clone() for t in step(*s)] for s in sets]
     side = torch.cuda.Stream()
