@@ -54,7 +54,7 @@ __device__ __forceinline__ void nr_angles(const NrParams& p, double pos, int d0,
   constexpr int V = NrVec<DT>::V;
   auto sc = [&](int i, float& sn, float& cs) {
     double t = pos * p.turns[i];
-    t -= rint(t);                        // whole turns drop out in fp64: exact for positions whose turns are below 2^52
+    t -= rint(t);                        // whole turns drop out in fp64: right to fp32 rounding up to positions of 2^31
     sincospif(2.f * (float)t, &sn, &cs);
   };
   if (p.inter) {

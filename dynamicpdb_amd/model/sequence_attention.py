@@ -92,8 +92,9 @@ def _require_cuda(t):
 
 
 def _same_device(dev, name, t):
-    if t is not None and t.device != dev:
-        raise ValueError(f"{name} is on {t.device}, expected {dev}")
+    """dev: the device's number (-1: the CPU)"""
+    if t.get_device() != dev:
+        raise ValueError(f"{name} is on {t.device}, expected {'cpu' if dev < 0 else f'cuda:{dev}'}")
 
 
 def _rows16(t):
@@ -181,6 +182,12 @@ def _rel_desc(table, num_buckets, max_distance, bidirectional, q_offset, q_offse
     return _REL.pack(table.data_ptr(), _addr(q_offsets), q_offset, num_buckets, bidirectional, 0, _border_bytes(num_buckets, max_distance, bidirectional))
 
 
+def _once(fn):
+    """once_differentiable, whose bookkeeping only a pass that builds a graph of the gradients needs"""
+    guarded = once_differentiable(fn)
+    return lambda ctx, *g: guarded(ctx, *g) if torch.is_grad_enabled() else fn(ctx, *g)
+
+
 # ------------------------------------------------------------------------------------------------
 # relative position bias as a matrix
 # ------------------------------------------------------------------------------------------------
@@ -201,7 +208,7 @@ class RelativeBiasFn(Function):
         return _bias_forward(table, *args)
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
         q_len, k_len, max_distance, bidirectional, q_offset, dtype = ctx.args
         nb, H = ctx.table_shape
@@ -265,9 +272,10 @@ class RelativePositionBias(nn.Module):
 def _rope_part(x, y, w, pos, g=None, dw=None):
     if x is None or x.numel() == 0:
         return _NO_PART
+    _, L, H, _ = x.shape
     pos_sb = 0 if pos is None or pos.shape[0] == 1 else pos.stride(0)
     return _PART.pack(x.data_ptr(), y.data_ptr(), _addr(g), _addr(w), _addr(dw), _addr(pos), *_strides(x), *(_strides(g) if g is not None else (0, 0, 0)),
-                      pos_sb, x.shape[1], x.shape[2])
+                      pos_sb, L, H)
 
 
 def _rope_desc(parts, ref, opts, ws=None):
@@ -277,13 +285,19 @@ def _rope_desc(parts, ref, opts, ws=None):
 
 def _rope_forward(q, k, w_q, w_k, q_pos, k_pos, *opts):
     """results and the (readable) inputs they were computed from"""
-    q, k = (None if t is None else _rows16(t) for t in (q, k))
-    w_q, w_k = (None if t is None else t.contiguous() for t in (w_q, w_k))
-    oq, ok = (None if t is None else _dense_like(t) for t in (q, k))
-    parts = _rope_part(q, oq, w_q, q_pos), _rope_part(k, ok, w_k, k_pos)
-    if parts != (_NO_PART, _NO_PART):
+    oq = ok = None
+    part_q = part_k = _NO_PART
+    if q is not None:
+        q = _rows16(q)
+        oq = _dense_like(q)
+        part_q = _rope_part(q, oq, w_q, q_pos)
+    if k is not None:
+        k = _rows16(k)
+        ok = _dense_like(k)
+        part_k = _rope_part(k, ok, w_k, k_pos)
+    if part_q is not _NO_PART or part_k is not _NO_PART:
         ref = q if q is not None else k
-        _call("dfold_qk_norm_rope_fwd", _rope_desc(parts, ref, opts), t=ref)
+        _call("dfold_qk_norm_rope_fwd", _rope_desc((part_q, part_k), ref, opts), t=ref)
     return oq, ok, (q, k, w_q, w_k, q_pos, k_pos)
 
 
@@ -296,7 +310,7 @@ class QKNormRopeFn(Function):
         return oq, ok
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, gq, gk):
         q, k, w_q, w_k, q_pos, k_pos = ctx.saved_tensors
         ref = q if q is not None else k
@@ -317,39 +331,52 @@ class QKNormRopeFn(Function):
         return (*grads, None, None, None, None, None, None)
 
 
-def _positions(pos, x, name):
+def _positions(pos, x, dev, name):
     if pos is None or x is None:
         return None
-    _same_device(x.device, name, pos)
+    _same_device(dev, name, pos)
     if pos.dtype != torch.int64:
         if pos.dtype != torch.int32:
             raise ValueError(f"{name} must be int64 or int32")
         pos = pos.long()
     if pos.dim() == 1:
         pos = pos[None]
-    if pos.dim() != 2 or pos.shape[0] not in (1, x.shape[0]) or pos.shape[1] != x.shape[1]:
-        raise ValueError(f"{name} must be [{x.shape[1]}] or [{x.shape[0]}, {x.shape[1]}]")
-    return pos if pos.stride(1) == 1 or pos.shape[1] <= 1 else pos.contiguous()
+    B, L = x.shape[:2]
+    if pos.dim() != 2 or pos.shape[0] not in (1, B) or pos.shape[1] != L:
+        raise ValueError(f"{name} must be [{L}] or [{B}, {L}]")
+    return pos if L <= 1 or pos.stride(1) == 1 else pos.contiguous()
+
+
+def _heads(t, dt, name):
+    if t.dim() != 4 or t.dtype is not dt:
+        raise ValueError(f"{name} must be [B, L, heads, D], q and k of one type")
+
+
+def _head_weight(w, D, dev, name):
+    _same_device(dev, name, w)
+    if w.dtype is not F32 or w.dim() != 1 or w.shape[0] != D:
+        raise ValueError(f"{name} must be fp32 [{D}]")
+    return w if w.is_contiguous() else w.contiguous()
 
 
 def qk_norm_rope(q, k, w_q=None, w_k=None, q_positions=None, k_positions=None, *, rotary_dim=None, base=10000.0, interleaved=False, eps=1e-6):
     """Every head of q [B, Lq, H, D] and k [B, Lk, Hkv, D] divided by its root mean square, times w (fp32 [D] or None), then its first
     rotary_dim dimensions (default: all; a multiple of 16; 0: none) rotated by position * base^(-2 i / rotary_dim): pairs
     (i, i + rotary_dim / 2), or (2 i, 2 i + 1) if interleaved.  k may be None (keys that are rotated already).  Positions: int64 / int32
-    [L] or [B, L], default 0, 1, ...; any size (angles are reduced in fp64).  bf16, fp16 or fp32; one launch for q and k; differentiable
-    (once) in q, k, w_q, w_k."""
+    [L] or [B, L], default 0, 1, ...; angles are reduced in fp64 (right to fp32 rounding up to positions of 2^31).  bf16, fp16 or fp32;
+    one launch for q and k; differentiable (once) in q, k, w_q, w_k."""
     ref = q if q is not None else k
     if ref is None:
         raise ValueError("qk_norm_rope needs q or k")
-    if ref.dtype not in DTYPES:
+    dt, dev = ref.dtype, ref.get_device()
+    if dt not in DTYPES:
         raise ValueError("q, k must be bfloat16, float16 or float32")
-    for name, t in (("q", q), ("k", k)):
-        if t is not None and (t.dim() != 4 or t.dtype != ref.dtype):
-            raise ValueError(f"{name} must be [B, L, heads, D], q and k of one type")
-    D, dev = ref.shape[3], ref.device
-    if q is not None and k is not None:
+    _heads(ref, dt, "q" if q is not None else "k")
+    B, _, _, D = ref.shape
+    if k is not None and k is not ref:
+        _heads(k, dt, "k")
         _same_device(dev, "k", k)
-        if q.shape[0] != k.shape[0] or k.shape[3] != D:
+        if k.shape[0] != B or k.shape[3] != D:
             raise ValueError("q and k differ in batch or head size")
     if D % 8 or not 8 <= D <= 256:
         raise ValueError("the head size must be a multiple of 8, at most 256")
@@ -359,17 +386,19 @@ def qk_norm_rope(q, k, w_q=None, w_k=None, q_positions=None, k_positions=None, *
         rotary_dim = D
     if not isinstance(rotary_dim, int) or not 0 <= rotary_dim <= D or rotary_dim % 16:
         raise ValueError("rotary_dim must be a multiple of 16, at most the head size")
-    if not (base > 0 and math.isfinite(base) and eps >= 0):
+    if not (0 < base < math.inf and eps >= 0):
         raise ValueError("base must be positive and eps not negative")
-    for name, w in (("w_q", w_q), ("w_k", w_k)):
-        if w is not None:
-            _same_device(dev, name, w)
-            if w.dtype != F32 or w.dim() != 1 or w.shape[0] != D:
-                raise ValueError(f"{name} must be fp32 [{D}]")
-    q_positions, k_positions = _positions(q_positions, q, "q_positions"), _positions(k_positions, k, "k_positions")
+    grad = ref.requires_grad or (k is not None and k.requires_grad)
+    if w_q is not None:
+        w_q = _head_weight(w_q, D, dev, "w_q")
+        grad = grad or w_q.requires_grad
+    if w_k is not None:
+        w_k = _head_weight(w_k, D, dev, "w_k")
+        grad = grad or w_k.requires_grad
+    q_positions, k_positions = _positions(q_positions, q, dev, "q_positions"), _positions(k_positions, k, dev, "k_positions")
     _require_cuda(ref)
     args = (q, k, w_q, w_k, q_positions, k_positions, rotary_dim, float(base), bool(interleaved), float(eps))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args[:4]):
+    if grad and torch.is_grad_enabled():
         return QKNormRopeFn.apply(*args)
     return _rope_forward(*args)[:2]
 
@@ -457,7 +486,7 @@ class CrossAttentionFn(Function):
         return o
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, g):
         q, k, v, table, key_mask, kv_lens, q_offsets, o, lse = ctx.saved_tensors
         q_offset, max_distance, bidirectional, scale = ctx.opts
@@ -494,10 +523,10 @@ def cross_attention(q, k, v, *, key_mask=None, kv_lens=None, rel_table=None, max
     [num_buckets, H] adds the bias of relative_position_bias without forming it; q_offset: position of query 0 minus position of key 0, a
     whole number or an int32 / int64 tensor [B] (one token at its own position per sequence).  scale defaults to D^-1/2.
     Differentiable (once) in q, k, v and rel_table; repeated calls give the same bits."""
-    dt, dev = q.dtype, q.device
+    dt, dev = q.dtype, q.get_device()
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError("q must be [B, Lq, H, D], k and v [B, Lk, Hkv, D]")
-    if (dt is not BF16 and dt is not F16) or k.dtype != dt or v.dtype != dt:
+    if (dt is not BF16 and dt is not F16) or k.dtype is not dt or v.dtype is not dt:
         raise ValueError("q, k, v must all be bfloat16 or all float16")
     B, Lq, H, D = q.shape
     Bk, Lk, Hkv, Dk = k.shape
@@ -518,9 +547,9 @@ def cross_attention(q, k, v, *, key_mask=None, kv_lens=None, rel_table=None, max
         key_mask = _mask_bytes(key_mask)
     if kv_lens is not None:
         _same_device(dev, "kv_lens", kv_lens)
-        if kv_lens.shape != (B,) or kv_lens.dtype not in (torch.int32, torch.int64):
+        if kv_lens.dim() != 1 or kv_lens.shape[0] != B or (kv_lens.dtype is not torch.int32 and kv_lens.dtype is not torch.int64):
             raise ValueError(f"kv_lens must be int32 or int64 [{B}]")
-        if kv_lens.dtype == torch.int64:
+        if kv_lens.dtype is torch.int64:
             kv_lens = kv_lens.clamp(0, Lk).int()
         kv_lens = kv_lens.contiguous()
     q_offsets = None
@@ -540,7 +569,7 @@ def cross_attention(q, k, v, *, key_mask=None, kv_lens=None, rel_table=None, max
     else:
         q_offset = 0
     scale = D ** -0.5 if scale is None else float(scale)
-    if not math.isfinite(scale) or scale == 0:
+    if not 0 < abs(scale) < math.inf:
         raise ValueError("scale must be finite and not 0")
     _require_cuda(q)
     args = (q, k, v, rel_table, key_mask, kv_lens, q_offsets, q_offset, max_distance, bool(bidirectional), scale)
