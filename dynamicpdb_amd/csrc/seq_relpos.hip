@@ -97,14 +97,16 @@ __global__ __launch_bounds__(256, 5) void relpos_bwd_kernel(const SaMatParams p)
   float aL = 0.f, aR = 0.f;
   if (i0 < i1) {
     // far distances: columns [0, jl) and [jr, Lk) of a row, as the aligned chunks that hold them -- a lane's loads are all issued before the
-    // first sum; a chunk over a border counts by element.  (The loads go through a buffer descriptor that ends with the tensor: nothing
-    // to test.  Single elements in front of the first and behind the last border, each loaded under a test, cost an L2 round trip each.)
+    // first sum; a chunk over a border counts by element.  (The loads go through a buffer descriptor that ends with the tensor's last
+    // whole chunk: nothing to test.  Single elements in front of the first and behind the last border, each loaded under a test, cost an
+    // L2 round trip each; only what lies behind the tensor's last whole chunk is read that way.)
+    const long whole = (long)p.H * n / V * V;
     for (int i = i0 + w; i < i1; i += 4) {
       const long at = (long)i + off;
       const int jl = (int)min(max(at - W + 1, 0L), (long)p.Lk), jr = (int)min(max(at + W, (long)jl), (long)p.Lk);
       const long row = head * n + (long)i * p.Lk, base = row / V * V;
       const int shift = (int)(row - base);
-      const unsigned bytes = (unsigned)min(((long)p.H * n - base) * (long)sizeof(E), 0x7fffffffL);
+      const unsigned bytes = (unsigned)min(max(whole - base, 0L) * (long)sizeof(E), 0x7ffffff0L);
       const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc((void*)((const E*)p.g + base), 0, bytes, 0x00020000);
       const int nl = jl > 0 ? (jl + shift + V - 1) / V : 0;                                  // chunks on the left: 0 .. nl
       const int r0 = (jr + shift) / V, nr = jr < p.Lk ? (p.Lk + shift + V - 1) / V - r0 : 0;  // and on the right: r0 .. r0 + nr
@@ -141,6 +143,13 @@ __global__ __launch_bounds__(256, 5) void relpos_bwd_kernel(const SaMatParams p)
             }
             if (left) aL += a; else aR += a;
           }
+        }
+      }
+      if (row + p.Lk > whole) {          // (the last rows of the last head)
+        const long e = whole + lane, j = e - row;
+        if (lane < V && j >= 0 && j < p.Lk && (j < jl || j >= jr)) {
+          const float x = sa_to_f32<DT>(((const E*)p.g)[e]);
+          if (j < jl) aL += x; else aR += x;
         }
       }
     }

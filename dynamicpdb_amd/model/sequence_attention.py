@@ -114,7 +114,7 @@ def _strides(t):
     """strides of the three leading axes, 0 for axes of one entry (theirs may be anything)"""
     a, b, c, _ = t.stride()
     if t.is_contiguous():
-        return a, b, c
+        return (a, b, c) if t.numel() else (0, 0, 0)
     n = t.shape
     return (a if n[0] > 1 else 0, b if n[1] > 1 else 0, c if n[2] > 1 else 0)
 

@@ -200,6 +200,9 @@ def test_attention_empty_axes(Lq, Lk):
     table = torch.randn(32, 4, device=DEV)
     got = run(q, k, v, g, table)
     assert got["o"].shape == q.shape and got["dk"].shape == k.shape
+    if Lk == 0:                             # an empty part of a cache whose rows are not 16-byte aligned
+        none = torch.randn(2, 9, 2, 36, device=DEV).to(BF)[:, :0, :, 1:33]
+        assert bool((run(q, none, none, g, table)["o"] == 0).all())
     assert all(bool((x == 0).all()) for x in got.values())
 
 
@@ -391,7 +394,8 @@ def test_attention_saved_tensors_may_move():
 
 @pytest.mark.parametrize("H,Lq,Lk,nb,dist,both,off", [(1, 1, 1, 4, 2, True, 0), (3, 7, 5, 32, 128, True, 0), (8, 256, 256, 32, 128, True, 0), (2, 300, 1, 16, 64, True, 3),
                                                       (5, 1, 777, 32, 128, False, 700), (4, 333, 1001, 64, 500, True, -20), (2, 1100, 1300, 17, 1024, False, 0),
-                                                      (16, 3, 2, 512, 1024, True, 1000000), (1, 2000, 2600, 32, 128, True, 0)])
+                                                      (16, 3, 2, 512, 1024, True, 1000000), (1, 2000, 2600, 32, 128, True, 0), (1, 33, 401, 16, 20, True, 0),
+                                                      (3, 1, 5, 4, 2, True, -50), (1, 7, 1, 4, 2, True, -50), (3, 3, 3, 4, 2, True, 50), (1, 1, 9, 8, 5, False, 40)])
 @pytest.mark.parametrize("dt", [F32, BF, HF])
 def test_bias_matrix(H, Lq, Lk, nb, dist, both, off, dt):
     gen = torch.Generator(device=DEV).manual_seed(Lq)
