@@ -155,6 +155,29 @@ struct SaDma {
       if (!((live >> (row + i * STEP)) & 1)) *(sa_u32x4*)(tile + (i * 64 * NW + tid) * 16) = (sa_u32x4){0u, 0u, 0u, 0u};
   }
 };
+// The two tiles of a step side by side in LDS (K and V, or Q and dO).  One group of four waves: each loads its share of both; two
+// groups: the first loads one, the second the other.
+#define SA_PAIR_LDS (SA_WAVES * 64 * 8)        // what pairs exchange beside the tiles' memory: two floats per lane
+template <int DP, bool PAIR>
+struct SaKvTiles {
+  using T = SaTile<DP>;
+  const char *a, *b;
+  SaDma<DP> la, lb;
+  int tid, w, half;
+  __device__ __forceinline__ SaKvTiles(const char* pa, long rsa, const char* pb, long rsb, int D, int t, int wave)
+      : a(PAIR && wave >= SA_WAVES ? pb : pa), b(pb), la(PAIR && wave >= SA_WAVES ? rsb : rsa, D, t & (64 * SA_WAVES - 1)), lb(rsb, D, t & (64 * SA_WAVES - 1)),
+        tid(t & (64 * SA_WAVES - 1)), w(wave & (SA_WAVES - 1)), half(wave / SA_WAVES) {}
+  __device__ __forceinline__ void load(int row0, int end, char* tile) const { load(a, b, row0, end, tile); }
+  // the same from other bases (sa, sb: this wave's first, and for one group its second matrix)
+  __device__ __forceinline__ void load(const char* sa, const char* sb, int row0, int end, char* tile) const {
+    la.load(sa, row0, end, tile + (PAIR ? half * T::BYTES : 0), w);
+    if constexpr (!PAIR) lb.load(sb, row0, end, tile + T::BYTES, w);
+  }
+  __device__ __forceinline__ void zero(unsigned long live, char* tile) const {
+    la.zero(live, tile + (PAIR ? half * T::BYTES : 0), tid);
+    if constexpr (!PAIR) lb.zero(live, tile + T::BYTES, tid);
+  }
+};
 // every DMA of this wave has landed, then everybody's
 __device__ __forceinline__ void sa_landed() {
   asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
@@ -196,9 +219,10 @@ __device__ __forceinline__ int sa_q_offset(const SaRel& r, int b) {
   return min(max(r.q_offsets ? r.q_offsets[b] : r.q_offset, -(1 << 29)), 1 << 29);
 }
 // LDS rows of 2 W + 1 values per head: entry W + delta, delta = key position - query position in [-W, W]
+template <int NW>
 __device__ __forceinline__ void sa_fill_bias(float* lds, const SaRel& r, int head0, int nheads, int tid) {
   const int n = 2 * r.W + 1;
-  for (int i = tid; i < n * nheads; i += 64 * SA_WAVES) {
+  for (int i = tid; i < n * nheads; i += 64 * NW) {
     const int h = i / n, d = i - h * n - r.W;
     lds[i] = sa_bias_log2(r.table[(long)sa_bucket(r, d) * r.H + head0 + h]);
   }
@@ -206,8 +230,9 @@ __device__ __forceinline__ void sa_fill_bias(float* lds, const SaRel& r, int hea
 
 // one wave's share of a workgroup: the histogram over distances (hist[reach + delta], |delta| <= reach) summed into buckets j = w,
 // w + waves, ...; out[j].  A bucket is a run of distances on one side.
+template <int NW>
 __device__ __forceinline__ void sa_bucket_sums(const SaRel& r, const float* hist, int reach, int num_buckets, float* out, int w, int lane) {
-  for (int j = w; j < num_buckets; j += SA_WAVES) {
+  for (int j = w; j < num_buckets; j += NW) {
     const bool pos = r.both && j >= r.half;
     const int jj = pos ? j - r.half : j;
     const int nlo = max(sa_bucket_lo(r, jj), pos ? 1 : 0);

@@ -55,19 +55,21 @@ __device__ __forceinline__ void sa_logits(f32x16& s, float sl2, float nlse, cons
   }
 }
 
-template <int DT, int DP, bool REL>
-__global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_dq_kernel(const SaBwdParams p) {
+// PAIR: as in the forward, two waves for the same 32 rows, one per half of a key tile
+template <int DT, int DP, bool REL, bool PAIR>
+__global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_dq_kernel(const SaBwdParams p) {
   using T = SaTile<DP>;
-  constexpr int KS = T::KS, NT = T::NT;
+  constexpr int KS = T::KS, NT = T::NT, NW = PAIR ? 2 * SA_WAVES : SA_WAVES, NB = PAIR ? 1 : 2;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  float* const ldsB = (float*)(smem + 4 * T::BYTES);
+  float* const ldsB = (float*)(smem + 4 * T::BYTES + (PAIR ? SA_PAIR_LDS : 0));
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l31 = lane & 31, h = lane >> 5;
   unsigned id = sa_work_id();
   const int rb = id % p.nrb; id /= p.nrb;
   const int sp = id % p.splits_q; id /= p.splits_q;
   const int head = id % p.H, b = id / p.H, hkv = head / (p.H / p.Hkv);
-  const int row_w = rb * SA_ROWS + w * 32, row = row_w + l31;
+  const int wr = w & (SA_WAVES - 1), half = PAIR ? w / SA_WAVES : 0;
+  const int row_w = rb * SA_ROWS + wr * 32, row = row_w + l31;
   const bool wave_on = row_w < p.Lq, on = row < p.Lq;
   const int qi = min(row, p.Lq - 1);
 
@@ -80,7 +82,7 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_dq_kernel(const SaB
   float bL = 0.f, bR = 0.f;
   const float* myb = ldsB + p.rel.W;
   if constexpr (REL) {
-    sa_fill_bias(ldsB, p.rel, head, 1, tid);
+    sa_fill_bias<NW>(ldsB, p.rel, head, 1, tid);
     const int off = sa_q_offset(p.rel, b);
     qpos = qi + off;
     qlo = row_w + off;
@@ -126,12 +128,11 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_dq_kernel(const SaB
     for (int r = 0; r < 16; ++r) dq[i][r] = 0.f;
 
   float left = 0.f;          // row sum of dS
-  const SaAddr<DP> ad(lane);
-  const SaDma<DP> ldk(p.k_sl, p.D, tid), ldv(p.v_sl, p.D, tid);
+  const SaAddr<DP> ad(lane, half * 32);
+  const SaKvTiles<DP, PAIR> kv(kb_, p.k_sl, vb_, p.v_sl, p.D, tid, w);
   int kmask = 0;
   auto fetch = [&](int t, char* tile) {
-    ldk.load(kb_, t * SA_KT, kv_end, tile, w);
-    ldv.load(vb_, t * SA_KT, kv_end, tile + T::BYTES, w);
+    kv.load(t * SA_KT, kv_end, tile);
     const int key = t * SA_KT + lane;
     kmask = key < kv_end ? (mb_ ? mb_[key] : 1) : 0;
   };
@@ -143,13 +144,12 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_dq_kernel(const SaB
     if (t + 1 < t1) fetch(t + 1, smem + (1 - decltype(stage)::value) * 2 * T::BYTES);
     if (live != ~0ul) {
       if (live == 0) return;
-      ldk.zero(live, lk, tid);
-      ldv.zero(live, lv, tid);
+      kv.zero(live, lk);
       __syncthreads();
     }
     if (!wave_on) return;
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
+    for (int kb = 0; kb < NB; ++kb) {
       f32x16 s, dp;
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[r] = dp[r] = 0.f;
@@ -158,11 +158,11 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_dq_kernel(const SaB
         s = sa_mfma<DT>(ad.rows(lk, kb * 32, ks), qf[ks], s);
         dp = sa_mfma<DT>(ad.rows(lv, kb * 32, ks), of[ks], dp);
       }
-      const int k0 = t * SA_KT + kb * 32;
+      const int k0 = t * SA_KT + (half + kb) * 32;
       const int far = !REL ? 0 : k0 - qhi >= p.rel.W ? 1 : k0 + 31 - qlo <= -p.rel.W ? -1 : 0;
       sa_logits<REL>(s, p.sl2, -lse, myb, p.rel.W, far, far > 0 ? bR : bL, k0 + 4 * h - qpos);
       if (live != ~0ul) {
-        const unsigned bits = (unsigned)(live >> (kb * 32)) >> (4 * h);
+        const unsigned bits = (unsigned)(live >> ((half + kb) * 32)) >> (4 * h);
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (!((bits >> (8 * (r >> 2) + (r & 3))) & 1)) s[r] = -INFINITY;
@@ -174,7 +174,7 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_dq_kernel(const SaB
       }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        sa_u32x4 df;      // dS in the operand type: relative error 2^-9 (bf16) / 2^-12 (f16) of each term of dQ's sum
+        sa_u32x4 df;      // dS in the operand type: relative error up to 2^-8 (bf16) / 2^-11 (f16) of each term of dQ's sum
 #pragma unroll
         for (int e = 0; e < 4; ++e) df[e] = sa_pack2<DT>(s[8 * c + 2 * e], s[8 * c + 2 * e + 1]);
 #pragma unroll
@@ -189,6 +189,21 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_dq_kernel(const SaB
   }
 
   left = sa_xsum(left);
+  if constexpr (PAIR) {
+    float* const ls = (float*)(smem + 4 * T::BYTES) + wr * 64 + lane;
+    f32x16* const acc = (f32x16*)smem + wr * NT * 64 + lane;
+    __syncthreads();
+    if (half) {
+      *ls = left;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) acc[i * 64] = dq[i];
+    }
+    __syncthreads();
+    if (half) return;
+    left += *ls;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) dq[i] += acc[i * 64];
+  }
   if (on && h == 0) {
     // parts of the key axis: plane 0 holds delta, plane 1 + part the part's row sum (seq_attn_delta_kernel adds them up)
     if (p.splits_q == 1) p.delta[rowi] = dl + left;
@@ -216,21 +231,23 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_dq_kernel(const SaB
   }
 }
 
-// Four waves of 32 keys each, K^T and V^T operands in registers.  At D = 128 that takes more than 256 registers: one wave per SIMD, and
-// nothing runs under its products.  PAIR: eight waves, two for the same 32 keys, one per 32-query half of a tile, V^T operands from LDS;
-// the two sums meet in LDS at the end.
-template <int DP, bool REL>
+// Four waves of 32 keys each, K^T and V^T operands in registers; PAIR: eight waves, two for the same 32 keys, one per 32-query half of
+// a tile; the two sums meet in LDS at the end.  Small launches then have two waves per SIMD.  At D = 128 the four-wave form needs more
+// than 256 registers, one wave per SIMD, and nothing runs under its products: always PAIR there, with V^T operands from LDS (417 -> 303
+// us) -- except with a bias, where the eight waves' blocks of dS would not fit LDS.
+template <int DP, bool REL, bool PAIR>
 struct SaDkvCfg {
-  static constexpr bool PAIR = DP == 128 && !REL;      // (with a bias the eight waves' blocks of dS would not fit LDS)
+  static constexpr bool VLDS = PAIR && DP == 128;
   static constexpr int WAVES = PAIR ? 2 * SA_WAVES : SA_WAVES;
-  static constexpr int LDS = 4 * SaTile<DP>::BYTES + 4 * SA_KT * 4 + (PAIR ? SA_ROWS * SaTile<DP>::PITCH : 0);
+  static constexpr int LDS = 4 * SaTile<DP>::BYTES + 4 * SA_KT * 4 + (VLDS ? SA_ROWS * SaTile<DP>::PITCH : 0);
+  static int bytes(int W) { return LDS + (REL ? (2 * W + 1 + WAVES * (2 * (W + SA_REACH) + 1 + SA_DIAG)) * 4 : 0); }
 };
-template <int DT, int DP, bool REL>
-__global__ __launch_bounds__((64 * SaDkvCfg<DP, REL>::WAVES), (DP == 128 && REL ? 1 : 2)) void seq_attn_dkv_kernel(const SaBwdParams p) {
+template <int DT, int DP, bool REL, bool PAIR>
+__global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, (DP == 128 && REL ? 1 : 2)) void seq_attn_dkv_kernel(const SaBwdParams p) {
   using T = SaTile<DP>;
   constexpr int KS = T::KS, NT = T::NT;
-  constexpr bool PAIR = SaDkvCfg<DP, REL>::PAIR;
-  constexpr int NW = SaDkvCfg<DP, REL>::WAVES;
+  constexpr bool VLDS = SaDkvCfg<DP, REL, PAIR>::VLDS;
+  constexpr int NW = SaDkvCfg<DP, REL, PAIR>::WAVES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   float* const ldsL = (float*)(smem + 4 * T::BYTES);            // [stage][log-sum | delta][SA_KT]
   char* const ldsV = smem + 4 * T::BYTES + 4 * SA_KT * 4;
@@ -244,7 +261,7 @@ __global__ __launch_bounds__((64 * SaDkvCfg<DP, REL>::WAVES), (DP == 128 && REL 
   const int kbk = id % nkb; id /= nkb;
   const int sp = id % p.splits_k; id /= p.splits_k;
   const int hkv = id % p.Hkv, b = id / p.Hkv;
-  const int wk = w & (SA_WAVES - 1), half = w / SA_WAVES;
+  const int wk = w & (SA_WAVES - 1), half = PAIR ? w / SA_WAVES : 0;
   const int key_w = kbk * SA_ROWS + wk * 32, key = key_w + l31;
 
   int kv_end = p.Lk;
@@ -257,7 +274,7 @@ __global__ __launch_bounds__((64 * SaDkvCfg<DP, REL>::WAVES), (DP == 128 && REL 
   const int nqt = (p.Lq + SA_KT - 1) / SA_KT, nu = G * nqt, per = (nu + p.splits_k - 1) / p.splits_k;
   const int u0 = sp * per, u1 = wg_on ? min(nu, u0 + per) : 0;
 
-  sa_u32x4 kf[KS], vf[PAIR ? 1 : KS];
+  sa_u32x4 kf[KS], vf[VLDS ? 1 : KS];
   {
     const char* sk = p.k + ((long)b * p.k_sb + (long)key * p.k_sl + (long)hkv * p.k_sh) * 2;
     const char* sv = p.v + ((long)b * p.v_sb + (long)key * p.v_sl + (long)hkv * p.v_sh) * 2;
@@ -266,13 +283,13 @@ __global__ __launch_bounds__((64 * SaDkvCfg<DP, REL>::WAVES), (DP == 128 && REL 
       const int d = ks * 16 + h * 8;
       kf[ks] = (sa_u32x4){0u, 0u, 0u, 0u};
       if (key_on && d < p.D) kf[ks] = *(const sa_u32x4*)(sk + d * 2);
-      if constexpr (!PAIR) {
+      if constexpr (!VLDS) {
         vf[ks] = (sa_u32x4){0u, 0u, 0u, 0u};
         if (key_on && d < p.D) vf[ks] = *(const sa_u32x4*)(sv + d * 2);
       }
     }
   }
-  if constexpr (PAIR)
+  if constexpr (VLDS)
     if (u0 < u1) {
       const SaDma<DP, NW, SA_ROWS> ldv(p.v_sl, p.D, tid);
       ldv.load(p.v + ((long)b * p.v_sb + (long)hkv * p.v_sh) * 2, kbk * SA_ROWS, kv_end, ldsV, w);
@@ -286,7 +303,7 @@ __global__ __launch_bounds__((64 * SaDkvCfg<DP, REL>::WAVES), (DP == 128 && REL 
   int off = 0, head_in = -1;
   const float* myb = ldsB + p.rel.W;
   float* const myh = ldsH + w * hn + p.rel.W + SA_REACH;
-  float* const diag = ldsH + SA_WAVES * hn + w * SA_DIAG + 32;   // 32 rows of 64 behind a margin of 32; columns 32 .. 63 and the margin are zero
+  float* const diag = ldsH + NW * hn + w * SA_DIAG + 32;   // 32 rows of 64 behind a margin of 32; columns 32 .. 63 and the margin are zero
   float accL = 0.f, accR = 0.f;
   auto table_part = [&](int head) { return p.ws_t + ((((long)b * p.H + head) * p.splits_k + sp) * nkb + kbk) * p.num_buckets; };
   // a head's histogram over distances -> its buckets; the far sums belong to the last bucket of their side
@@ -299,14 +316,14 @@ __global__ __launch_bounds__((64 * SaDkvCfg<DP, REL>::WAVES), (DP == 128 && REL 
     }
     accL = accR = 0.f;
     __syncthreads();
-    for (int i = tid; i < hn; i += 64 * SA_WAVES) {
+    for (int i = tid; i < hn; i += 64 * NW) {
       float a = 0.f;
 #pragma unroll
-      for (int c = 0; c < SA_WAVES; ++c) a += ldsH[c * hn + i];
+      for (int c = 0; c < NW; ++c) a += ldsH[c * hn + i];
       ldsH[i] = a;             // (entry i of every copy is this thread's)
     }
     __syncthreads();
-    sa_bucket_sums(p.rel, ldsH, p.rel.W + SA_REACH, p.num_buckets, table_part(head), w, lane);
+    sa_bucket_sums<NW>(p.rel, ldsH, p.rel.W + SA_REACH, p.num_buckets, table_part(head), w, lane);
     __syncthreads();
   };
   if constexpr (REL) {
@@ -314,19 +331,19 @@ __global__ __launch_bounds__((64 * SaDkvCfg<DP, REL>::WAVES), (DP == 128 && REL 
     for (int i = lane; i < SA_DIAG; i += 64) diag[i - 32] = 0.f;
     for (int g = 0; g < G; ++g)          // heads this part does not touch
       if (max(u0, g * nqt) >= min(u1, (g + 1) * nqt))
-        for (int j = tid; j < p.num_buckets; j += 64 * SA_WAVES) table_part(hkv * G + g)[j] = 0.f;
+        for (int j = tid; j < p.num_buckets; j += 64 * NW) table_part(hkv * G + g)[j] = 0.f;
   }
 
   const SaAddr<DP> ad(lane, half * 32);
-  const SaDma<DP, NW> ldq(p.q_sl, p.D, tid), ldg(p.do_sl, p.D, tid);
+  const SaKvTiles<DP, PAIR> qg(p.q, p.q_sl, p.d_o, p.do_sl, p.D, tid, w);
   const char* const lv = ldsV + (wk - half) * 32 * T::PITCH;
   float lse_r = 0.f, del_r = 0.f;
   // position in the walk of the unit that is fetched next, and of the one that is worked on
   int fg = u0 / nqt, fq = (u0 - fg * nqt) * SA_KT, wg = fg, wq = fq;
   auto fetch = [&](char* tile) {
     const int head = hkv * G + fg;
-    ldq.load(p.q + ((long)b * p.q_sb + (long)head * p.q_sh) * 2, fq, p.Lq, tile, w);
-    ldg.load(p.d_o + ((long)b * p.do_sb + (long)head * p.do_sh) * 2, fq, p.Lq, tile + T::BYTES, w);
+    const long oq = ((long)b * p.q_sb + (long)head * p.q_sh) * 2, og = ((long)b * p.do_sb + (long)head * p.do_sh) * 2;
+    qg.load(qg.a + (half ? og : oq), qg.b + og, fq, p.Lq, tile);
     if (tid < SA_KT) {
       const int qi = fq + tid;
       const long r = ((long)b * p.H + head) * p.Lq + qi;
@@ -344,8 +361,8 @@ __global__ __launch_bounds__((64 * SaDkvCfg<DP, REL>::WAVES), (DP == 128 && REL 
       const int head = hkv * G + wg;
       if (head != head_in) {       // (uniform)
         if (head_in >= 0) flush(head_in);      // (ends in a barrier: nobody reads the previous head's rows any more)
-        for (int i = tid; i < SA_WAVES * hn; i += 64 * SA_WAVES) ldsH[i] = 0.f;
-        sa_fill_bias(ldsB, p.rel, head, 1, tid);
+        for (int i = tid; i < NW * hn; i += 64 * NW) ldsH[i] = 0.f;
+        sa_fill_bias<NW>(ldsB, p.rel, head, 1, tid);
         head_in = head;
       }
     }
@@ -367,7 +384,7 @@ __global__ __launch_bounds__((64 * SaDkvCfg<DP, REL>::WAVES), (DP == 128 && REL 
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks) {
         s = sa_mfma<DT>(ad.rows(lq, qb * 32, ks), kf[ks], s);
-        dp = sa_mfma<DT>(ad.rows(lg, qb * 32, ks), PAIR ? ad.rows(lv, 0, ks) : vf[PAIR ? 0 : ks], dp);
+        dp = sa_mfma<DT>(ad.rows(lg, qb * 32, ks), VLDS ? ad.rows(lv, 0, ks) : vf[VLDS ? 0 : ks], dp);
       }
       const int qlo = q0 + qs + off, qhi = qlo + 31;
       const int far = !REL ? 0 : key_w - qhi >= p.rel.W ? 1 : key_w + 31 - qlo <= -p.rel.W ? -1 : 0;
@@ -421,7 +438,7 @@ __global__ __launch_bounds__((64 * SaDkvCfg<DP, REL>::WAVES), (DP == 128 && REL 
       }
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        sa_u32x4 pf, df;      // P and dS in the operand type: relative error 2^-9 (bf16) / 2^-12 (f16) of each term
+        sa_u32x4 pf, df;      // P and dS in the operand type: relative error up to 2^-8 (bf16) / 2^-11 (f16) of each term
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           pf[e] = sa_pack2<DT>(s[8 * c + 2 * e], s[8 * c + 2 * e + 1]);
@@ -513,13 +530,22 @@ static int sa_launch_bwd(K kernel, const SaBwdParams& p, long nwg, int waves, in
   DFOLD_LAUNCH(kernel, dim3((unsigned)nwg), dim3(64 * waves), lds, st, p);
   return dfold_check_launch();
 }
+template <int DT, int DP, bool REL, bool PAIR>
+static int sa_dq(const SaBwdParams& p, hipStream_t st) {
+  struct Mine;
+  const int lds = 4 * SaTile<DP>::BYTES + (PAIR ? SA_PAIR_LDS : 0) + (REL ? (2 * p.rel.W + 1) * 4 : 0);
+  return sa_launch_bwd<Mine>(seq_attn_dq_kernel<DT, DP, REL, PAIR>, p, (long)p.nrb * p.splits_q * p.H * p.B, PAIR ? 2 * SA_WAVES : SA_WAVES, lds, st);
+}
+template <int DT, int DP, bool REL, bool PAIR>
+static int sa_dkv(const SaBwdParams& p, hipStream_t st) {
+  struct Mine;
+  const long nkb = (p.Lk + SA_ROWS - 1) / SA_ROWS;
+  using C = SaDkvCfg<DP, REL, PAIR>;
+  return sa_launch_bwd<Mine>(seq_attn_dkv_kernel<DT, DP, REL, PAIR>, p, nkb * p.splits_k * p.Hkv * p.B, C::WAVES, C::bytes(p.rel.W), st);
+}
 template <int DT, int DP, bool REL>
-static int sa_bwd_dp(const SaBwdParams& p, hipStream_t st) {
-  const int bias = REL ? (2 * p.rel.W + 1) * 4 : 0, hist = REL ? SA_WAVES * (2 * (p.rel.W + SA_REACH) + 1 + SA_DIAG) * 4 : 0;
-  struct Dq;
-  struct Dkv;
-  int rc = sa_launch_bwd<Dq>(seq_attn_dq_kernel<DT, DP, REL>, p, (long)p.nrb * p.splits_q * p.H * p.B, SA_WAVES,
-                         4 * SaTile<DP>::BYTES + bias, st);
+static int sa_bwd_dp(const SaBwdParams& p, bool pair_q, bool pair_k, hipStream_t st) {
+  int rc = pair_q ? sa_dq<DT, DP, REL, true>(p, st) : sa_dq<DT, DP, REL, false>(p, st);
   if (rc != DFOLD_OK) return rc;
   if (p.splits_q > 1) {
     const long n8 = (long)p.B * p.Lq * p.H * p.D / 8;
@@ -530,8 +556,9 @@ static int sa_bwd_dp(const SaBwdParams& p, hipStream_t st) {
     if ((rc = dfold_check_launch()) != DFOLD_OK) return rc;
   }
   const long nkb = (p.Lk + SA_ROWS - 1) / SA_ROWS;
-  rc = sa_launch_bwd<Dkv>(seq_attn_dkv_kernel<DT, DP, REL>, p, nkb * p.splits_k * p.Hkv * p.B, SaDkvCfg<DP, REL>::WAVES,
-                     SaDkvCfg<DP, REL>::LDS + bias + hist, st);
+  if constexpr (DP == 128) rc = sa_dkv<DT, DP, REL, !REL>(p, st);
+  else if (pair_k && SaDkvCfg<DP, REL, true>::bytes(p.rel.W) <= SA_MAX_LDS) rc = sa_dkv<DT, DP, REL, true>(p, st);
+  else rc = sa_dkv<DT, DP, REL, false>(p, st);
   if (rc != DFOLD_OK) return rc;
   if (REL) {
     DFOLD_LAUNCH(seq_dtable_kernel, dim3(p.H, (p.num_buckets + 63) / 64), dim3(1024), 0, st, (const float*)p.ws_t, p.dtable, p.num_buckets,
@@ -548,10 +575,10 @@ static int sa_bwd_dp(const SaBwdParams& p, hipStream_t st) {
   return DFOLD_OK;
 }
 template <int DT>
-static int sa_bwd(const SaBwdParams& p, bool rel, hipStream_t st) {
-  if (p.D <= 32) return rel ? sa_bwd_dp<DT, 32, true>(p, st) : sa_bwd_dp<DT, 32, false>(p, st);
-  if (p.D <= 64) return rel ? sa_bwd_dp<DT, 64, true>(p, st) : sa_bwd_dp<DT, 64, false>(p, st);
-  return rel ? sa_bwd_dp<DT, 128, true>(p, st) : sa_bwd_dp<DT, 128, false>(p, st);
+static int sa_bwd(const SaBwdParams& p, bool rel, bool pq, bool pk, hipStream_t st) {
+  if (p.D <= 32) return rel ? sa_bwd_dp<DT, 32, true>(p, pq, pk, st) : sa_bwd_dp<DT, 32, false>(p, pq, pk, st);
+  if (p.D <= 64) return rel ? sa_bwd_dp<DT, 64, true>(p, pq, pk, st) : sa_bwd_dp<DT, 64, false>(p, pq, pk, st);
+  return rel ? sa_bwd_dp<DT, 128, true>(p, pq, pk, st) : sa_bwd_dp<DT, 128, false>(p, pq, pk, st);
 }
 
 extern "C" int dfold_seq_attn_bwd(const dfold_seq_attn_desc* d, const dfold_seq_attn_grad* g, void* stream) {
@@ -582,5 +609,6 @@ extern "C" int dfold_seq_attn_bwd(const dfold_seq_attn_desc* d, const dfold_seq_
   p.ws_q = g->ws;
   p.ws_k = g->ws + (p.splits_q > 1 ? up4(p.splits_q * nq) : 0);
   p.ws_t = p.ws_k + (p.splits_k > 1 ? up4(2 * p.splits_k * nk) : 0);
-  return d->dtype == DFOLD_DT_BF16 ? sa_bwd<DFOLD_DT_BF16>(p, rel, (hipStream_t)stream) : sa_bwd<DFOLD_DT_F16>(p, rel, (hipStream_t)stream);
+  const bool pq = g->pair_q != 0, pk = g->pair_k != 0;
+  return d->dtype == DFOLD_DT_BF16 ? sa_bwd<DFOLD_DT_BF16>(p, rel, pq, pk, (hipStream_t)stream) : sa_bwd<DFOLD_DT_F16>(p, rel, pq, pk, (hipStream_t)stream);
 }

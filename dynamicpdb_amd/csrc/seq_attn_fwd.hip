@@ -28,12 +28,14 @@ struct SaFwdParams {
 #define SA_LAZY 8.f
 #define SA_MAX_SPLITS 1024
 
-template <int DT, int DP, bool REL>
-__global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_fwd_kernel(const SaFwdParams p) {
+// PAIR: eight waves, two for the same 32 rows, one per half of a key tile, joined in LDS at the end: a launch of at most one workgroup
+// per CU has two waves per SIMD instead of one.
+template <int DT, int DP, bool REL, bool PAIR>
+__global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_fwd_kernel(const SaFwdParams p) {
   using T = SaTile<DP>;
-  constexpr int KS = T::KS, NT = T::NT;
+  constexpr int KS = T::KS, NT = T::NT, NW = PAIR ? 2 * SA_WAVES : SA_WAVES, NB = PAIR ? 1 : 2;      // NB: 32-key blocks of a wave
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  float* const ldsB = (float*)(smem + 4 * T::BYTES);
+  float* const ldsB = (float*)(smem + 4 * T::BYTES + (PAIR ? SA_PAIR_LDS : 0));
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l31 = lane & 31, h = lane >> 5;
   unsigned id = sa_work_id();
@@ -42,7 +44,8 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_fwd_kernel(const Sa
   const int hgs = p.H / p.pack, hg = id % hgs, b = id / hgs;
   const int head0 = hg * p.pack, hkv = head0 / (p.H / p.Hkv);
   const int rows = p.Lq * p.pack;
-  const int row_w = rb * SA_ROWS + w * 32, row = row_w + l31;
+  const int wr = w & (SA_WAVES - 1), half = PAIR ? w / SA_WAVES : 0;
+  const int row_w = rb * SA_ROWS + wr * 32, row = row_w + l31;
   const bool wave_on = row_w < rows, on = row < rows;
   const int rowc = min(row, rows - 1), qi = rowc / p.pack, hl = rowc - qi * p.pack;
 
@@ -56,7 +59,7 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_fwd_kernel(const Sa
   const float* myb = nullptr;
   float bL = 0.f, bR = 0.f;
   if constexpr (REL) {
-    sa_fill_bias(ldsB, p.rel, head0, p.pack, tid);
+    sa_fill_bias<NW>(ldsB, p.rel, head0, p.pack, tid);
     const int off = sa_q_offset(p.rel, b);
     qpos = qi + off;
     qlo = row_w / p.pack + off;
@@ -94,12 +97,11 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_fwd_kernel(const Sa
     for (int r = 0; r < 16; ++r) O[i][r] = 0.f;
   float m = -INFINITY, l = 0.f;
 
-  const SaAddr<DP> ad(lane);
-  const SaDma<DP> ldk(p.k_sl, p.D, tid), ldv(p.v_sl, p.D, tid);
+  const SaAddr<DP> ad(lane, half * 32);
+  const SaKvTiles<DP, PAIR> kv(kb_, p.k_sl, vb_, p.v_sl, p.D, tid, w);
   int kmask = 0;
   auto fetch = [&](int t, char* tile) {
-    ldk.load(kb_, t * SA_KT, kv_end, tile, w);
-    ldv.load(vb_, t * SA_KT, kv_end, tile + T::BYTES, w);
+    kv.load(t * SA_KT, kv_end, tile);
     const int key = t * SA_KT + lane;
     kmask = key < kv_end ? (mb_ ? mb_[key] : 1) : 0;
   };
@@ -111,16 +113,15 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_fwd_kernel(const Sa
     if (t + 1 < t1) fetch(t + 1, smem + (1 - decltype(stage)::value) * 2 * T::BYTES);
     if (live != ~0ul) {
       if (live == 0) return;
-      ldk.zero(live, lk, tid);
-      ldv.zero(live, lv, tid);
+      kv.zero(live, lk);
       __syncthreads();
     }
     if (!wave_on) return;
 
     // S^T: keys x rows
-    f32x16 s[2];
+    f32x16 s[NB];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
+    for (int kb = 0; kb < NB; ++kb) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) s[kb][r] = 0.f;
 #pragma unroll
@@ -128,8 +129,8 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_fwd_kernel(const Sa
     }
     if constexpr (REL) {
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        const int k0 = t * SA_KT + kb * 32;
+      for (int kb = 0; kb < NB; ++kb) {
+        const int k0 = t * SA_KT + (half + kb) * 32;
         if (k0 - qhi >= p.rel.W || k0 + 31 - qlo <= -p.rel.W) {       // the whole block lies in the last bucket of a side
           const float c = k0 - qhi >= p.rel.W ? bR : bL;
 #pragma unroll
@@ -146,16 +147,18 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_fwd_kernel(const Sa
     }
     if (live != ~0ul) {
 #pragma unroll
-      for (int kb = 0; kb < 2; ++kb) {
-        const unsigned bits = (unsigned)(live >> (kb * 32)) >> (4 * h);
+      for (int kb = 0; kb < NB; ++kb) {
+        const unsigned bits = (unsigned)(live >> ((half + kb) * 32)) >> (4 * h);
 #pragma unroll
         for (int r = 0; r < 16; ++r)
           if (!((bits >> (8 * (r >> 2) + (r & 3))) & 1)) s[kb][r] = -INFINITY;
       }
     }
-    float mt = fmaxf(s[0][0], s[1][0]);
+    float mt = -INFINITY;
 #pragma unroll
-    for (int r = 1; r < 16; ++r) mt = fmaxf(fmaxf(mt, s[0][r]), s[1][r]);
+    for (int kb = 0; kb < NB; ++kb)
+#pragma unroll
+      for (int r = 0; r < 16; r += 2) mt = fmaxf(fmaxf(mt, s[kb][r]), s[kb][r + 1]);
     mt = sa_xmax(mt);
     if (__ballot(mt > m + lazy)) {
       const float mn = fmaxf(m, mt), a = m == mn ? 1.f : sa_exp2((m - mn) * us);     // (m == mn also for rows without keys so far)
@@ -167,21 +170,21 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_fwd_kernel(const Sa
         for (int r = 0; r < 16; ++r) O[i][r] *= a;
     }
     const float nm = m == -INFINITY ? 0.f : -m * us;
-    sa_u32x4 pf[4];
+    sa_u32x4 pf[2 * NB];
 #pragma unroll
-    for (int kb = 0; kb < 2; ++kb) {
+    for (int kb = 0; kb < NB; ++kb) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
         s[kb][r] = sa_exp2(REL ? s[kb][r] + nm : __builtin_fmaf(s[kb][r], sl2, nm));
         l += s[kb][r];
       }
 #pragma unroll
-      for (int c = 0; c < 2; ++c)      // P in the operand type: relative error 2^-9 (bf16) / 2^-12 (f16) of each term of O's sum
+      for (int c = 0; c < 2; ++c)      // P in the operand type: relative error up to 2^-8 (bf16) / 2^-11 (f16) of each term of O's sum
 #pragma unroll
         for (int e = 0; e < 4; ++e) pf[kb * 2 + c][e] = sa_pack2<DT>(s[kb][8 * c + 2 * e], s[kb][8 * c + 2 * e + 1]);
     }
 #pragma unroll
-    for (int c = 0; c < 4; ++c)
+    for (int c = 0; c < 2 * NB; ++c)
 #pragma unroll
       for (int i = 0; i < NT; ++i) O[i] = sa_mfma<DT>(ad.cols(lv, c * 16, i), pf[c], O[i]);
   };
@@ -191,8 +194,32 @@ __global__ __launch_bounds__(64 * SA_WAVES, 2) void seq_attn_fwd_kernel(const Sa
     if (t + 1 < t1) step(t + 1, SaInt<1>());
   }
 
-  if (!wave_on) return;
   l = sa_xsum(l);
+  if constexpr (PAIR) {
+    // the second wave of a pair hands its maximum, sum and O over through the tiles' memory
+    float* const ml = (float*)(smem + 4 * T::BYTES) + (wr * 64 + lane) * 2;
+    f32x16* const acc = (f32x16*)smem + wr * NT * 64 + lane;
+    __syncthreads();
+    if (half) {
+      ml[0] = m;
+      ml[1] = l;
+#pragma unroll
+      for (int i = 0; i < NT; ++i) acc[i * 64] = O[i];
+    }
+    __syncthreads();
+    if (half) return;
+    const float m1 = ml[0], mn = fmaxf(m, m1);
+    const float a0 = m == mn ? 1.f : sa_exp2((m - mn) * us), a1 = m1 == mn ? 1.f : sa_exp2((m1 - mn) * us);
+    m = mn;
+    l = l * a0 + ml[1] * a1;
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const f32x16 o1 = acc[i * 64];
+#pragma unroll
+      for (int r = 0; r < 16; ++r) O[i][r] = O[i][r] * a0 + o1[r] * a1;
+    }
+  }
+  if (!wave_on) return;
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
   if (!on) return;
   const int head = head0 + hl;
@@ -301,21 +328,23 @@ __global__ __launch_bounds__(256) void seq_attn_combine_row_kernel(const SaFwdPa
       (uint2){sa_pack2<DT>(o[0] * inv, o[1] * inv), sa_pack2<DT>(o[2] * inv, o[3] * inv)};
 }
 
-template <int DT, int DP, bool REL>
+template <int DT, int DP, bool REL, bool PAIR>
 static int sa_launch_fwd(const SaFwdParams& p, unsigned nwg, hipStream_t st) {
-  const int lds = 4 * SaTile<DP>::BYTES + (REL ? p.pack * (2 * p.rel.W + 1) * 4 : 0);
   struct Mine;
+  const int lds = 4 * SaTile<DP>::BYTES + (PAIR ? SA_PAIR_LDS : 0) + (REL ? p.pack * (2 * p.rel.W + 1) * 4 : 0);
   if (lds > SA_MAX_LDS) return DFOLD_EINVAL;
-  if (!sa_raise_lds<Mine>(seq_attn_fwd_kernel<DT, DP, REL>, lds)) return DFOLD_ELAUNCH;
-  DFOLD_LAUNCH((seq_attn_fwd_kernel<DT, DP, REL>), dim3(nwg), dim3(64 * SA_WAVES), lds, st, p);
+  if (!sa_raise_lds<Mine>(seq_attn_fwd_kernel<DT, DP, REL, PAIR>, lds)) return DFOLD_ELAUNCH;
+  DFOLD_LAUNCH((seq_attn_fwd_kernel<DT, DP, REL, PAIR>), dim3(nwg), dim3((PAIR ? 2 : 1) * 64 * SA_WAVES), lds, st, p);
   return dfold_check_launch();
 }
+template <int DT, int DP>
+static int sa_fwd_dp(const SaFwdParams& p, bool rel, bool pair, unsigned nwg, hipStream_t st) {
+  if (rel) return pair ? sa_launch_fwd<DT, DP, true, true>(p, nwg, st) : sa_launch_fwd<DT, DP, true, false>(p, nwg, st);
+  return pair ? sa_launch_fwd<DT, DP, false, true>(p, nwg, st) : sa_launch_fwd<DT, DP, false, false>(p, nwg, st);
+}
 template <int DT>
-static int sa_fwd(const SaFwdParams& p, bool rel, unsigned nwg, hipStream_t st) {
-  int rc;
-  if (p.D <= 32) rc = rel ? sa_launch_fwd<DT, 32, true>(p, nwg, st) : sa_launch_fwd<DT, 32, false>(p, nwg, st);
-  else if (p.D <= 64) rc = rel ? sa_launch_fwd<DT, 64, true>(p, nwg, st) : sa_launch_fwd<DT, 64, false>(p, nwg, st);
-  else rc = rel ? sa_launch_fwd<DT, 128, true>(p, nwg, st) : sa_launch_fwd<DT, 128, false>(p, nwg, st);
+static int sa_fwd(const SaFwdParams& p, bool rel, bool pair, unsigned nwg, hipStream_t st) {
+  const int rc = p.D <= 32 ? sa_fwd_dp<DT, 32>(p, rel, pair, nwg, st) : p.D <= 64 ? sa_fwd_dp<DT, 64>(p, rel, pair, nwg, st) : sa_fwd_dp<DT, 128>(p, rel, pair, nwg, st);
   if (rc != DFOLD_OK || p.splits == 1) return rc;
   const long rows = (long)p.B * p.Lq * p.H, n = rows * (p.D / 8);
   if (p.splits >= 8 && rows <= 65536) {
@@ -342,6 +371,6 @@ extern "C" int dfold_seq_attn_fwd(const dfold_seq_attn_desc* d, void* stream) {
   const long nwg = nrb * d->splits * (d->H / d->pack) * d->B, n = (long)d->B * d->Lq * d->H * (d->D / 8);
   if (rows > 0x7fffff00L || nwg > 0x7fffffffL || n / 256 > 0x7ffffff0L) return DFOLD_EINVAL;
   p.nrb = (int)nrb;
-  return d->dtype == DFOLD_DT_BF16 ? sa_fwd<DFOLD_DT_BF16>(p, d->rel.table != nullptr, (unsigned)nwg, (hipStream_t)stream)
-                                   : sa_fwd<DFOLD_DT_F16>(p, d->rel.table != nullptr, (unsigned)nwg, (hipStream_t)stream);
+  return d->dtype == DFOLD_DT_BF16 ? sa_fwd<DFOLD_DT_BF16>(p, d->rel.table != nullptr, d->pair != 0, (unsigned)nwg, (hipStream_t)stream)
+                                   : sa_fwd<DFOLD_DT_F16>(p, d->rel.table != nullptr, d->pair != 0, (unsigned)nwg, (hipStream_t)stream);
 }

@@ -172,7 +172,7 @@ __global__ __launch_bounds__(256, 5) void relpos_bwd_kernel(const SaMatParams p)
   __syncthreads();
   if (tid < 2) hist[tid ? 2 * W : 0] = (side[tid][0] + side[tid][1]) + (side[tid][2] + side[tid][3]);
   __syncthreads();
-  sa_bucket_sums(p.rel, hist, W, p.nb, p.ws + ((long)head * p.nblk + blockIdx.x) * p.nb, w, lane);
+  sa_bucket_sums<4>(p.rel, hist, W, p.nb, p.ws + ((long)head * p.nblk + blockIdx.x) * p.nb, w, lane);
 }
 
 // row blocks of the backward: five workgroups per CU, one round of what fits (2048 of them: a second round of three, 170 -> 167 us at

@@ -44,12 +44,12 @@ class RelBias(ctypes.Structure):
 class AttnDesc(ctypes.Structure):
     _fields_ = ([(n, c_void_p) for n in ("q", "k", "v", "o", "lse", "ws", "key_mask", "kv_lens")] +
                 [(n, c_int64) for n in ("q_sb", "q_sl", "q_sh", "k_sb", "k_sl", "k_sh", "v_sb", "v_sl", "v_sh", "o_sb", "o_sl", "o_sh", "mask_sb")] +
-                [(n, c_int32) for n in ("dtype", "B", "Lq", "Lk", "H", "Hkv", "D", "splits", "pack")] + [("scale", c_float), ("rel", RelBias)])
+                [(n, c_int32) for n in ("dtype", "B", "Lq", "Lk", "H", "Hkv", "D", "splits", "pack", "pair")] + [("scale", c_float), ("rel", RelBias)])
 
 
 class AttnGrad(ctypes.Structure):
     _fields_ = [("d_o", c_void_p), ("do_sb", c_int64), ("do_sl", c_int64), ("do_sh", c_int64), ("dq", c_void_p), ("dk", c_void_p),
-                ("dv", c_void_p), ("delta", c_void_p), ("dtable", c_void_p), ("ws", c_void_p), ("splits_q", c_int32), ("splits_k", c_int32)]
+                ("dv", c_void_p), ("delta", c_void_p), ("dtable", c_void_p), ("ws", c_void_p), ("splits_q", c_int32), ("splits_k", c_int32), ("pair_q", c_int32), ("pair_k", c_int32)]
 
 
 class RopePart(ctypes.Structure):
@@ -63,8 +63,8 @@ class RopeDesc(ctypes.Structure):
 
 
 _REL = struct.Struct(f"@2P4i{2 * REL_FAR}s")
-_ATTN = struct.Struct("@8P13q9if")
-_GRAD = struct.Struct("@P3q6P2i")
+_ATTN = struct.Struct("@8P13q10if4x")
+_GRAD = struct.Struct("@P3q6P4i")
 _PART = struct.Struct("@6P7q2i")
 _ROPE = struct.Struct("@Pdf5i")
 _NO_REL = bytes(_REL.size)
@@ -427,32 +427,40 @@ def _parts(groups, units, n_cu, join, alone=False):
     return best
 
 
+def _pair(workgroups, n_cu):
+    """two waves per 32 rows (keys) where a launch would otherwise leave a SIMD with a single wave"""
+    return int(workgroups <= n_cu)
+
+
 @functools.lru_cache(maxsize=4096)
 def _attn_plan(B, Lq, Lk, H, Hkv, rel_width, n_cu):
-    """(pack, splits) of the forward.  pack: the query heads of a group share tiles if that at least halves the number of row blocks
+    """(pack, splits, pair) of the forward.  pack: the query heads of a group share tiles if that at least halves the number of row blocks
     (their bias rows have to fit 32 KB of LDS); K and V are then read once per group."""
     G = H // Hkv
     blocks, packed = -(-Lq // ROWS) * G, -(-(Lq * G) // ROWS)
     pack = G if 2 * packed <= blocks and G * rel_width * 4 <= 32768 else 1
-    return pack, _parts(B * (H // pack) * -(-(Lq * pack) // ROWS), -(-Lk // TILE), n_cu, 5)
+    groups = B * (H // pack) * -(-(Lq * pack) // ROWS)
+    parts = _parts(groups, -(-Lk // TILE), n_cu, 5)
+    return pack, parts, _pair(groups * parts, n_cu)
 
 
 @functools.lru_cache(maxsize=4096)
 def _grad_plan(B, Lq, Lk, H, Hkv, D, num_buckets, n_cu):
-    """(splits_q, splits_k, floats of delta, floats of delta and workspace) of the backward"""
+    """(splits_q, splits_k, pair_q, pair_k, floats of delta, floats of delta and workspace) of the backward"""
     nrb, nkb = -(-Lq // ROWS), -(-Lk // ROWS)
     splits_q = _parts(B * H * nrb, -(-Lk // TILE), n_cu, 6)
     splits_k = _parts(B * Hkv * nkb, (H // Hkv) * -(-Lq // TILE), n_cu, 6, alone=D > 64)
     delta = (B * H * Lq * (1 + splits_q if splits_q > 1 else 1) + 3) // 4 * 4
     ws = (splits_q * B * Lq * H * D if splits_q > 1 else 0) + (2 * splits_k * B * Lk * Hkv * D if splits_k > 1 else 0)
-    return splits_q, splits_k, delta, delta + ws + splits_k * B * H * nkb * num_buckets
+    return (splits_q, splits_k, _pair(B * H * nrb * splits_q, n_cu), _pair(B * Hkv * nkb * splits_k, n_cu), delta,
+            delta + ws + splits_k * B * H * nkb * num_buckets)
 
 
-def _attn_desc(q, k, v, o, lse, ws, key_mask, kv_lens, rel, scale, pack=1, splits=1):
+def _attn_desc(q, k, v, o, lse, ws, key_mask, kv_lens, rel, scale, pack=1, splits=1, pair=0):
     B, Lq, H, D = q.shape
     mask_sb = 0 if key_mask is None or B == 1 else key_mask.stride(0)
     return _ATTN.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), o.data_ptr(), _addr(lse), _addr(ws), _addr(key_mask), _addr(kv_lens), *_strides(q),
-                      *_strides(k), *_strides(v), *_strides(o), mask_sb, DTYPES[q.dtype], B, Lq, k.shape[1], H, k.shape[2], D, splits, pack, scale) + rel
+                      *_strides(k), *_strides(v), *_strides(o), mask_sb, DTYPES[q.dtype], B, Lq, k.shape[1], H, k.shape[2], D, splits, pack, pair, scale) + rel
 
 
 def _attn_forward(train, q, k, v, table, key_mask, kv_lens, q_offsets, q_offset, max_distance, bidirectional, scale):
@@ -471,9 +479,9 @@ def _attn_forward(train, q, k, v, table, key_mask, kv_lens, q_offsets, q_offset,
             nb = table.shape[0]
             rel = _rel_desc(table, nb, max_distance, bidirectional, q_offset, q_offsets)
             width = 2 * _reach(nb, max_distance, bidirectional) + 1
-        pack, splits = _attn_plan(B, Lq, Lk, H, Hkv, width, ops.cu_count(dev))
+        pack, splits, pair = _attn_plan(B, Lq, Lk, H, Hkv, width, ops.cu_count(dev))
         ws = torch.empty(splits * B * H * Lq * (D + 1), dtype=F32, device=dev) if splits > 1 else None
-        _call("dfold_seq_attn_fwd", _attn_desc(q, k, v, o, lse, ws, key_mask, kv_lens, rel, scale, pack, splits), t=q)
+        _call("dfold_seq_attn_fwd", _attn_desc(q, k, v, o, lse, ws, key_mask, kv_lens, rel, scale, pack, splits, pair), t=q)
     return o, (q, k, v, table, key_mask, kv_lens, q_offsets, o, lse)
 
 
@@ -504,11 +512,11 @@ class CrossAttentionFn(Function):
             if table is not None:
                 dtable, nb = torch.empty_like(table), table.shape[0]
                 rel = _rel_desc(table, nb, max_distance, bidirectional, q_offset, q_offsets)
-            splits_q, splits_k, n_delta, n = _grad_plan(B, Lq, Lk, H, Hkv, D, nb, ops.cu_count(q.device))
+            splits_q, splits_k, pair_q, pair_k, n_delta, n = _grad_plan(B, Lq, Lk, H, Hkv, D, nb, ops.cu_count(q.device))
             ws = torch.empty(n, dtype=F32, device=q.device)          # delta, then the workspace
             delta = ws.data_ptr()
             grad = _GRAD.pack(g.data_ptr(), *_strides(g), dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), delta, _addr(dtable), delta + 4 * n_delta,
-                              splits_q, splits_k)
+                              splits_q, splits_k, pair_q, pair_k)
             _call("dfold_seq_attn_bwd", _attn_desc(q, k, v, o, lse, None, key_mask, kv_lens, rel, scale), grad, t=q)
         need = ctx.needs_input_grad
         return (dq if need[0] else None, dk if need[1] else None, dv if need[2] else None, dtable if need[3] else None) + (None,) * 7

@@ -639,7 +639,8 @@ int dfold_relpos_ws(int32_t H, int32_t Lq, int32_t num_buckets);
  * are never used (they may hold NaN); a row without any key gives zeros.
  *   lse [B][H][Lq] fp32 (optional): log2 of the row's sum of exp2 (logits x log2 e); +inf for a row without keys.
  *   splits > 1: the keys are cut into that many parts; ws: splits * B * H * Lq * (D + 1) floats.
- *   pack = 1, or H / Hkv (rows of the query heads of a group share tiles: few queries). */
+ *   pack = 1, or H / Hkv (rows of the query heads of a group share tiles: few queries).
+ *   pair = 1: two waves per 32 rows, one per half of a key tile (launches that leave SIMDs idle); 0: one.  Any value is right. */
 typedef struct {
   const void *q, *k, *v;
   void* o;
@@ -647,16 +648,16 @@ typedef struct {
   const uint8_t* key_mask;
   const int32_t* kv_lens;
   int64_t q_sb, q_sl, q_sh, k_sb, k_sl, k_sh, v_sb, v_sl, v_sh, o_sb, o_sl, o_sh, mask_sb;
-  int32_t dtype, B, Lq, Lk, H, Hkv, D, splits, pack;
+  int32_t dtype, B, Lq, Lk, H, Hkv, D, splits, pack, pair;
   float scale;
   dfold_rel_bias rel;
 } dfold_seq_attn_desc;
 int dfold_seq_attn_fwd(const dfold_seq_attn_desc* desc, void* stream);
 
-/* Backward (Lk >= 1).  fwd: the descriptor of the forward call (o, lse as written there; splits, pack, ws unused).  d_o like o (strides
+/* Backward (Lk >= 1).  fwd: the descriptor of the forward call (o, lse as written there; splits, pack, pair, ws unused).  d_o like o (strides
  * do_*); dq [B][Lq][H][D], dk, dv [B][Lk][Hkv][D] dense (every element is written; masked keys get zeros).  delta [B][H][Lq] fp32
  * scratch (1 + splits_q planes of it if splits_q > 1).  dtable [num_buckets][H] fp32 (NULL without bias).  splits_q / splits_k: parts of the key axis in the dQ pass / of the
- * (head of group, query) axis in the dK, dV pass.  ws, floats: (splits_q > 1: splits_q B Lq H D) + (splits_k > 1: 2 splits_k B Lk
+ * (head of group, query) axis in the dK, dV pass; pair_q / pair_k: two waves per 32 rows / 32 keys.  ws, floats: (splits_q > 1: splits_q B Lq H D) + (splits_k > 1: 2 splits_k B Lk
  * Hkv D) + (bias: splits_k B H ceil(Lk / 128) num_buckets), the three parts each rounded up to a multiple of 4.  No atomics on
  * global memory: deterministic. */
 typedef struct {
@@ -664,7 +665,7 @@ typedef struct {
   int64_t do_sb, do_sl, do_sh;
   void *dq, *dk, *dv;
   float *delta, *dtable, *ws;
-  int32_t splits_q, splits_k;
+  int32_t splits_q, splits_k, pair_q, pair_k;
 } dfold_seq_attn_grad;
 int dfold_seq_attn_bwd(const dfold_seq_attn_desc* fwd, const dfold_seq_attn_grad* grad, void* stream);
 

@@ -98,15 +98,15 @@ def test_module_refuses():
 
 def test_launch_plans():
     # a token over a long cache: the group's heads share tiles, the keys are cut; a long prompt: neither
-    pack, parts = S._attn_plan(16, 1, 16384, 32, 8, 0, 256)
-    assert pack == 4 and parts > 1
-    assert S._attn_plan(2, 8192, 8192, 16, 16, 0, 256) == (1, 1)
-    assert S._attn_plan(1, 1, 1, 8, 8, 0, 256) == (1, 1) and S._attn_plan(1, 4, 0, 8, 8, 0, 256) == (1, 1)
+    pack, parts, pair = S._attn_plan(16, 1, 16384, 32, 8, 0, 256)
+    assert pack == 4 and parts > 1 and not pair
+    assert S._attn_plan(2, 8192, 8192, 16, 16, 0, 256) == (1, 1, 0)
+    assert S._attn_plan(1, 1, 1, 8, 8, 0, 256) == (1, 1, 1) and S._attn_plan(1, 4, 0, 8, 8, 0, 256) == (1, 1, 1)
     # bias rows of a group that do not fit: the heads stay apart
     assert S._attn_plan(1, 1, 64, 32, 1, 2049, 256)[0] == 1
     # no part without a tile of its own
     for B, Lq, Lk, H, Hkv in ((1, 1, 100, 1, 1), (1, 17, 6001, 16, 4), (3, 200, 999, 8, 8), (1, 1, 1 << 20, 1, 1)):
-        pack, s = S._attn_plan(B, Lq, Lk, H, Hkv, 0, 256)
+        pack, s, _ = S._attn_plan(B, Lq, Lk, H, Hkv, 0, 256)
         nt = -(-Lk // 64)
         assert 1 <= s <= nt and s <= 1024
 
@@ -118,10 +118,10 @@ def rel_of(table, dist, both):
 def test_packed_descriptors_have_the_layout_of_the_structures():
     assert S._REL.size == sizeof(S.RelBias) and S._ATTN.size + S._REL.size == sizeof(S.AttnDesc) and S._GRAD.size == sizeof(S.AttnGrad)
     assert S._PART.size == sizeof(S.RopePart) and 2 * S._PART.size + S._ROPE.size == sizeof(S.RopeDesc)
-    d = S.AttnDesc.from_buffer_copy(S._ATTN.pack(*range(1, 31), 0.5) + S._NO_REL)
-    assert [getattr(d, n) for n, _ in S.AttnDesc._fields_[:30]] == list(range(1, 31)) and d.scale == 0.5
-    g = S.AttnGrad.from_buffer_copy(S._GRAD.pack(*range(1, 13)))
-    assert [getattr(g, n) for n, _ in S.AttnGrad._fields_] == list(range(1, 13))
+    d = S.AttnDesc.from_buffer_copy(S._ATTN.pack(*range(1, 32), 0.5) + S._NO_REL)
+    assert [getattr(d, n) for n, _ in S.AttnDesc._fields_[:31]] == list(range(1, 32)) and d.scale == 0.5
+    g = S.AttnGrad.from_buffer_copy(S._GRAD.pack(*range(1, 15)))
+    assert [getattr(g, n) for n, _ in S.AttnGrad._fields_] == list(range(1, 15))
     r = S.RopeDesc.from_buffer_copy(S._PART.pack(*range(1, 16)) + S._PART.pack(*range(21, 36)) + S._ROPE.pack(51, 2.5, 0.25, *range(52, 57)))
     assert [getattr(r.part[1], n) for n, _ in S.RopePart._fields_] == list(range(21, 36))
     assert [getattr(r, n) for n, _ in S.RopeDesc._fields_[1:]] == [51, 2.5, 0.25, 52, 53, 54, 55, 56]

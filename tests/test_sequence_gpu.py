@@ -328,10 +328,11 @@ def test_attention_split_keys_equal_whole(D):
     table = torch.randn(32, H, device=DEV)
     ref = reference(q, k, v, g, live, None, None, D ** -0.5)
     with_table = reference(q, k, v, g, live, table, bucket_matrix(Lq, Lk, 32, 128, True, 0), D ** -0.5)
-    plan = S._parts
+    plan, pair = S._parts, S._pair
     try:
         for parts in (1, 2, 3, 7, 15, 40):
             S._parts = lambda *a, n=parts, **kw: n
+            S._pair = lambda *a, n=parts: n % 2              # both forms of the kernels at every size
             S._attn_plan.cache_clear(), S._grad_plan.cache_clear()
             got = run(q, k, v, g, **kw)
             for n in ref:
@@ -340,7 +341,7 @@ def test_attention_split_keys_equal_whole(D):
             for n in with_table:
                 within(f"{n} with bias in {parts} parts", got[n], with_table[n])
     finally:
-        S._parts = plan
+        S._parts, S._pair = plan, pair
         S._attn_plan.cache_clear(), S._grad_plan.cache_clear()
 
 
