@@ -157,7 +157,15 @@ struct SaDma {
 };
 // The two tiles of a step side by side in LDS (K and V, or Q and dO).  One group of four waves: each loads its share of both; two
 // groups: the first loads one, the second the other.
-#define SA_PAIR_LDS (SA_WAVES * 64 * 8)        // what pairs exchange beside the tiles' memory: two floats per lane
+#define SA_MASKS 64                    // tiles whose key masks wait in LDS
+// Stages of the K, V walk: two where two workgroups share a CU's LDS and cover for each other; a launch of one workgroup per CU (pairs)
+// waits for every tile's way through the caches unless more are in flight.
+template <int DP, bool PAIR>
+struct SaKvCfg {
+  static constexpr int NST = PAIR ? (DP == 128 ? 3 : 4) : 2;
+  static constexpr int TILES = NST * 2 * SaTile<DP>::BYTES;
+  static constexpr int LDS = TILES + SA_MASKS * 8 + (PAIR ? SA_WAVES * 64 * 8 : 0);      // tiles, mask words, what pairs exchange; then the bias
+};
 template <int DP, bool PAIR>
 struct SaKvTiles {
   using T = SaTile<DP>;
@@ -167,6 +175,7 @@ struct SaKvTiles {
   __device__ __forceinline__ SaKvTiles(const char* pa, long rsa, const char* pb, long rsb, int D, int t, int wave)
       : a(PAIR && wave >= SA_WAVES ? pb : pa), b(pb), la(PAIR && wave >= SA_WAVES ? rsb : rsa, D, t & (64 * SA_WAVES - 1)), lb(rsb, D, t & (64 * SA_WAVES - 1)),
         tid(t & (64 * SA_WAVES - 1)), w(wave & (SA_WAVES - 1)), half(wave / SA_WAVES) {}
+  static constexpr int LOADS = (PAIR ? 1 : 2) * SaDma<DP>::NCH;      // instructions per wave
   __device__ __forceinline__ void load(int row0, int end, char* tile) const { load(a, b, row0, end, tile); }
   // the same from other bases (sa, sb: this wave's first, and for one group its second matrix)
   __device__ __forceinline__ void load(const char* sa, const char* sb, int row0, int end, char* tile) const {
@@ -178,14 +187,72 @@ struct SaKvTiles {
     if constexpr (!PAIR) lb.zero(live, tile + T::BYTES, tid);
   }
 };
-// every DMA of this wave has landed, then everybody's
+// All but this wave's youngest N loads have landed, then everybody's; LDS accesses in front are done.  (Anything else the wave has in
+// flight only makes the wait stricter.)  Not __syncthreads(): that would wait for the younger ones too.
+template <int N>
 __device__ __forceinline__ void sa_landed() {
-  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-  __syncthreads();
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+// a barrier for LDS accesses only
+__device__ __forceinline__ void sa_lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
 }
 template <int I>
 struct SaInt {
   static constexpr int value = I;
+};
+// The walk over tiles n0 .. n1 through NST stages of LDS, NST - 1 tiles ahead: load(n, stage) issues LOADS loads per wave, work(n, stage)
+// runs when tile n has landed for everybody.  The stage of tile n is n - n0 modulo NST, a constant inside work.
+template <int NST, int LOADS, typename L, typename W>
+__device__ __forceinline__ void sa_walk(int n0, int n1, L load, W work) {
+#pragma unroll
+  for (int i = 0; i < NST - 1; ++i)
+    if (n0 + i < n1) load(n0 + i, i);
+  auto one = [&](int n, auto stage) {
+    constexpr int S = decltype(stage)::value;
+    if (n + NST - 2 < n1) sa_landed<(NST - 2) * LOADS>();
+    else sa_landed<0>();                              // (the last tiles: fewer are in flight)
+    if (n + NST - 1 < n1) load(n + NST - 1, (S + NST - 1) % NST);      // into the stage of tile n - 1: everybody is done with it
+    work(n, stage);
+  };
+  for (int n = n0; n < n1; n += NST) {
+    one(n, SaInt<0>());
+    if (n + 1 < n1) one(n + 1, SaInt<1>());
+    if constexpr (NST > 2)
+      if (n + 2 < n1) one(n + 2, SaInt<2>());
+    if constexpr (NST > 3)
+      if (n + 3 < n1) one(n + 3, SaInt<3>());
+  }
+}
+// Which keys of a tile exist, one bit per key.  Without a key mask that is arithmetic; with one, the words of SA_MASKS tiles at a time are
+// formed by all waves (a byte per lane, a ballot per tile) and wait in LDS.
+template <int NW>
+struct SaLive {
+  const uint8_t* mask;
+  int end, t0, t1, w, lane;
+  unsigned long* lds;
+  // (every wave calls it for every tile in order, behind the tile's barrier)
+  __device__ __forceinline__ unsigned long tile(int t) const {
+    if (!mask) {
+      const int n = end - t * SA_KT;
+      return n >= SA_KT ? ~0ul : (1ul << n) - 1;
+    }
+    const int i = (t - t0) & (SA_MASKS - 1);
+    if (i == 0) {
+      for (int k = w; k < SA_MASKS && t + k < t1; k += NW) {
+        const int key = (t + k) * SA_KT + lane;
+        const unsigned long live = __ballot(key < end && mask[min(key, end - 1)] != 0);
+        if (lane == 0) lds[k] = live;
+      }
+      sa_lds_barrier();
+    }
+    const unsigned long v = lds[i];
+    return ((unsigned long)(unsigned)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32) | (unsigned)__builtin_amdgcn_readfirstlane((int)v);
+  }
 };
 
 // ---- bucketed relative position bias ----

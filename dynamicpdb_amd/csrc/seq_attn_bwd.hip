@@ -61,7 +61,8 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_dq
   using T = SaTile<DP>;
   constexpr int KS = T::KS, NT = T::NT, NW = PAIR ? 2 * SA_WAVES : SA_WAVES, NB = PAIR ? 1 : 2;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  float* const ldsB = (float*)(smem + 4 * T::BYTES + (PAIR ? SA_PAIR_LDS : 0));
+  using C = SaKvCfg<DP, PAIR>;
+  float* const ldsB = (float*)(smem + C::LDS);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l31 = lane & 31, h = lane >> 5;
   unsigned id = sa_work_id();
@@ -130,22 +131,16 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_dq
   float left = 0.f;          // row sum of dS
   const SaAddr<DP> ad(lane, half * 32);
   const SaKvTiles<DP, PAIR> kv(kb_, p.k_sl, vb_, p.v_sl, p.D, tid, w);
-  int kmask = 0;
-  auto fetch = [&](int t, char* tile) {
-    kv.load(t * SA_KT, kv_end, tile);
-    const int key = t * SA_KT + lane;
-    kmask = key < kv_end ? (mb_ ? mb_[key] : 1) : 0;
-  };
+  const SaLive<NW> keys{mb_, kv_end, t0, t1, w, lane, (unsigned long*)(smem + C::TILES)};
+  auto fetch = [&](int t, int stage) { kv.load(t * SA_KT, kv_end, smem + stage * 2 * T::BYTES); };
   auto step = [&](int t, auto stage) {
     char* const lk = smem + decltype(stage)::value * 2 * T::BYTES;
     char* const lv = lk + T::BYTES;
-    sa_landed();
-    const unsigned long live = __ballot(kmask != 0);
-    if (t + 1 < t1) fetch(t + 1, smem + (1 - decltype(stage)::value) * 2 * T::BYTES);
+    const unsigned long live = keys.tile(t);
     if (live != ~0ul) {
       if (live == 0) return;
       kv.zero(live, lk);
-      __syncthreads();
+      sa_lds_barrier();
     }
     if (!wave_on) return;
 #pragma unroll
@@ -182,15 +177,11 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_dq
       }
     }
   };
-  if (t0 < t1) fetch(t0, smem);
-  for (int t = t0; t < t1; t += 2) {
-    step(t, SaInt<0>());
-    if (t + 1 < t1) step(t + 1, SaInt<1>());
-  }
+  sa_walk<C::NST, SaKvTiles<DP, PAIR>::LOADS>(t0, t1, fetch, step);
 
   left = sa_xsum(left);
   if constexpr (PAIR) {
-    float* const ls = (float*)(smem + 4 * T::BYTES) + wr * 64 + lane;
+    float* const ls = (float*)(smem + C::TILES + SA_MASKS * 8) + wr * 64 + lane;
     f32x16* const acc = (f32x16*)smem + wr * NT * 64 + lane;
     __syncthreads();
     if (half) {
@@ -239,7 +230,9 @@ template <int DP, bool REL, bool PAIR>
 struct SaDkvCfg {
   static constexpr bool VLDS = PAIR && DP == 128;
   static constexpr int WAVES = PAIR ? 2 * SA_WAVES : SA_WAVES;
-  static constexpr int LDS = 4 * SaTile<DP>::BYTES + 4 * SA_KT * 4 + (VLDS ? SA_ROWS * SaTile<DP>::PITCH : 0);
+  static constexpr int NST = PAIR ? (DP == 128 || REL ? 3 : 4) : 2;
+  static constexpr int TILES = NST * 2 * SaTile<DP>::BYTES, ROWS = NST * 2 * SA_KT * 4;      // tiles; log-sums and deltas of their rows
+  static constexpr int LDS = TILES + ROWS + (VLDS ? SA_ROWS * SaTile<DP>::PITCH : 0);
   static int bytes(int W) { return LDS + (REL ? (2 * W + 1 + WAVES * (2 * (W + SA_REACH) + 1 + SA_DIAG)) * 4 : 0); }
 };
 template <int DT, int DP, bool REL, bool PAIR>
@@ -249,9 +242,10 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, (DP == 128 && REL ?
   constexpr bool VLDS = SaDkvCfg<DP, REL, PAIR>::VLDS;
   constexpr int NW = SaDkvCfg<DP, REL, PAIR>::WAVES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  float* const ldsL = (float*)(smem + 4 * T::BYTES);            // [stage][log-sum | delta][SA_KT]
-  char* const ldsV = smem + 4 * T::BYTES + 4 * SA_KT * 4;
-  float* const ldsB = ldsL + 4 * SA_KT;
+  using C = SaDkvCfg<DP, REL, PAIR>;
+  float* const ldsL = (float*)(smem + C::TILES);                // [stage][log-sum | delta][SA_KT]
+  char* const ldsV = smem + C::TILES + C::ROWS;
+  float* const ldsB = (float*)(smem + C::LDS);
   float* const ldsH = ldsB + (REL ? 2 * p.rel.W + 1 : 0);       // [wave][distance]
   const int hn = REL ? 2 * (p.rel.W + SA_REACH) + 1 : 0;
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -337,22 +331,20 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, (DP == 128 && REL ?
   const SaAddr<DP> ad(lane, half * 32);
   const SaKvTiles<DP, PAIR> qg(p.q, p.q_sl, p.d_o, p.do_sl, p.D, tid, w);
   const char* const lv = ldsV + (wk - half) * 32 * T::PITCH;
-  float lse_r = 0.f, del_r = 0.f;
   // position in the walk of the unit that is fetched next, and of the one that is worked on
   int fg = u0 / nqt, fq = (u0 - fg * nqt) * SA_KT, wg = fg, wq = fq;
-  auto fetch = [&](char* tile) {
+  auto fetch = [&](int, int stage) {
     const int head = hkv * G + fg;
     const long oq = ((long)b * p.q_sb + (long)head * p.q_sh) * 2, og = ((long)b * p.do_sb + (long)head * p.do_sh) * 2;
-    qg.load(qg.a + (half ? og : oq), qg.b + og, fq, p.Lq, tile);
-    if (tid < SA_KT) {
-      const int qi = fq + tid;
-      const long r = ((long)b * p.H + head) * p.Lq + qi;
-      lse_r = qi < p.Lq ? -p.lse[r] : -INFINITY;       // rows past the end: P = 0
-      del_r = qi < p.Lq ? p.delta[r] : 0.f;
-    }
+    qg.load(qg.a + (half ? og : oq), qg.b + og, fq, p.Lq, smem + stage * 2 * T::BYTES);
+    // the rows' log-sums and deltas, a lane each; every wave writes the same numbers (all waves then count the same loads)
+    const long r = ((long)b * p.H + head) * p.Lq + min(fq + lane, p.Lq - 1);
+    float* const ll = ldsL + stage * 2 * SA_KT;
+    __builtin_amdgcn_global_load_lds((const void*)(p.lse + r), (sa_lds_ptr)ll, 4, 0, 0);
+    __builtin_amdgcn_global_load_lds((const void*)(p.delta + r), (sa_lds_ptr)(ll + SA_KT), 4, 0, 0);
     if ((fq += SA_KT) >= p.Lq) { fq = 0; ++fg; }
   };
-  auto step = [&](bool more, auto stage) {
+  auto step = [&](int, auto stage) {
     char* const lq = smem + decltype(stage)::value * 2 * T::BYTES;
     char* const lg = lq + T::BYTES;
     float* const ll = ldsL + decltype(stage)::value * 2 * SA_KT;
@@ -364,15 +356,14 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, (DP == 128 && REL ?
         for (int i = tid; i < NW * hn; i += 64 * NW) ldsH[i] = 0.f;
         sa_fill_bias<NW>(ldsB, p.rel, head, 1, tid);
         head_in = head;
+        sa_lds_barrier();
       }
     }
     if ((wq += SA_KT) >= p.Lq) { wq = 0; ++wg; }
-    if (tid < SA_KT) {
-      ll[tid] = lse_r;
-      ll[SA_KT + tid] = del_r;
+    if (q0 + SA_KT > p.Lq) {       // rows past the end repeat the last one: P = 0 for them
+      if (tid < SA_KT && q0 + tid >= p.Lq) ll[tid] = INFINITY;
+      sa_lds_barrier();
     }
-    sa_landed();
-    if (more) fetch(smem + (1 - decltype(stage)::value) * 2 * T::BYTES);
     if (!wave_on) return;
 #pragma unroll
     for (int qb = 0; qb < (PAIR ? 1 : 2); ++qb) {
@@ -408,7 +399,7 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, (DP == 128 && REL ?
           const int r = g * 4 + e;
           // a masked key's column holds products with zeros: whatever comes of them stays in that column, which is not stored (only the
           // bias gradient sums over columns)
-          const float x = sa_exp2(REL ? s[r] + rl[e] : __builtin_fmaf(s[r], p.sl2, rl[e]));
+          const float x = sa_exp2(REL ? s[r] - rl[e] : __builtin_fmaf(s[r], p.sl2, -rl[e]));
           s[r] = REL ? (key_on ? x : 0.f) : x;
           dp[r] = s[r] * (dp[r] - rd[e]);
         }
@@ -452,11 +443,7 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, (DP == 128 && REL ?
       }
     }
   };
-  if (u0 < u1) fetch(smem);
-  for (int u = u0; u < u1; u += 2) {
-    step(u + 1 < u1, SaInt<0>());
-    if (u + 1 < u1) step(u + 2 < u1, SaInt<1>());
-  }
+  sa_walk<C::NST, SaKvTiles<DP, PAIR>::LOADS + 2>(u0, u1, fetch, step);
 
   if constexpr (REL)
     if (head_in >= 0) flush(head_in);
@@ -533,7 +520,7 @@ static int sa_launch_bwd(K kernel, const SaBwdParams& p, long nwg, int waves, in
 template <int DT, int DP, bool REL, bool PAIR>
 static int sa_dq(const SaBwdParams& p, hipStream_t st) {
   struct Mine;
-  const int lds = 4 * SaTile<DP>::BYTES + (PAIR ? SA_PAIR_LDS : 0) + (REL ? (2 * p.rel.W + 1) * 4 : 0);
+  const int lds = SaKvCfg<DP, PAIR>::LDS + (REL ? (2 * p.rel.W + 1) * 4 : 0);
   return sa_launch_bwd<Mine>(seq_attn_dq_kernel<DT, DP, REL, PAIR>, p, (long)p.nrb * p.splits_q * p.H * p.B, PAIR ? 2 * SA_WAVES : SA_WAVES, lds, st);
 }
 template <int DT, int DP, bool REL, bool PAIR>

@@ -3,8 +3,8 @@
 //
 // A workgroup owns 128 softmax rows of one key head (4 waves x 32 rows; with pack > 1 the rows of the query heads of a group are
 // interleaved, head fastest, so that one token of a grouped layer fills its tile), walks its part of the keys in tiles of 64 and
-// keeps S, P and O in registers; K and V tiles go to LDS by DMA one tile ahead of the arithmetic, two stages, one barrier per tile.
-// Key masks are one ballot per tile: an empty tile is skipped, a full one takes no mask arithmetic, K / V rows of masked keys are
+// keeps S, P and O in registers; K and V tiles go to LDS by DMA ahead of the arithmetic, one barrier per tile.  Key masks are one
+// word per tile: an empty tile is skipped, a full one takes no mask arithmetic, K / V rows of masked keys are
 // zeroed in LDS behind one more barrier (0 * NaN would not stay 0).
 // Few rows and many keys: the key axis is cut over workgroups (splits), partial results meet in seq_attn_combine_kernel in split
 // order (deterministic).
@@ -35,7 +35,8 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_fw
   using T = SaTile<DP>;
   constexpr int KS = T::KS, NT = T::NT, NW = PAIR ? 2 * SA_WAVES : SA_WAVES, NB = PAIR ? 1 : 2;      // NB: 32-key blocks of a wave
   extern __shared__ __attribute__((aligned(16))) char smem[];
-  float* const ldsB = (float*)(smem + 4 * T::BYTES + (PAIR ? SA_PAIR_LDS : 0));
+  using C = SaKvCfg<DP, PAIR>;
+  float* const ldsB = (float*)(smem + C::LDS);
   const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l31 = lane & 31, h = lane >> 5;
   unsigned id = sa_work_id();
@@ -99,22 +100,16 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_fw
 
   const SaAddr<DP> ad(lane, half * 32);
   const SaKvTiles<DP, PAIR> kv(kb_, p.k_sl, vb_, p.v_sl, p.D, tid, w);
-  int kmask = 0;
-  auto fetch = [&](int t, char* tile) {
-    kv.load(t * SA_KT, kv_end, tile);
-    const int key = t * SA_KT + lane;
-    kmask = key < kv_end ? (mb_ ? mb_[key] : 1) : 0;
-  };
+  const SaLive<NW> keys{mb_, kv_end, t0, t1, w, lane, (unsigned long*)(smem + C::TILES)};
+  auto fetch = [&](int t, int stage) { kv.load(t * SA_KT, kv_end, smem + stage * 2 * T::BYTES); };
   auto step = [&](int t, auto stage) {
     char* const lk = smem + decltype(stage)::value * 2 * T::BYTES;
     char* const lv = lk + T::BYTES;
-    sa_landed();
-    const unsigned long live = __ballot(kmask != 0);
-    if (t + 1 < t1) fetch(t + 1, smem + (1 - decltype(stage)::value) * 2 * T::BYTES);
+    const unsigned long live = keys.tile(t);
     if (live != ~0ul) {
       if (live == 0) return;
       kv.zero(live, lk);
-      __syncthreads();
+      sa_lds_barrier();
     }
     if (!wave_on) return;
 
@@ -188,16 +183,12 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_fw
 #pragma unroll
       for (int i = 0; i < NT; ++i) O[i] = sa_mfma<DT>(ad.cols(lv, c * 16, i), pf[c], O[i]);
   };
-  if (t0 < t1) fetch(t0, smem);
-  for (int t = t0; t < t1; t += 2) {
-    step(t, SaInt<0>());
-    if (t + 1 < t1) step(t + 1, SaInt<1>());
-  }
+  sa_walk<C::NST, SaKvTiles<DP, PAIR>::LOADS>(t0, t1, fetch, step);
 
   l = sa_xsum(l);
   if constexpr (PAIR) {
     // the second wave of a pair hands its maximum, sum and O over through the tiles' memory
-    float* const ml = (float*)(smem + 4 * T::BYTES) + (wr * 64 + lane) * 2;
+    float* const ml = (float*)(smem + C::TILES + SA_MASKS * 8) + (wr * 64 + lane) * 2;
     f32x16* const acc = (f32x16*)smem + wr * NT * 64 + lane;
     __syncthreads();
     if (half) {
@@ -331,7 +322,7 @@ __global__ __launch_bounds__(256) void seq_attn_combine_row_kernel(const SaFwdPa
 template <int DT, int DP, bool REL, bool PAIR>
 static int sa_launch_fwd(const SaFwdParams& p, unsigned nwg, hipStream_t st) {
   struct Mine;
-  const int lds = 4 * SaTile<DP>::BYTES + (PAIR ? SA_PAIR_LDS : 0) + (REL ? p.pack * (2 * p.rel.W + 1) * 4 : 0);
+  const int lds = SaKvCfg<DP, PAIR>::LDS + (REL ? p.pack * (2 * p.rel.W + 1) * 4 : 0);
   if (lds > SA_MAX_LDS) return DFOLD_EINVAL;
   if (!sa_raise_lds<Mine>(seq_attn_fwd_kernel<DT, DP, REL, PAIR>, lds)) return DFOLD_ELAUNCH;
   DFOLD_LAUNCH((seq_attn_fwd_kernel<DT, DP, REL, PAIR>), dim3(nwg), dim3((PAIR ? 2 : 1) * 64 * SA_WAVES), lds, st, p);

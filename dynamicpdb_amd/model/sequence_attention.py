@@ -427,9 +427,11 @@ def _parts(groups, units, n_cu, join, alone=False):
     return best
 
 
-def _pair(workgroups, n_cu):
-    """two waves per 32 rows (keys) where a launch would otherwise leave a SIMD with a single wave"""
-    return int(workgroups <= n_cu)
+def _pair(workgroups, tiles, n_cu):
+    """Two waves per 32 rows (keys) where a launch would otherwise leave SIMDs with a single wave and a workgroup walks enough tiles to pay
+    for the join.  One against two, us: D = 64, 64 workgroups of 64 tiles 67 / 52 (forward), 76 / 60 (dQ); 256 of 16 tiles 23.5 / 20.8,
+    29.0 / 26.2; D = 32, 256 of 8 tiles 10.1 / 10.2, 12.7 / 12.2; a token, 3 tiles 10.3 / 10.8."""
+    return int(workgroups <= n_cu and tiles >= 12)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -441,7 +443,7 @@ def _attn_plan(B, Lq, Lk, H, Hkv, rel_width, n_cu):
     pack = G if 2 * packed <= blocks and G * rel_width * 4 <= 32768 else 1
     groups = B * (H // pack) * -(-(Lq * pack) // ROWS)
     parts = _parts(groups, -(-Lk // TILE), n_cu, 5)
-    return pack, parts, _pair(groups * parts, n_cu)
+    return pack, parts, _pair(groups * parts, -(-Lk // TILE) // parts, n_cu)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -452,7 +454,8 @@ def _grad_plan(B, Lq, Lk, H, Hkv, D, num_buckets, n_cu):
     splits_k = _parts(B * Hkv * nkb, (H // Hkv) * -(-Lq // TILE), n_cu, 6, alone=D > 64)
     delta = (B * H * Lq * (1 + splits_q if splits_q > 1 else 1) + 3) // 4 * 4
     ws = (splits_q * B * Lq * H * D if splits_q > 1 else 0) + (2 * splits_k * B * Lk * Hkv * D if splits_k > 1 else 0)
-    return (splits_q, splits_k, _pair(B * H * nrb * splits_q, n_cu), _pair(B * Hkv * nkb * splits_k, n_cu), delta,
+    return (splits_q, splits_k, _pair(B * H * nrb * splits_q, -(-Lk // TILE) // splits_q, n_cu),
+            _pair(B * Hkv * nkb * splits_k, (H // Hkv) * -(-Lq // TILE) // splits_k, n_cu), delta,
             delta + ws + splits_k * B * H * nkb * num_buckets)
 
 

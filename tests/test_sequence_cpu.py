@@ -101,7 +101,9 @@ def test_launch_plans():
     pack, parts, pair = S._attn_plan(16, 1, 16384, 32, 8, 0, 256)
     assert pack == 4 and parts > 1 and not pair
     assert S._attn_plan(2, 8192, 8192, 16, 16, 0, 256) == (1, 1, 0)
-    assert S._attn_plan(1, 1, 1, 8, 8, 0, 256) == (1, 1, 1) and S._attn_plan(1, 4, 0, 8, 8, 0, 256) == (1, 1, 1)
+    assert S._attn_plan(1, 1, 1, 8, 8, 0, 256) == (1, 1, 0) and S._attn_plan(1, 4, 0, 8, 8, 0, 256) == (1, 1, 0)
+    # one workgroup per CU and many tiles: two waves per 32 rows
+    assert S._attn_plan(4, 1001, 1001, 8, 8, 0, 256) == (1, 1, 1)
     # bias rows of a group that do not fit: the heads stay apart
     assert S._attn_plan(1, 1, 64, 32, 1, 2049, 256)[0] == 1
     # no part without a tile of its own
