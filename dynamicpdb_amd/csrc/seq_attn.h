@@ -158,13 +158,11 @@ struct SaDma {
 // The two tiles of a step side by side in LDS (K and V, or Q and dO).  One group of four waves: each loads its share of both; two
 // groups: the first loads one, the second the other.
 #define SA_MASKS 64                    // tiles whose key masks wait in LDS
-// Stages of the K, V walk: two where two workgroups share a CU's LDS and cover for each other; a launch of one workgroup per CU (pairs)
-// waits for every tile's way through the caches unless more are in flight.
+// LDS of the K, V walk: two stages of two tiles, mask words, what pairs exchange; then the bias
 template <int DP, bool PAIR>
 struct SaKvCfg {
-  static constexpr int NST = PAIR ? (DP == 128 ? 3 : 4) : 2;
-  static constexpr int TILES = NST * 2 * SaTile<DP>::BYTES;
-  static constexpr int LDS = TILES + SA_MASKS * 8 + (PAIR ? SA_WAVES * 64 * 8 : 0);      // tiles, mask words, what pairs exchange; then the bias
+  static constexpr int TILES = 4 * SaTile<DP>::BYTES;
+  static constexpr int LDS = TILES + SA_MASKS * 8 + (PAIR ? SA_WAVES * 64 * 8 : 0);
 };
 template <int DP, bool PAIR>
 struct SaKvTiles {
@@ -175,7 +173,6 @@ struct SaKvTiles {
   __device__ __forceinline__ SaKvTiles(const char* pa, long rsa, const char* pb, long rsb, int D, int t, int wave)
       : a(PAIR && wave >= SA_WAVES ? pb : pa), b(pb), la(PAIR && wave >= SA_WAVES ? rsb : rsa, D, t & (64 * SA_WAVES - 1)), lb(rsb, D, t & (64 * SA_WAVES - 1)),
         tid(t & (64 * SA_WAVES - 1)), w(wave & (SA_WAVES - 1)), half(wave / SA_WAVES) {}
-  static constexpr int LOADS = (PAIR ? 1 : 2) * SaDma<DP>::NCH;      // instructions per wave
   __device__ __forceinline__ void load(int row0, int end, char* tile) const { load(a, b, row0, end, tile); }
   // the same from other bases (sa, sb: this wave's first, and for one group its second matrix)
   __device__ __forceinline__ void load(const char* sa, const char* sb, int row0, int end, char* tile) const {
@@ -187,11 +184,9 @@ struct SaKvTiles {
     if constexpr (!PAIR) lb.zero(live, tile + T::BYTES, tid);
   }
 };
-// All but this wave's youngest N loads have landed, then everybody's; LDS accesses in front are done.  (Anything else the wave has in
-// flight only makes the wait stricter.)  Not __syncthreads(): that would wait for the younger ones too.
-template <int N>
+// every DMA of this wave has landed and its LDS accesses are done, then everybody's
 __device__ __forceinline__ void sa_landed() {
-  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
@@ -205,27 +200,19 @@ template <int I>
 struct SaInt {
   static constexpr int value = I;
 };
-// The walk over tiles n0 .. n1 through NST stages of LDS, NST - 1 tiles ahead: load(n, stage) issues LOADS loads per wave, work(n, stage)
-// runs when tile n has landed for everybody.  The stage of tile n is n - n0 modulo NST, a constant inside work.
-template <int NST, int LOADS, typename L, typename W>
+// The walk over tiles n0 .. n1 through two stages of LDS, one tile ahead: load(n, stage) requests tile n, work(n, stage) runs when it has
+// landed for everybody, its stage a constant.  (Three and four stages, also for a single workgroup per CU: no gain at any size.)
+template <typename L, typename W>
 __device__ __forceinline__ void sa_walk(int n0, int n1, L load, W work) {
-#pragma unroll
-  for (int i = 0; i < NST - 1; ++i)
-    if (n0 + i < n1) load(n0 + i, i);
+  if (n0 < n1) load(n0, 0);
   auto one = [&](int n, auto stage) {
-    constexpr int S = decltype(stage)::value;
-    if (n + NST - 2 < n1) sa_landed<(NST - 2) * LOADS>();
-    else sa_landed<0>();                              // (the last tiles: fewer are in flight)
-    if (n + NST - 1 < n1) load(n + NST - 1, (S + NST - 1) % NST);      // into the stage of tile n - 1: everybody is done with it
+    sa_landed();
+    if (n + 1 < n1) load(n + 1, 1 - decltype(stage)::value);      // into the stage of tile n - 1: everybody is done with it
     work(n, stage);
   };
-  for (int n = n0; n < n1; n += NST) {
+  for (int n = n0; n < n1; n += 2) {
     one(n, SaInt<0>());
     if (n + 1 < n1) one(n + 1, SaInt<1>());
-    if constexpr (NST > 2)
-      if (n + 2 < n1) one(n + 2, SaInt<2>());
-    if constexpr (NST > 3)
-      if (n + 3 < n1) one(n + 3, SaInt<3>());
   }
 }
 // Which keys of a tile exist, one bit per key.  Without a key mask that is arithmetic; with one, the words of SA_MASKS tiles at a time are

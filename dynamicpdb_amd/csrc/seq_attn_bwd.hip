@@ -177,7 +177,7 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_dq
       }
     }
   };
-  sa_walk<C::NST, SaKvTiles<DP, PAIR>::LOADS>(t0, t1, fetch, step);
+  sa_walk(t0, t1, fetch, step);
 
   left = sa_xsum(left);
   if constexpr (PAIR) {
@@ -230,8 +230,7 @@ template <int DP, bool REL, bool PAIR>
 struct SaDkvCfg {
   static constexpr bool VLDS = PAIR && DP == 128;
   static constexpr int WAVES = PAIR ? 2 * SA_WAVES : SA_WAVES;
-  static constexpr int NST = PAIR ? (DP == 128 || REL ? 3 : 4) : 2;
-  static constexpr int TILES = NST * 2 * SaTile<DP>::BYTES, ROWS = NST * 2 * SA_KT * 4;      // tiles; log-sums and deltas of their rows
+  static constexpr int TILES = 4 * SaTile<DP>::BYTES, ROWS = 4 * SA_KT * 4;      // two stages of two tiles; log-sums and deltas of their rows
   static constexpr int LDS = TILES + ROWS + (VLDS ? SA_ROWS * SaTile<DP>::PITCH : 0);
   static int bytes(int W) { return LDS + (REL ? (2 * W + 1 + WAVES * (2 * (W + SA_REACH) + 1 + SA_DIAG)) * 4 : 0); }
 };
@@ -337,11 +336,11 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, (DP == 128 && REL ?
     const int head = hkv * G + fg;
     const long oq = ((long)b * p.q_sb + (long)head * p.q_sh) * 2, og = ((long)b * p.do_sb + (long)head * p.do_sh) * 2;
     qg.load(qg.a + (half ? og : oq), qg.b + og, fq, p.Lq, smem + stage * 2 * T::BYTES);
-    // the rows' log-sums and deltas, a lane each; every wave writes the same numbers (all waves then count the same loads)
+    // the rows' log-sums and deltas, a lane each
     const long r = ((long)b * p.H + head) * p.Lq + min(fq + lane, p.Lq - 1);
     float* const ll = ldsL + stage * 2 * SA_KT;
-    __builtin_amdgcn_global_load_lds((const void*)(p.lse + r), (sa_lds_ptr)ll, 4, 0, 0);
-    __builtin_amdgcn_global_load_lds((const void*)(p.delta + r), (sa_lds_ptr)(ll + SA_KT), 4, 0, 0);
+    if (w == 0) __builtin_amdgcn_global_load_lds((const void*)(p.lse + r), (sa_lds_ptr)ll, 4, 0, 0);
+    if (w == 1) __builtin_amdgcn_global_load_lds((const void*)(p.delta + r), (sa_lds_ptr)(ll + SA_KT), 4, 0, 0);
     if ((fq += SA_KT) >= p.Lq) { fq = 0; ++fg; }
   };
   auto step = [&](int, auto stage) {
@@ -443,7 +442,7 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, (DP == 128 && REL ?
       }
     }
   };
-  sa_walk<C::NST, SaKvTiles<DP, PAIR>::LOADS + 2>(u0, u1, fetch, step);
+  sa_walk(u0, u1, fetch, step);
 
   if constexpr (REL)
     if (head_in >= 0) flush(head_in);
