@@ -155,8 +155,6 @@ struct SaDma {
       if (!((live >> (row + i * STEP)) & 1)) *(sa_u32x4*)(tile + (i * 64 * NW + tid) * 16) = (sa_u32x4){0u, 0u, 0u, 0u};
   }
 };
-// The two tiles of a step side by side in LDS (K and V, or Q and dO).  One group of four waves: each loads its share of both; two
-// groups: the first loads one, the second the other.
 #define SA_MASKS 64                    // tiles whose key masks wait in LDS
 // LDS of the K, V walk: two stages of two tiles, mask words, what pairs exchange; then the bias
 template <int DP, bool PAIR>
@@ -164,6 +162,8 @@ struct SaKvCfg {
   static constexpr int TILES = 4 * SaTile<DP>::BYTES;
   static constexpr int LDS = TILES + SA_MASKS * 8 + (PAIR ? SA_WAVES * 64 * 8 : 0);
 };
+// The two tiles of a step side by side in LDS (K and V, or Q and dO).  One group of four waves: each loads its share of both; two
+// groups: the first loads one, the second the other.
 template <int DP, bool PAIR>
 struct SaKvTiles {
   using T = SaTile<DP>;

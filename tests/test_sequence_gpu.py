@@ -144,6 +144,10 @@ CASES = [
     (2, 7, 50, 8, 1, 24, BF, "none", (4, 2, True, 20)),
     (1, 513, 1025, 1, 1, 48, HF, "both", (48, 300, True, 0)),
     (1, 100, 100, 2, 2, 32, BF, "none", (32, 128, True, 100000)),
+    (1, 900, 1000, 2, 2, 64, BF, "keys", (64, 1024, True, 0)),
+    (1, 800, 850, 4, 2, 64, HF, "none", (48, 500, True, 30)),
+    (1, 900, 4500, 2, 1, 128, BF, "keys", None),
+    (1, 4300, 70, 1, 1, 40, BF, "keys", None),
 ]
 
 
