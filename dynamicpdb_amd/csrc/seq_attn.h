@@ -116,7 +116,7 @@ struct SaAddr {
 // SA_KT (or ROWS) rows of a [rows][D] matrix with row stride `rs` elements (< SA_MAX_ROW) into an LDS tile, by LDS-DMA: no registers and
 // no LDS write instructions.  A wave's instruction fills 1 KB of the tile in lane order, so the chunk permutation is applied to the
 // source.  Rows past the last one repeat it (never out of range; their content is masked by the caller), columns past D repeat
-// column 0 (they meet zeros of the other operand, or results that are not stored).
+// column 0: they meet zeros of the other operand, or results that are not stored, or zero_columns() clears them.
 #define SA_MAX_ROW (1 << 24)
 typedef __attribute__((address_space(3))) void* sa_lds_ptr;
 template <int DP, int NW = SA_WAVES, int ROWS = SA_KT>
@@ -147,6 +147,13 @@ struct SaDma {
       for (int i = 0; i < NCH; ++i)
         __builtin_amdgcn_global_load_lds((const void*)(src + (min(row + i * STEP, last) * rs2 + col)), (sa_lds_ptr)(tile + (i * NW + w) * 1024), 16, 0, 0);
     }
+  }
+  // columns past D of what this wave loaded become zeros (its loads have landed by then; a barrier before others read)
+  __device__ __forceinline__ void zero_columns(int D, char* tile, int tid) const {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if ((((tid % T::CPR) ^ T::key(row)) * 8) < D) return;
+#pragma unroll
+    for (int i = 0; i < NCH; ++i) *(sa_u32x4*)(tile + (i * 64 * NW + tid) * 16) = (sa_u32x4){0u, 0u, 0u, 0u};
   }
   // rows whose bit is 0 become zeros (this thread's share; between two barriers)
   __device__ __forceinline__ void zero(unsigned long live, char* tile, int tid) const {

@@ -286,6 +286,7 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, (DP == 128 && REL ?
     if (u0 < u1) {
       const SaDma<DP, NW, SA_ROWS> ldv(p.v_sl, p.D, tid);
       ldv.load(p.v + ((long)b * p.v_sb + (long)hkv * p.v_sh) * 2, kbk * SA_ROWS, kv_end, ldsV, w);
+      if (p.D < DP) ldv.zero_columns(p.D, ldsV, tid);      // both operands of dP come from LDS: one of them holds zeros past D
     }
   f32x16 dk[NT], dv[NT];
 #pragma unroll

@@ -148,6 +148,11 @@ CASES = [
     (1, 800, 850, 4, 2, 64, HF, "none", (48, 500, True, 30)),
     (1, 900, 4500, 2, 1, 128, BF, "keys", None),
     (1, 4300, 70, 1, 1, 40, BF, "keys", None),
+    # head sizes between 64 and 128: columns that only the tile has
+    (2, 129, 200, 4, 2, 96, BF, "keys", None),
+    (1, 70, 130, 2, 2, 72, HF, "none", None),
+    (1, 200, 300, 2, 1, 104, BF, "lens", None),
+    (2, 40, 90, 4, 4, 120, HF, "both", None),
 ]
 
 
