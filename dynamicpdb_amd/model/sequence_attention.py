@@ -315,6 +315,7 @@ class QKNormRopeFn(Function):
         q, k, w_q, w_k, q_pos, k_pos = ctx.saved_tensors
         ref = q if q is not None else k
         grads, parts, ws = [None] * 4, [], None
+        gq, gk = (None if x is None else _rows16(g) for x, g in ((q, gq), (k, gk)))      # (copies live until the launch)
         for i, (x, w, pos, g) in enumerate(((q, w_q, q_pos, gq), (k, w_k, k_pos, gk))):
             if x is None:
                 parts.append(_NO_PART)
@@ -325,7 +326,7 @@ class QKNormRopeFn(Function):
                 dw = grads[2 + i] = torch.empty_like(w) if x.numel() else torch.zeros_like(w)
                 if ws is None:
                     ws = torch.empty(_lib.lib().dfold_qk_norm_rope_ws(), dtype=F32, device=ref.device)
-            parts.append(_rope_part(x, dx, w, pos, _rows16(g), dw))
+            parts.append(_rope_part(x, dx, w, pos, g, dw))
         if parts != [_NO_PART, _NO_PART]:
             _call("dfold_qk_norm_rope_bwd", _rope_desc(parts, ref, ctx.opts, ws), t=ref)
         return (*grads, None, None, None, None, None, None)

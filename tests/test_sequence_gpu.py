@@ -531,6 +531,24 @@ def test_norm_rope_layouts_and_options():
     assert bool((y == 0).all()) and bool(torch.isfinite(torch.autograd.grad(y, zero, torch.ones_like(y))[0]).all())
 
 
+@pytest.mark.parametrize("dt", [F32, BF])
+def test_norm_rope_copies_of_gradients_live(dt):
+    """gradients that have to be copied before the kernel can read them, of q and k alike in size: the copies, the results and the
+    workspace are distinct memory until the launch"""
+    gen = torch.Generator(device=DEV).manual_seed(4)
+    r = lambda *s: torch.randn(*s, generator=gen, device=DEV).to(dt)
+    for B, L, H, D in ((1, 10, 30, 120), (2, 6, 4, 32), (1, 300, 8, 64)):
+        leaves = [r(B, L, H, D).requires_grad_(True), r(B, L, H, D).requires_grad_(True)] + [(1 + 0.2 * r(D).float()).requires_grad_(True) for _ in range(2)]
+        gq, gk = r(B, L, H, D), r(B, L, H, D)
+        out = S.qk_norm_rope(*leaves, rotary_dim=32)
+        want = torch.autograd.grad(out, leaves, [gq, gk], retain_graph=True)
+        odd = lambda g: torch.cat([g.new_zeros(1), g.reshape(-1)])[1:].view(g.shape)          # an address that is no multiple of 16
+        part = lambda g: torch.cat([g, g[..., :1]], -1)[..., :D]                                # rows that are not
+        for a, b in ((odd, odd), (part, part), (odd, part), (part, lambda g: g), (lambda g: g, odd)):
+            got = torch.autograd.grad(out, leaves, [a(gq), b(gk)], retain_graph=True)
+            assert all(torch.equal(x, y) for x, y in zip(want, got))
+
+
 # ---- together ---------------------------------------------------------------------------------------------------------------------------
 
 def chain(qkv, wq, wk, table, lens, dist):
