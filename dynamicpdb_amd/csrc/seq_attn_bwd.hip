@@ -55,6 +55,37 @@ __device__ __forceinline__ void sa_logits(f32x16& s, float sl2, float nlse, cons
   }
 }
 
+// A block of dS that f16 cannot hold, though the products' sums may well be within it (dS is nobody's gradient): every column beyond the type
+// is scaled by a power of two to just below its largest value, and the accumulators' same column with it for the length of `products`.
+// Both lane halves of a column agree on the factor; columns within the type keep theirs, bit for bit.  f16 pays a maximum per block for
+// it (bf16 holds every finite dS).
+template <int DT, int N, typename F>
+__device__ __forceinline__ void sa_within(f32x16& ds, f32x16(&acc)[N], F products) {
+  bool beyond = false;
+  int e = 0;
+  if constexpr (DT == DFOLD_DT_F16) {
+    float mx = 0.f;
+#pragma unroll
+    for (int r = 0; r < 16; r += 2) mx = fmaxf(fmaxf(mx, fabsf(ds[r])), fabsf(ds[r + 1]));
+    beyond = __ballot(mx > 65504.f) != 0;
+    if (__builtin_expect(beyond, 0)) {
+      mx = sa_xmax(mx);
+      e = mx > 65504.f && mx < INFINITY ? __builtin_amdgcn_frexp_expf(mx) - 15 : 0;      // mx < 2^(15 + e)
+      const float down = ldexpf(1.f, -e);
+#pragma unroll
+      for (int r = 0; r < 16; ++r) ds[r] *= down;
+#pragma unroll
+      for (int i = 0; i < N; ++i) acc[i] *= down;
+    }
+  }
+  products();
+  if (__builtin_expect(beyond, 0)) {
+    const float up = ldexpf(1.f, e);
+#pragma unroll
+    for (int i = 0; i < N; ++i) acc[i] *= up;
+  }
+}
+
 // PAIR: as in the forward, two waves for the same 32 rows, one per half of a key tile
 template <int DT, int DP, bool REL, bool PAIR>
 __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_dq_kernel(const SaBwdParams p) {
@@ -167,14 +198,16 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_dq
         s[r] = sa_exp2(s[r]) * (dp[r] - dl);
         left += s[r];
       }
+      sa_within<DT>(s, dq, [&] {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        sa_u32x4 df;      // dS in the operand type: relative error up to 2^-8 (bf16) / 2^-11 (f16) of each term of dQ's sum
+        for (int c = 0; c < 2; ++c) {
+          sa_u32x4 df;      // dS in the operand type: relative error up to 2^-8 (bf16) / 2^-11 (f16) of each term of dQ's sum
 #pragma unroll
-        for (int e = 0; e < 4; ++e) df[e] = sa_pack2<DT>(s[8 * c + 2 * e], s[8 * c + 2 * e + 1]);
+          for (int e = 0; e < 4; ++e) df[e] = sa_pack2<DT>(s[8 * c + 2 * e], s[8 * c + 2 * e + 1]);
 #pragma unroll
-        for (int i = 0; i < NT; ++i) dq[i] = sa_mfma<DT>(ad.cols(lk, kb * 32 + c * 16, i), df, dq[i]);
-      }
+          for (int i = 0; i < NT; ++i) dq[i] = sa_mfma<DT>(ad.cols(lk, kb * 32 + c * 16, i), df, dq[i]);
+        }
+      });
     }
   };
   sa_walk(t0, t1, fetch, step);
@@ -427,20 +460,22 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, (DP == 128 && REL ?
           __builtin_amdgcn_wave_barrier();
         }
       }
+      sa_within<DT>(dp, dk, [&] {
 #pragma unroll
-      for (int c = 0; c < 2; ++c) {
-        sa_u32x4 pf, df;      // P and dS in the operand type: relative error up to 2^-8 (bf16) / 2^-11 (f16) of each term
+        for (int c = 0; c < 2; ++c) {
+          sa_u32x4 pf, df;      // P and dS in the operand type: relative error up to 2^-8 (bf16) / 2^-11 (f16) of each term
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          pf[e] = sa_pack2<DT>(s[8 * c + 2 * e], s[8 * c + 2 * e + 1]);
-          df[e] = sa_pack2<DT>(dp[8 * c + 2 * e], dp[8 * c + 2 * e + 1]);
+          for (int e = 0; e < 4; ++e) {
+            pf[e] = sa_pack2<DT>(s[8 * c + 2 * e], s[8 * c + 2 * e + 1]);
+            df[e] = sa_pack2<DT>(dp[8 * c + 2 * e], dp[8 * c + 2 * e + 1]);
+          }
+#pragma unroll
+          for (int i = 0; i < NT; ++i) {
+            dv[i] = sa_mfma<DT>(ad.cols(lg, qb * 32 + c * 16, i), pf, dv[i]);
+            dk[i] = sa_mfma<DT>(ad.cols(lq, qb * 32 + c * 16, i), df, dk[i]);
+          }
         }
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          dv[i] = sa_mfma<DT>(ad.cols(lg, qb * 32 + c * 16, i), pf, dv[i]);
-          dk[i] = sa_mfma<DT>(ad.cols(lq, qb * 32 + c * 16, i), df, dk[i]);
-        }
-      }
+      });
     }
   };
   sa_walk(u0, u1, fetch, step);

@@ -535,7 +535,7 @@ def cross_attention(q, k, v, *, key_mask=None, kv_lens=None, rel_table=None, max
     [num_buckets, H] adds the bias of relative_position_bias without forming it; q_offset: position of query 0 minus position of key 0, a
     whole number or an int32 / int64 tensor [B] (one token at its own position per sequence).  scale defaults to D^-1/2.
     Differentiable (once) in q, k, v and rel_table; repeated calls give the same bits.  P and dS are rounded to the operand type between
-    the products: an fp16 dS beyond 65504 becomes infinite, as any fp16 gradient does."""
+    the products (an fp16 dS beyond 65504 in units of a power of two that holds it: only the gradients themselves have to fit the type)."""
     dt, dev = q.dtype, q.get_device()
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError("q must be [B, Lq, H, D], k and v [B, Lk, Hkv, D]")

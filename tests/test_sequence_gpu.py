@@ -663,3 +663,50 @@ def test_module(context):
     assert out.dtype == x.dtype and rel(out.detach(), ref.detach()) <= 5 * 2.0 ** -8
     for (name, a), b in zip([("x", got[0])] + ([("context", got[1])] if context else []) + list(zip([k for k, _ in m.named_parameters()], got[1 + context:])), refs):
         assert rel(a, b) <= 5 * 2.0 ** -8, name
+
+
+# ---- every form of the kernels -----------------------------------------------------------------------------------------------------------
+
+class forms:
+    """both directions in `parts` parts of the walked axis, with one or two waves per 32 rows"""
+
+    def __init__(self, parts, pair):
+        self.new = (lambda *a, **kw: parts), (lambda *a: pair)
+
+    def __enter__(self):
+        self.old = S._parts, S._pair
+        S._parts, S._pair = self.new
+        S._attn_plan.cache_clear(), S._grad_plan.cache_clear()
+
+    def __exit__(self, *exc):
+        S._parts, S._pair = self.old
+        S._attn_plan.cache_clear(), S._grad_plan.cache_clear()
+
+
+@pytest.mark.parametrize("rel", [False, True])
+@pytest.mark.parametrize("B,Lq,Lk,H,Hkv,D", [(1, 40, 180, 2, 1, 32), (1, 70, 150, 2, 2, 64), (2, 130, 200, 4, 2, 128), (1, 200, 300, 2, 1, 72)])
+def test_attention_fp16_gradient_beyond_the_type(B, Lq, Lk, H, Hkv, D, rel):
+    """dS = P (dP - delta) beyond 65504 where dQ, dK and dV are not: a few rows (keys) of it, the others stay as they are"""
+    q, k, v, g = make(B, Lq, Lk, H, Hkv, D, HF, seed=8)
+    # rows 0, 7, ...: dS around 2^17 on key 3 (P about 0.6 / n over n keys), as much in sum on the others
+    n = Lk // 2 + 1
+    g[:, ::7] *= 2.0 ** 13
+    v[:, 3] *= 2.0 ** 17 * n / 0.6 / (2.0 ** 13 * D ** 0.5)
+    q[:, ::7], k[:, 3] = q[:, ::7] * 2.0 ** -6, k[:, 3] * 2.0 ** -8
+    live, kw = make_mask("lens", B, Lk)
+    table = buckets = None
+    if rel:
+        table = 0.25 * torch.randn(32, H, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))
+        buckets = bucket_matrix(Lq, Lk, 32, 128, True, 0)
+    ref = reference(q, k, v, g, live, table, buckets, D ** -0.5)
+    q64, k64, v64, g64 = (t.cpu().double().transpose(1, 2).repeat_interleave(H // t.shape[2], 1) for t in (q, k, v, g))
+    s = q64 @ k64.transpose(-1, -2) * D ** -0.5 + (table.cpu().double()[buckets.cpu()].permute(0, 3, 1, 2) if rel else 0)
+    p = torch.softmax(s.masked_fill(~live.cpu()[:, None, None], -1e300), -1)
+    dp = g64 @ v64.transpose(-1, -2)
+    assert (p * (dp - (p * dp).sum(-1, keepdim=True)))[0].abs().max() > 2 * 65504
+    assert all(ref[n][0].abs().max() < 60000 for n in ("dq", "dk", "dv"))
+    for parts, pair in ((1, 0), (1, 1), (3, 1)):
+        with forms(parts, pair):
+            got = run(q, k, v, g, table, **kw)
+        for n in ref:
+            within(f"{n} in {parts} parts", got[n], ref[n])
