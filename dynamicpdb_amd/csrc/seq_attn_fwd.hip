@@ -1,6 +1,10 @@
 // Attention of one sequence over another, forward:  o = softmax(scale q k^T + bias) v  per head, one pass over the keys with the
 // running maximum and sum of the softmax.
 //
+// What is kept of a row are two numbers, the reference mu of its exponents (log2 units, as rounded where it is subtracted) and the sum l of
+// exp2(logit - mu): one, mu + log2(l), would lose l wherever |mu| is large (a row of nothing but keys whose bias is -1e9: the sum of n ones
+// drops out).  Parts and pairs meet with weights exp2(mu_part - mu) l_part, the backward takes P = exp2(logit - mu) / l.
+//
 // A workgroup owns 128 softmax rows of one key head (4 waves x 32 rows; with pack > 1 the rows of the query heads of a group are
 // interleaved, head fastest, so that one token of a grouped layer fills its tile), walks its part of the keys in tiles of 64 and
 // keeps S, P and O in registers; K and V tiles go to LDS by DMA ahead of the arithmetic, one barrier per tile.  Key masks are one
@@ -27,6 +31,13 @@ struct SaFwdParams {
 // maximum only when it has grown by more than this (P stays <= 2^8: exact in fp32 sums, harmless in 16-bit operands)
 #define SA_LAZY 8.f
 #define SA_MAX_SPLITS 1024
+
+// a row's statistics for the backward: plane 0 the reference of its exponents (+inf: no keys), plane 1 the inverse of their sum
+__device__ __forceinline__ void sa_row_stat(const SaFwdParams& p, int b, int head, int qi, float mu, float inv) {
+  float* const st = p.lse + ((long)b * p.H + head) * p.Lq + qi;
+  st[0] = mu;
+  st[(long)p.B * p.H * p.Lq] = inv;
+}
 
 // PAIR: eight waves, two for the same 32 rows, one per half of a key tile, joined in LDS at the end: a launch of at most one workgroup
 // per CU has two waves per SIMD instead of one.
@@ -156,7 +167,8 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_fw
       for (int r = 0; r < 16; r += 2) mt = fmaxf(fmaxf(mt, s[kb][r]), s[kb][r + 1]);
     mt = sa_xmax(mt);
     if (__ballot(mt > m + lazy)) {
-      const float mn = fmaxf(m, mt), a = m == mn ? 1.f : sa_exp2((m - mn) * us);     // (m == mn also for rows without keys so far)
+      // (the difference of the references as they are subtracted below; m == mn also for rows without keys so far)
+      const float mn = fmaxf(m, mt), a = m == mn ? 1.f : sa_exp2(m * us - mn * us);
       m = mn;
       l *= a;
 #pragma unroll
@@ -200,7 +212,7 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_fw
     __syncthreads();
     if (half) return;
     const float m1 = ml[0], mn = fmaxf(m, m1);
-    const float a0 = m == mn ? 1.f : sa_exp2((m - mn) * us), a1 = m1 == mn ? 1.f : sa_exp2((m1 - mn) * us);
+    const float a0 = m == mn ? 1.f : sa_exp2(m * us - mn * us), a1 = m1 == mn ? 1.f : sa_exp2(m1 * us - mn * us);
     m = mn;
     l = l * a0 + ml[1] * a1;
 #pragma unroll
@@ -211,11 +223,12 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_fw
     }
   }
   if (!wave_on) return;
-  const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+  const bool any = l > 0.f || l != l;
+  const float inv = any ? 1.f / l : 0.f;
   if (!on) return;
   const int head = head0 + hl;
   if (p.splits == 1) {
-    if (p.lse && h == 0) p.lse[((long)b * p.H + head) * p.Lq + qi] = l > 0.f || l != l ? m * us + __log2f(l) : INFINITY;
+    if (p.lse && h == 0) sa_row_stat(p, b, head, qi, any ? m * us : INFINITY, inv);
     char* const dst = p.o + ((long)b * p.o_sb + (long)qi * p.o_sl + (long)head * p.o_sh) * 2;
 #pragma unroll
     for (int i = 0; i < NT; ++i)
@@ -226,10 +239,14 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_fw
         *(uint2*)(dst + d * 2) = (uint2){sa_pack2<DT>(O[i][g * 4] * inv, O[i][g * 4 + 1] * inv), sa_pack2<DT>(O[i][g * 4 + 2] * inv, O[i][g * 4 + 3] * inv)};
       }
   } else {
-    // partial result: normalised O and the log2 of the part's sum (-inf: no keys), [split][b][query][head][D], [split][b][query][head]
+    // partial result: normalised O [split][b][query][head][D], then the part's reference (-inf: no keys) and its sum [2][split][b][query][head]
     const long r1 = ((long)b * p.Lq + qi) * p.H + head, nr = (long)p.B * p.Lq * p.H;
     float* const dst = p.ws + ((long)sp * nr + r1) * p.D;
-    if (h == 0) p.ws[p.splits * nr * p.D + sp * nr + r1] = l > 0.f || l != l ? m * us + __log2f(l) : -INFINITY;
+    if (h == 0) {
+      float* const st = p.ws + p.splits * nr * p.D + sp * nr + r1;
+      st[0] = any ? m * us : -INFINITY;
+      st[p.splits * nr] = l;
+    }
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -240,7 +257,7 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_fw
   }
 }
 
-// o = sum_s 2^(lse_s - max) o_s / sum_s 2^(lse_s - max), splits in order.  One 8-element chunk of a row per thread.
+// o = sum_s w_s o_s / sum_s w_s, w_s = 2^(mu_s - max mu) l_s, splits in order.  One 8-element chunk of a row per thread.
 template <int DT>
 __global__ __launch_bounds__(256) void seq_attn_combine_kernel(const SaFwdParams p) {
   const int cpr = p.D / 8;
@@ -248,13 +265,13 @@ __global__ __launch_bounds__(256) void seq_attn_combine_kernel(const SaFwdParams
   if (idx >= nr * cpr) return;
   const long r = idx / cpr;
   const int c = (int)(idx - r * cpr);
-  const float* const ls = p.ws + p.splits * nr * p.D + r;
+  const float *const ls = p.ws + p.splits * nr * p.D + r, *const sums = ls + p.splits * nr;
   float m = -INFINITY;
   for (int s = 0; s < p.splits; ++s) m = fmaxf(m, ls[s * nr]);
   const float mu = m == -INFINITY ? 0.f : m;
   float l = 0.f, o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
   for (int s = 0; s < p.splits; ++s) {
-    const float wgt = sa_exp2(ls[s * nr] - mu);
+    const float wgt = sa_exp2(ls[s * nr] - mu) * sums[s * nr];
     const float* const src = p.ws + (s * nr + r) * p.D + c * 8;
     const f32x4 a = *(const f32x4*)src, bb = *(const f32x4*)(src + 4);
     l += wgt;
@@ -268,7 +285,7 @@ __global__ __launch_bounds__(256) void seq_attn_combine_kernel(const SaFwdParams
   const int head = (int)(r % p.H);
   const long bq = r / p.H;
   const int qi = (int)(bq % p.Lq), b = (int)(bq / p.Lq);
-  if (p.lse && c == 0) p.lse[((long)b * p.H + head) * p.Lq + qi] = l > 0.f || l != l ? m + __log2f(l) : INFINITY;
+  if (p.lse && c == 0) sa_row_stat(p, b, head, qi, l > 0.f || l != l ? m : INFINITY, inv);
   sa_u32x4 u;
 #pragma unroll
   for (int e = 0; e < 4; ++e) u[e] = sa_pack2<DT>(o[2 * e] * inv, o[2 * e + 1] * inv);
@@ -283,14 +300,14 @@ __global__ __launch_bounds__(256) void seq_attn_combine_row_kernel(const SaFwdPa
   __shared__ f32x4 part[256];
   const int tid = threadIdx.x, lane = tid & 63;
   const long nr = (long)p.B * p.Lq * p.H, r = blockIdx.x;
-  const float* const ls = p.ws + p.splits * nr * p.D + r;
+  const float *const ls = p.ws + p.splits * nr * p.D + r, *const sums = ls + p.splits * nr;
   // (every wave forms the maximum and the sum for itself)
   float m = -INFINITY, l = 0.f;
   for (int s = lane; s < p.splits; s += 64) m = fmaxf(m, ls[s * nr]);
   m = wave_max(m);
   const float mu = m == -INFINITY ? 0.f : m;
   for (int s = lane; s < p.splits; s += 64) {
-    const float x = sa_exp2(ls[s * nr] - mu);
+    const float x = sa_exp2(ls[s * nr] - mu) * sums[s * nr];
     if (tid < 64) wgt[s] = x;
     l += x;
   }
@@ -314,7 +331,7 @@ __global__ __launch_bounds__(256) void seq_attn_combine_row_kernel(const SaFwdPa
   const int head = (int)(r % p.H);
   const long bq = r / p.H;
   const int qi = (int)(bq % p.Lq), b = (int)(bq / p.Lq);
-  if (p.lse && tid == 0) p.lse[((long)b * p.H + head) * p.Lq + qi] = l > 0.f || l != l ? m + __log2f(l) : INFINITY;
+  if (p.lse && tid == 0) sa_row_stat(p, b, head, qi, l > 0.f || l != l ? m : INFINITY, inv);
   *(uint2*)(p.o + ((long)b * p.o_sb + (long)qi * p.o_sl + (long)head * p.o_sh + tid * 4) * 2) =
       (uint2){sa_pack2<DT>(o[0] * inv, o[1] * inv), sa_pack2<DT>(o[2] * inv, o[3] * inv)};
 }

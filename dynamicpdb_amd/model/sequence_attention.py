@@ -474,7 +474,7 @@ def _attn_forward(train, q, k, v, table, key_mask, kv_lens, q_offsets, q_offset,
     Lk, Hkv = k.shape[1], k.shape[2]
     dev = q.device
     o = _dense_like(q)
-    lse = torch.empty((B, H, Lq), dtype=F32, device=dev) if train else None
+    lse = torch.empty((2, B, H, Lq), dtype=F32, device=dev) if train else None
     if table is not None and not table.is_contiguous():
         table = table.contiguous()
     if B and Lq:
@@ -484,7 +484,7 @@ def _attn_forward(train, q, k, v, table, key_mask, kv_lens, q_offsets, q_offset,
             rel = _rel_desc(table, nb, max_distance, bidirectional, q_offset, q_offsets)
             width = 2 * _reach(nb, max_distance, bidirectional) + 1
         pack, splits, pair = _attn_plan(B, Lq, Lk, H, Hkv, width, ops.cu_count(dev))
-        ws = torch.empty(splits * B * H * Lq * (D + 1), dtype=F32, device=dev) if splits > 1 else None
+        ws = torch.empty(splits * B * H * Lq * (D + 2), dtype=F32, device=dev) if splits > 1 else None
         _call("dfold_seq_attn_fwd", _attn_desc(q, k, v, o, lse, ws, key_mask, kv_lens, rel, scale, pack, splits, pair), t=q)
     return o, (q, k, v, table, key_mask, kv_lens, q_offsets, o, lse)
 

@@ -35,9 +35,10 @@ extern "C" {
 /* Bumped whenever a signature, a pointer's element type or a struct layout changes (2: round-3 changes of
  * dfold_ipa_softmax_bwd / dfold_ipa_col_bwd (bf16 probabilities, `ctr`) and dfold_ipa_bias_grad (`nh_pitch`); the
  * round-4 additions; 3: round 6, the zero-frame fields at the end of dfold_gemm_desc, the two extra arguments of
- * dfold_conv_wgrad_tn, dfold_grid_load_flags).  The Python binding reads the number from THIS header and refuses a library that reports
- * another one (dynamicpdb_amd/_lib.py), so a stale or variant .so cannot be called with shifted arguments. */
-#define DFOLD_ABI_VERSION 3
+ * dfold_conv_wgrad_tn, dfold_grid_load_flags; 4: two planes of dfold_seq_attn_desc.lse, D + 2 floats a row in its ws).  The
+ * Python binding reads the number from THIS header and refuses a library that reports another one (dynamicpdb_amd/_lib.py), so a
+ * stale or variant .so cannot be called with shifted arguments. */
+#define DFOLD_ABI_VERSION 4
 int dfold_abi_version(void);
 
 /* ------------------------------------------------------------------------------------------------
@@ -637,8 +638,9 @@ int dfold_relpos_ws(int32_t H, int32_t Lq, int32_t num_buckets);
  * strides in elements, multiples of 8, row strides (*_sl) below 2^24, base pointers 16-byte aligned; D a multiple of 8, <= 128; H a multiple of Hkv (query head h
  * reads key head h / (H / Hkv)).  Keys j >= kv_lens[b] and keys with key_mask[b * mask_sb + j] == 0 do not exist: their K and V
  * are never used (they may hold NaN); a row without any key gives zeros.
- *   lse [B][H][Lq] fp32 (optional): log2 of the row's sum of exp2 (logits x log2 e); +inf for a row without keys.
- *   splits > 1: the keys are cut into that many parts; ws: splits * B * H * Lq * (D + 1) floats.
+ *   lse [2][B][H][Lq] fp32 (optional): what the backward needs of a row -- a reference mu near the maximum of its logits x log2 e (+inf for a
+ *   row without keys), and 1 / the row's sum of exp2(logits x log2 e - mu) (0 for such a row).
+ *   splits > 1: the keys are cut into that many parts; ws: splits * B * H * Lq * (D + 2) floats.
  *   pack = 1, or H / Hkv (rows of the query heads of a group share tiles: few queries).
  *   pair = 1: two waves per 32 rows, one per half of a key tile (launches that leave SIMDs idle); 0: one.  Any value is right. */
 typedef struct {

@@ -710,3 +710,49 @@ def test_attention_fp16_gradient_beyond_the_type(B, Lq, Lk, H, Hkv, D, rel):
             got = run(q, k, v, g, table, **kw)
         for n in ref:
             within(f"{n} in {parts} parts", got[n], ref[n])
+
+
+# ---- rows whose logits are far from zero ------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("low", [-1e9, -1e30, torch.finfo(torch.float32).min])
+@pytest.mark.parametrize("B,Lq,Lk,H,Hkv,D,mask", [(1, 3, 1000, 2, 1, 64, "none"), (2, 130, 700, 4, 2, 32, "both"), (2, 70, 333, 2, 2, 128, "lens"),
+                                                  (1, 40, 90, 2, 2, 40, "keys")])
+def test_attention_rows_of_large_bias(B, Lq, Lk, H, Hkv, D, mask, low):
+    """every key of every row in a bucket of a large negative entry: an ordinary softmax over them, forward and backward, also where the
+    walk is cut into parts of unequal length.  At -1e9 the step of fp32 is 64, so the logits (|logit| < 16 here) drop out and every key
+    weighs the same: the definition at a scale of 2^-60 (logits below 2^-50), its dQ and dK taken to the scale of the call."""
+    q, k, v, g = make(B, Lq, Lk, H, Hkv, D, BF, seed=11)
+    live, kw = make_mask(mask, B, Lk, seed=1)
+    table = torch.randn(8, H, device=DEV)
+    table[3] = low
+    off = Lk + 16                                # distances of -16 and beyond only
+    buckets = bucket_matrix(Lq, Lk, 8, 16, True, off)
+    assert bool((buckets == 3).all())
+    ref = reference(q, k, v, g, live, table, buckets, 2.0 ** -60)
+    for n in ("dq", "dk"):
+        ref[n] = tuple(x * (2.0 ** 60 * D ** -0.5) for x in ref[n])
+    for parts, pair in ((None, None), (1, 0), (3, 1), (7, 0)):
+        if parts is None:
+            got = run(q, k, v, g, table, max_distance=16, q_offset=off, **kw)
+        else:
+            with forms(parts, pair):
+                got = run(q, k, v, g, table, max_distance=16, q_offset=off, **kw)
+        for n in ref:
+            within(f"{n} in {parts} parts", got[n], ref[n])
+
+
+@pytest.mark.parametrize("dt", [BF, HF])
+@pytest.mark.parametrize("B,Lq,Lk,H,Hkv,D", [(1, 3, 700, 2, 1, 64), (1, 130, 300, 2, 2, 32), (2, 40, 500, 2, 1, 128)])
+def test_attention_rows_of_large_logits(B, Lq, Lk, H, Hkv, D, dt):
+    """logits of 2^24 without a bias, all the same (one column of Q and K, products exact): uniform rows, forward and backward"""
+    _, _, v, g = make(B, Lq, Lk, H, Hkv, D, dt, seed=12)
+    q, k = torch.zeros(B, Lq, H, D, dtype=dt, device=DEV), torch.zeros(B, Lk, Hkv, D, dtype=dt, device=DEV)
+    q[..., 0], k[..., 0] = 4096.0, 4096.0
+    k[..., 1] = v[..., 1]                        # (q is zero there: not part of the logits, but of dQ)
+    live, kw = make_mask("lens", B, Lk, seed=2)
+    ref = reference(q, k, v, g, live, None, None, 1.0)
+    for parts, pair in ((1, 0), (1, 1), (3, 1), (7, 0)):
+        with forms(parts, pair):
+            got = run(q, k, v, g, scale=1.0, **kw)
+        for n in ref:
+            within(f"{n} in {parts} parts", got[n], ref[n])
