@@ -111,12 +111,11 @@ def _rows16(t):
 
 
 def _strides(t):
-    """strides of the three leading axes, 0 for axes of one entry (theirs may be anything)"""
-    a, b, c, _ = t.stride()
-    if t.is_contiguous():
-        return (a, b, c) if t.numel() else (0, 0, 0)
-    n = t.shape
-    return (a if n[0] > 1 else 0, b if n[1] > 1 else 0, c if n[2] > 1 else 0)
+    """strides of the three leading axes, 0 for axes of one entry (theirs may be anything, also in a tensor that is dense for torch)"""
+    n, (a, b, c, _) = t.shape, t.stride()
+    if t.numel() == 0:
+        return 0, 0, 0
+    return a if n[0] > 1 else 0, b if n[1] > 1 else 0, c if n[2] > 1 else 0
 
 
 def _dense_like(t):

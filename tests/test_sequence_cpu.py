@@ -198,3 +198,13 @@ def test_cabi_refuses_bad_descriptors():
         assert L.dfold_qk_norm_rope_fwd(byref(rope(**kw)), st) == -1, kw
     for kw in (dict(), dict(g=tok, g_sl=4), dict(g=tok, dw=tok)):
         assert L.dfold_qk_norm_rope_bwd(byref(rope(**kw)), st) == -1, kw
+
+
+def test_strides_of_axes_of_one_entry_are_zero():
+    """dense for torch, whatever the strides of axes of one entry: the kernels get 0 for those"""
+    a = torch.zeros(1, 7, 132)[..., :128].unflatten(-1, (4, 32))[:, :1]
+    b = torch.zeros(64).as_strided((1, 1, 2, 32), (3, (1 << 24) + 5, 32, 1))
+    c = torch.zeros(2, 1, 36)[:1, :, :32].unflatten(-1, (1, 32))
+    for t, heads in ((a, 32), (b, 32), (c, 0)):
+        assert t.is_contiguous() and S._rows16(t) is t and S._strides(t) == (0, 0, heads)
+    assert S._strides(torch.zeros(2, 3, 4, 8)) == (96, 32, 8) and S._strides(torch.zeros(2, 0, 4, 8)) == (0, 0, 0)

@@ -756,3 +756,29 @@ def test_attention_rows_of_large_logits(B, Lq, Lk, H, Hkv, D, dt):
             got = run(q, k, v, g, scale=1.0, **kw)
         for n in ref:
             within(f"{n} in {parts} parts", got[n], ref[n])
+
+
+def test_axes_of_one_entry_take_any_stride():
+    """one token of a batch of one out of a projection whose rows are not a multiple of 16 bytes: dense for torch, whatever the strides of
+    the axes of one entry"""
+    H, Hkv, D, Lk = 4, 2, 32, 50
+    gen = torch.Generator(device=DEV).manual_seed(6)
+    r = lambda *s: torch.randn(*s, generator=gen, device=DEV).to(BF)
+    one = lambda h: r(1, 7, h * D + 4)[..., :h * D].unflatten(-1, (h, D))[:, :1]
+    far = r(1, 1, H, D).as_strided((1, 1, H, D), (3, (1 << 24) + 5, D, 1))
+    k, v = r(1, Lk, Hkv, D), r(1, Lk, Hkv, D)
+    for q, g in ((one(H), one(H)), (far, one(H)), (one(H), far)):
+        assert q.is_contiguous() and (q.stride(1) % 8 or q.stride(0) % 8 or g.stride(1) % 8)
+        want = run(q.clone(), k, v, g.clone())
+        got = run(q, k, v, g)
+        assert all(torch.equal(want[n], got[n]) for n in want)
+        got = run(r(1, 5, H, D), one(Hkv), one(Hkv), r(1, 5, H, D))
+        assert all(bool(torch.isfinite(x).all()) for x in got.values())
+        w = torch.ones(D, device=DEV)
+        want = S.qk_norm_rope(q.clone(), one(Hkv), w, w)[0]
+        x = q.detach().requires_grad_(True)
+        y = S.qk_norm_rope(x, one(Hkv), w, w)[0]
+        assert torch.equal(y, want)
+        (dx,) = torch.autograd.grad(y, x, g)
+        x2 = q.clone().requires_grad_(True)
+        assert torch.equal(dx, torch.autograd.grad(S.qk_norm_rope(x2, None, w)[0], x2, g.clone())[0])
