@@ -782,3 +782,25 @@ def test_axes_of_one_entry_take_any_stride():
         (dx,) = torch.autograd.grad(y, x, g)
         x2 = q.clone().requires_grad_(True)
         assert torch.equal(dx, torch.autograd.grad(S.qk_norm_rope(x2, None, w)[0], x2, g.clone())[0])
+
+
+@pytest.mark.parametrize("dt", [F32, BF])
+@pytest.mark.parametrize("B,Lq,Lk,H,Hkv,D", [(1, 3, 1, 5, 1, 64), (1, 2731, 9, 3, 2, 256), (2, 700, 700, 7, 1, 96)])
+@pytest.mark.parametrize("eps", [0.0, 1e-60])
+def test_norm_rope_without_eps(B, Lq, Lk, H, Hkv, D, dt, eps):
+    """eps of 0 (or one that is 0 in fp32): rows that are not zero are ordinary, in blocks that the rows do not fill too"""
+    gen = torch.Generator(device=DEV).manual_seed(9)
+    r = lambda *s: torch.randn(*s, generator=gen, device=DEV)
+    q, k = r(B, Lq, H, D).to(dt).requires_grad_(True), r(B, Lk, Hkv, D).to(dt).requires_grad_(True)
+    wq, wk = (1 + 0.2 * r(D)).requires_grad_(True), (1 + 0.2 * r(D)).requires_grad_(True)
+    gq, gk = r(B, Lq, H, D).to(dt), r(B, Lk, Hkv, D).to(dt)
+    oq, ok = S.qk_norm_rope(q, k, wq, wk, rotary_dim=32, eps=eps)
+    grads = torch.autograd.grad([oq, ok], [q, k, wq, wk], [gq, gk])
+    u = torch.finfo(dt).eps / 2
+    for x, w, g, o, dx, dw in ((q, wq, gq, oq, grads[0], grads[2]), (k, wk, gk, ok, grads[1], grads[3])):
+        with torch.no_grad():
+            ref = rope_reference(x, w, torch.arange(x.shape[1], device=DEV)[None], 32, 10000.0, False, 0.0, g)
+        for n, got, (want, err) in zip(("y", "dx"), (o.detach(), dx), ref):
+            within(n, got, (want, err + u * (want.abs() + err) + 1e-30))
+        rows = x.numel() // D
+        within("dw", dw, (ref[2][0], ref[2][1] * (1 + (rows / 1024 + 256) / 64)))
