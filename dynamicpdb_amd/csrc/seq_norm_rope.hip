@@ -143,8 +143,8 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(const NrParams p) {
 #pragma unroll
       for (int e = 0; e < V; ++e) ss = __builtin_fmaf(x[e], x[e], ss);
       for (int o = 1; o < lanes; o <<= 1) ss += __shfl_xor(ss, o, 64);
-      // (lanes without a row would divide by 0 where eps is 0: 0 * inf in dw's sum)
-      const float rstd = use ? 1.f / sqrtf(__builtin_fmaf(ss, invD, p.eps)) : 0.f;
+      // (lanes without a row would divide by 0 where eps is 0: 0 * inf in dw's sum.  Chosen before the root: no branch around it)
+      const float rstd = 1.f / sqrtf(use ? __builtin_fmaf(ss, invD, p.eps) : 1.f);
       if constexpr (!BWD) {
 #pragma unroll
         for (int e = 0; e < V; ++e) x[e] = x[e] * rstd * w[e];
