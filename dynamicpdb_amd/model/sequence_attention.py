@@ -363,7 +363,7 @@ def qk_norm_rope(q, k, w_q=None, w_k=None, q_positions=None, k_positions=None, *
     """Every head of q [B, Lq, H, D] and k [B, Lk, Hkv, D] divided by its root mean square, times w (fp32 [D] or None), then its first
     rotary_dim dimensions (default: all; a multiple of 16; 0: none) rotated by position * base^(-2 i / rotary_dim): pairs
     (i, i + rotary_dim / 2), or (2 i, 2 i + 1) if interleaved.  k may be None (keys that are rotated already).  Positions: int64 / int32
-    [L] or [B, L], default 0, 1, ...; angles are reduced in fp64 (right to fp32 rounding up to positions of 2^31).  bf16, fp16 or fp32;
+    [L] or [B, L], default 0, 1, ...; angles are reduced in fp64 (right to fp32 rounding up to positions of 2^28).  bf16, fp16 or fp32;
     one launch for q and k; differentiable (once) in q, k, w_q, w_k."""
     ref = q if q is not None else k
     if ref is None:

@@ -676,7 +676,7 @@ int dfold_seq_attn_bwd(const dfold_seq_attn_desc* fwd, const dfold_seq_attn_grad
  * outputs dense.  w [D] fp32 or NULL (ones).  Rotation of the first rotary_dim dimensions (a multiple of 16, 0: none): pairs
  * (i, i + rotary_dim / 2), or (2 i, 2 i + 1) if interleaved, turned by position * base^(-2 i / rotary_dim); positions int64 [B][L],
  * row stride pos_sb (0: shared by the batch), or NULL: 0, 1, ...  The angle is reduced in fp64: right to fp32 rounding up to
- * positions of 2^31.  Backward: dx like x but dense, dw [D] fp32 (optional; ws: dfold_qk_norm_rope_ws() floats). */
+ * positions of 2^28.  Backward: dx like x but dense, dw [D] fp32 (optional; ws: dfold_qk_norm_rope_ws() floats). */
 typedef struct {
   const void* x;
   void* y;             /* output; backward: dx */

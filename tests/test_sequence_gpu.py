@@ -804,3 +804,32 @@ def test_norm_rope_without_eps(B, Lq, Lk, H, Hkv, D, dt, eps):
             within(n, got, (want, err + u * (want.abs() + err) + 1e-30))
         rows = x.numel() // D
         within("dw", dw, (ref[2][0], ref[2][1] * (1 + (rows / 1024 + 256) / 64)))
+
+
+def _turns(pos, i, rd, base):
+    """whole-number position x base^(-2 i / rd) / (2 pi), less its whole turns, from 60 digits"""
+    from decimal import Decimal, localcontext
+    with localcontext() as c:
+        c.prec = 60
+        atan = lambda n: sum((-1) ** m / (Decimal(2 * m + 1) * Decimal(n) ** (2 * m + 1)) for m in range(60))
+        two_pi = 8 * (4 * atan(5) - atan(239))
+        t = Decimal(pos) * (Decimal(base).ln() * Decimal(-2 * i) / Decimal(rd)).exp() / two_pi
+        return float(t - t.to_integral_value())
+
+
+@pytest.mark.parametrize("inter", [False, True])
+def test_norm_rope_far_positions(inter):
+    """angles at positions up to 2^28 against 60 digits.  Heads of ones have a root mean square of 1 exactly (eps = 0), so a pair becomes
+    (cos - sin, cos + sin).  Roundings, in 2^-24: the turn in fp32 (half a step of 2^-25, times 2 pi) 1.6, its factor (half a step of 2^-55, at
+    2^28 and times 2 pi) 0.4 and product (half a step of 2^-27, times 2 pi) 0.4, these times sqrt 2 in a result; cosine and sine two steps of
+    2^-24 each; the result (below 1.5) one: 8.4, at most 9"""
+    D = rd = 32
+    gen = torch.Generator().manual_seed(0)
+    pos = torch.cat([torch.tensor([0, 1, -7, 1000003, (1 << 28) - 1, 1 << 28, -(1 << 28)]), torch.randint(1 << 27, 1 << 28, (40,), generator=gen)])
+    x = torch.ones(1, len(pos), 1, D, device=DEV)
+    y, _ = S.qk_norm_rope(x, None, q_positions=pos.to(DEV), eps=0.0, interleaved=inter)
+    y = y[0, :, 0].double().cpu()
+    lo, hi = (y[:, ::2], y[:, 1::2]) if inter else (y[:, :rd // 2], y[:, rd // 2:])
+    t = torch.tensor([[_turns(int(p), i, rd, 10000) for i in range(rd // 2)] for p in pos], dtype=torch.float64) * (2 * math.pi)
+    for got, want in ((lo, t.cos() - t.sin()), (hi, t.cos() + t.sin())):
+        assert (got - want).abs().max() <= 9 * 2.0 ** -24
