@@ -18,7 +18,7 @@ from ctypes import c_double, c_float, c_int16, c_int32, c_int64, c_void_p
 
 import torch
 import torch.nn as nn
-from torch.autograd import Function
+from torch.autograd import Function, forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import _lib, ops
@@ -187,6 +187,13 @@ def _once(fn):
     return lambda ctx, *g: guarded(ctx, *g) if torch.is_grad_enabled() else fn(ctx, *g)
 
 
+def _needs_node(grad):
+    """whether a call goes through its autograd node: an input takes a gradient (grad), or may carry a forward-mode tangent (the node has
+    no derivative for that and raises), or the call is traced (the node is recorded).  The bare call would give, or record, a result
+    without its derivative or its launch."""
+    return (grad and torch.is_grad_enabled()) or forward_ad._current_level >= 0 or torch._C._get_tracing_state() is not None
+
+
 # ------------------------------------------------------------------------------------------------
 # relative position bias as a matrix
 # ------------------------------------------------------------------------------------------------
@@ -244,7 +251,7 @@ def relative_position_bias(table, q_len, k_len, *, max_distance=128, bidirection
         raise ValueError("the table needs between 1 and 65535 heads")
     _require_cuda(table)
     args = (table, q_len, k_len, max_distance, bool(bidirectional), q_offset, dtype)
-    if table.requires_grad and torch.is_grad_enabled():
+    if _needs_node(table.requires_grad):
         return RelativeBiasFn.apply(*args)
     return _bias_forward(*args)
 
@@ -398,7 +405,7 @@ def qk_norm_rope(q, k, w_q=None, w_k=None, q_positions=None, k_positions=None, *
     q_positions, k_positions = _positions(q_positions, q, dev, "q_positions"), _positions(k_positions, k, dev, "k_positions")
     _require_cuda(ref)
     args = (q, k, w_q, w_k, q_positions, k_positions, rotary_dim, float(base), bool(interleaved), float(eps))
-    if grad and torch.is_grad_enabled():
+    if _needs_node(grad):
         return QKNormRopeFn.apply(*args)
     return _rope_forward(*args)[:2]
 
@@ -585,7 +592,7 @@ def cross_attention(q, k, v, *, key_mask=None, kv_lens=None, rel_table=None, max
         raise ValueError("scale must be finite and not 0")
     _require_cuda(q)
     args = (q, k, v, rel_table, key_mask, kv_lens, q_offsets, q_offset, max_distance, bool(bidirectional), scale)
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad or (rel_table is not None and rel_table.requires_grad)):
+    if _needs_node(q.requires_grad or k.requires_grad or v.requires_grad or (rel_table is not None and rel_table.requires_grad)):
         return CrossAttentionFn.apply(*args)
     return _attn_forward(False, *args)[0]
 

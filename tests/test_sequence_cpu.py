@@ -208,3 +208,27 @@ def test_strides_of_axes_of_one_entry_are_zero():
     for t, heads in ((a, 32), (b, 32), (c, 0)):
         assert t.is_contiguous() and S._rows16(t) is t and S._strides(t) == (0, 0, heads)
     assert S._strides(torch.zeros(2, 3, 4, 8)) == (96, 32, 8) and S._strides(torch.zeros(2, 0, 4, 8)) == (0, 0, 0)
+
+
+def test_forward_mode_and_tracing_are_not_silent(monkeypatch):
+    """inputs with a tangent reach the autograd node, which has no forward-mode derivative and says so; a traced call records it or raises (the kernels
+    replaced by empty results: no GPU)"""
+    import torch.autograd.forward_ad as fw
+    from ctypes import ArgumentError
+    monkeypatch.setattr(S, "_require_cuda", lambda t: None)
+    monkeypatch.setattr(S, "_call", lambda *a, **kw: None)
+    monkeypatch.setattr(S.ops, "cu_count", lambda dev: 256)
+    q, k, v = _qkv()
+    table, w = torch.zeros(32, 4), torch.ones(32)
+    for f, t in ((lambda t: S.cross_attention(t, k, v), q), (lambda t: S.cross_attention(q, k, v, rel_table=t), table),
+                 (lambda t: S.relative_position_bias(t, 4, 4), table), (lambda t: S.qk_norm_rope(q, t)[1], k), (lambda t: S.qk_norm_rope(q, k, w_q=t)[0], w)):
+        with fw.dual_level():
+            f(t)
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError, match="jvp"):
+                    f(fw.make_dual(t, torch.ones_like(t)))
+        try:
+            graph = str(torch.jit.trace(f, (t,), check_trace=False).graph)
+        except (RuntimeError, ValueError, ArgumentError):
+            continue
+        assert "Fn" in graph

@@ -833,3 +833,26 @@ def test_norm_rope_far_positions(inter):
     t = torch.tensor([[_turns(int(p), i, rd, 10000) for i in range(rd // 2)] for p in pos], dtype=torch.float64) * (2 * math.pi)
     for got, want in ((lo, t.cos() - t.sin()), (hi, t.cos() + t.sin())):
         assert (got - want).abs().max() <= 9 * 2.0 ** -24
+
+
+def test_forward_mode_and_tracing_are_not_silent():
+    """the operators have no forward-mode derivative: inputs with a tangent raise, in every one of them, instead of giving a result without
+    its tangent; a traced call is recorded, or raises where the sizes it traces are no numbers"""
+    import torch.autograd.forward_ad as fw
+    from ctypes import ArgumentError
+    q, k, v, g = make(1, 5, 6, 2, 2, 32, BF)
+    table, w = torch.randn(32, 2, device=DEV), torch.ones(32, device=DEV)
+    calls = [(lambda t: S.cross_attention(t, k, v), q), (lambda t: S.cross_attention(q, k, t), v), (lambda t: S.cross_attention(q, k, v, rel_table=t), table),
+             (lambda t: S.relative_position_bias(t, 4, 4), table), (lambda t: S.qk_norm_rope(t, k)[0], q), (lambda t: S.qk_norm_rope(q, k, w_k=t)[1], w)]
+    for f, t in calls:
+        want = f(t)
+        with fw.dual_level():
+            assert torch.equal(f(t), want)           # (nothing here has a tangent)
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
+                    f(fw.make_dual(t, torch.ones_like(t)))
+        try:
+            graph = str(torch.jit.trace(f, (t,), check_trace=False).graph)
+        except (RuntimeError, ValueError, ArgumentError):
+            continue
+        assert "Fn" in graph
