@@ -348,6 +348,9 @@ static inline bool sa_desc_ok(const dfold_seq_attn_desc* d) {
   const int64_t st[12] = {d->q_sb, d->q_sl, d->q_sh, d->k_sb, d->k_sl, d->k_sh, d->v_sb, d->v_sl, d->v_sh, d->o_sb, d->o_sl, d->o_sh};
   for (int i = 0; i < 12; ++i)
     if (st[i] % 8 || st[i] < 0) return false;
-  if (d->q_sl >= SA_MAX_ROW || d->k_sl >= SA_MAX_ROW || d->v_sl >= SA_MAX_ROW || !(d->scale != 0.f)) return false;
+  if (d->q_sl >= SA_MAX_ROW || d->k_sl >= SA_MAX_ROW || d->v_sl >= SA_MAX_ROW) return false;
+  // scale, scale x log2 e and the forward's threshold 8 / (scale x log2 e) are normal fp32 numbers
+  const float sc = d->scale < 0.f ? -d->scale : d->scale;
+  if (!(sc >= 0x1p-120f && sc <= 0x1p120f)) return false;
   return d->mask_sb >= 0;
 }

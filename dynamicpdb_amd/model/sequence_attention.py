@@ -30,6 +30,7 @@ F16, F32 = torch.float16, torch.float32
 DTYPES = {BF16: 0, F16: 1, F32: 2}                                    # DFOLD_DT_*
 REL_FAR, REL_MAX_DISTANCE = 256, 1024                                 # DFOLD_REL_*
 MAX_OFFSET, MAX_LEN, MAX_ROW = 1 << 29, 1 << 30, 1 << 24
+MIN_SCALE = 2.0 ** -120                                               # what the kernels form of a scale stays a normal fp32 number
 ROWS, TILE = 128, 64                                                  # softmax rows / keys of a workgroup, rows of an LDS tile
 
 # The C ABI's descriptors as struct formats: one pack per call (filling ctypes structures field by field costs as much host time as the
@@ -539,7 +540,8 @@ def cross_attention(q, k, v, *, key_mask=None, kv_lens=None, rel_table=None, max
     key_mask [B, Lk] (bool, or 0 / 1 in any type) and kv_lens [B] (int32 / int64: keys j < kv_lens[b] exist) remove keys: what K and V
     hold there is never used, gradients there are zero.  A query without any key gives zeros and takes no gradient.  rel_table fp32
     [num_buckets, H] adds the bias of relative_position_bias without forming it; q_offset: position of query 0 minus position of key 0, a
-    whole number or an int32 / int64 tensor [B] (one token at its own position per sequence).  scale defaults to D^-1/2.
+    whole number or an int32 / int64 tensor [B] (one token at its own position per sequence).  scale defaults to D^-1/2 (2^-120 to 2^120
+    in magnitude, either sign).
     Differentiable (once) in q, k, v and rel_table; repeated calls give the same bits.  P and dS are rounded to the operand type between
     the products (an fp16 dS beyond 65504 in units of a power of two that holds it: only the gradients themselves have to fit the type)."""
     dt, dev = q.dtype, q.get_device()
@@ -588,8 +590,8 @@ def cross_attention(q, k, v, *, key_mask=None, kv_lens=None, rel_table=None, max
     else:
         q_offset = 0
     scale = D ** -0.5 if scale is None else float(scale)
-    if not 0 < abs(scale) < math.inf:
-        raise ValueError("scale must be finite and not 0")
+    if not MIN_SCALE <= abs(scale) <= 1 / MIN_SCALE:
+        raise ValueError("scale must be between 2^-120 and 2^120 in magnitude")
     _require_cuda(q)
     args = (q, k, v, rel_table, key_mask, kv_lens, q_offsets, q_offset, max_distance, bool(bidirectional), scale)
     if _needs_node(q.requires_grad or k.requires_grad or v.requires_grad or (rel_table is not None and rel_table.requires_grad)):

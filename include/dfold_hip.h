@@ -642,6 +642,7 @@ int dfold_relpos_ws(int32_t H, int32_t Lq, int32_t num_buckets);
  *   row without keys), and 1 / the row's sum of exp2(logits x log2 e - mu) (0 for such a row).
  *   splits > 1: the keys are cut into that many parts; ws: splits * B * H * Lq * (D + 2) floats.
  *   pack = 1, or H / Hkv (rows of the query heads of a group share tiles: few queries).
+ *   scale: 2^-120 to 2^120 in magnitude, either sign.
  *   pair = 1: two waves per 32 rows, one per half of a key tile (launches that leave SIMDs idle); 0: one.  Any value is right. */
 typedef struct {
   const void *q, *k, *v;

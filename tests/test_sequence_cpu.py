@@ -232,3 +232,16 @@ def test_forward_mode_and_tracing_are_not_silent(monkeypatch):
         except (RuntimeError, ValueError, ArgumentError):
             continue
         assert "Fn" in graph
+
+
+@pytest.mark.parametrize("scale", [1e39, -1e39, 1e-50, 1e-39, 2.0 ** -121, 2.0 ** 121, float("inf"), 0.0])
+def test_cross_attention_refuses_scales_outside_fp32(scale):
+    """the kernels hold the scale, its product with log2 e and the inverse of that in fp32: none of them may leave its normal range"""
+    with pytest.raises(ValueError):
+        S.cross_attention(*_qkv(), scale=scale)
+    from dynamicpdb_amd import _lib
+    if abs(scale) < 1e38:
+        d = S.AttnDesc()
+        d.q = d.k = d.v = d.o = 16
+        d.B, d.Lq, d.Lk, d.H, d.Hkv, d.D, d.splits, d.pack, d.scale = 1, 4, 4, 4, 2, 64, 1, 1, scale
+        assert _lib.lib().dfold_seq_attn_fwd(byref(d), c_void_p(0)) == -1
