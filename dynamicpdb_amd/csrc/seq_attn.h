@@ -62,6 +62,18 @@ __device__ __forceinline__ float sa_xsum(float v) {
 }
 __device__ __forceinline__ float sa_exp2(float v) { return __builtin_amdgcn_exp2f(v); }
 
+// A row's softmax is two numbers: the reference mu of its exponents (log2 units, as rounded where it is subtracted) and the sum l of exp2(logit - mu).
+// One fp32, mu + log2(l), would lose l where |mu| is large (rows of nothing but keys whose bias is -1e9).  Up to SA_WIDE the sum of the two is right to
+// 2^-16, and the backward subtracts it at once; beyond, it subtracts one after the other.
+#define SA_WIDE 256.f
+// Without a bias the exponent is fma(s, sl2, -mu) for mu = m sl2 as rounded.  The exact product differs from a rounded one by up to half a step of mu: a
+// factor common to the row, but a step is 2 from 2^24 on, and the factor leaves fp32 at 2^31 (f16 P at 2^28).  Rows beyond 2^24 round the product as
+// the reference was, forward and backward alike.
+#define SA_HUGE 0x1p24f
+__device__ __forceinline__ float sa_exponent(float s, float sl2, float mu) {
+  return fabsf(mu) >= SA_HUGE ? s * sl2 - mu : __builtin_fmaf(s, sl2, -mu);
+}
+
 // workgroup id -> work id: blockIdx round-robins over the 8 XCDs, consecutive work ids (which share K and V) stay on one of them
 __device__ __forceinline__ unsigned sa_work_id() {
   const unsigned nwg = gridDim.x, bid = blockIdx.x;

@@ -1,14 +1,13 @@
-// Attention of one sequence over another, backward.  With P = exp2(logit - mu) / l from the forward's two numbers of a row, dP = dO V^T and
+// Attention of one sequence over another, backward.  With P = exp2(logit - the row's numbers of the forward), dP = dO V^T and
 // delta = rowsum(dO O) = rowsum(P dP):   dS = P (dP - delta),  dV = P^T dO,  dK = scale dS^T Q,  dQ = scale dS K,
 // dtable[bucket] = sum of dS over the bucket's diagonals.
 //
 // Two passes, each recomputing S and dP (7 products instead of 5) rather than adding to one of the gradients with atomics: results do
 // not depend on the order of workgroups.
-//   * dQ pass: the forward's walk (128 rows, key tiles of 64).  S^T and dP^T have the softmax rows as columns, so the row's mu
-//     and delta are one register each, and l dS^T = exp2(logit - mu) (dP - delta) is at once the B operand of l dQ^T = K^T (l dS^T);
-//     dQ is divided by l when it is stored.  delta = dO O comes from the lane's own operand of dO and the stored O, whose two roundings
-//     (P's and its own) it inherits; exact arithmetic makes a row of dS sum to zero, so the row sum that is left, taken in fp32, is what
-//     delta lacks: delta + that sum goes to the second pass.
+//   * dQ pass: the forward's walk (128 rows, key tiles of 64).  S^T and dP^T have the softmax rows as columns, so the row's log-sum
+//     and delta are one register each, and dS^T is at once the B operand of dQ^T = K^T dS^T.  delta = dO O comes from the lane's own
+//     operand of dO and the stored O, whose two roundings (P's and its own) it inherits; exact arithmetic makes a row of dS sum to
+//     zero, so the row sum that is left, taken in fp32, is what delta lacks: delta + that sum goes to the second pass.
 //   * dK, dV pass: 128 keys per workgroup, K^T and V^T operands in registers, query tiles of 64 of all heads of the group in LDS:
 //     the sum over shared heads is the accumulator's.  The bias gradient (an fp32 result) is formed here, from fp32 dS with the
 //     corrected delta.
@@ -35,24 +34,32 @@ struct SaBwdParams {
   SaRel rel;
 };
 
-// logits x log2 e, rounded as in the forward, minus the row's reference, of a block whose columns are softmax rows (rows: keys
-// d0 + 8 (r / 4) + r % 4).  (A bias near the type's lowest value absorbs the product in both directions alike.)
+// logits x log2 e minus the row's log-sum (lse, and base where wide: see SA_WIDE) of a block whose columns are softmax rows (rows: keys
+// d0 + 8 (r / 4) + r % 4).  A wide row's logits are rounded as in the forward before its reference goes.
 template <bool REL>
-__device__ __forceinline__ void sa_logits(f32x16& s, float sl2, float mu, const float* myb, int W, int far, float farv, int d0) {
+__device__ __forceinline__ void sa_logits(f32x16& s, float sl2, float lse, float base, bool wide, const float* myb, int W, int far, float farv, int d0) {
   if constexpr (REL) {
-    if (far) {
+    auto near = [&](int r) { return myb[min(max(d0 + 8 * (r >> 2) + (r & 3), -W), W)]; };
+    if (__builtin_expect(wide, 0)) {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], sl2, farv) - mu;
+      for (int r = 0; r < 16; ++r) s[r] = (__builtin_fmaf(s[r], sl2, far ? farv : near(r)) - base) - lse;
+    } else if (far) {
+      const float c = farv - lse;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], sl2, c);
     } else {
 #pragma unroll
-      for (int r = 0; r < 16; ++r) {
-        const int d = d0 + 8 * (r >> 2) + (r & 3);
-        s[r] = __builtin_fmaf(s[r], sl2, myb[min(max(d, -W), W)]) - mu;
-      }
+      for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], sl2, near(r) - lse);
     }
   } else {
+    float mult = sl2;
+    if (__builtin_expect(wide, 0)) {
+      mult = 1.f;
 #pragma unroll
-    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], sl2, -mu);
+      for (int r = 0; r < 16; ++r) s[r] = sa_exponent(s[r], sl2, base);
+    }
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], mult, -lse);
   }
 }
 
@@ -149,7 +156,8 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_dq
   }
   dl = sa_xsum(dl);
   const long rowi = ((long)b * p.H + head) * p.Lq + qi;
-  const float mu = on ? p.lse[rowi] : INFINITY;
+  const float lse = on ? p.lse[rowi] : INFINITY, base = on ? p.lse[(long)p.B * p.H * p.Lq + rowi] : 0.f;
+  const bool wide = __ballot(base != 0.f) != 0;
 
   const char* const kb_ = p.k + ((long)b * p.k_sb + (long)hkv * p.k_sh) * 2;
   const char* const vb_ = p.v + ((long)b * p.v_sb + (long)hkv * p.v_sh) * 2;
@@ -160,7 +168,7 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_dq
 #pragma unroll
     for (int r = 0; r < 16; ++r) dq[i][r] = 0.f;
 
-  float left = 0.f;          // row sum of l dS, like dq a sum of l dS K
+  float left = 0.f;          // row sum of dS
   const SaAddr<DP> ad(lane, half * 32);
   const SaKvTiles<DP, PAIR> kv(kb_, p.k_sl, vb_, p.v_sl, p.D, tid, w);
   const SaLive<NW> keys{mb_, kv_end, t0, t1, w, lane, (unsigned long*)(smem + C::TILES)};
@@ -187,7 +195,7 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_dq
       }
       const int k0 = t * SA_KT + (half + kb) * 32;
       const int far = !REL ? 0 : k0 - qhi >= p.rel.W ? 1 : k0 + 31 - qlo <= -p.rel.W ? -1 : 0;
-      sa_logits<REL>(s, p.sl2, mu, myb, p.rel.W, far, far > 0 ? bR : bL, k0 + 4 * h - qpos);
+      sa_logits<REL>(s, p.sl2, lse, base, wide, myb, p.rel.W, far, far > 0 ? bR : bL, k0 + 4 * h - qpos);
       if (live != ~0ul) {
         const unsigned bits = (unsigned)(live >> ((half + kb) * 32)) >> (4 * h);
 #pragma unroll
@@ -202,7 +210,7 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_dq
       sa_within<DT>(s, dq, [&] {
 #pragma unroll
         for (int c = 0; c < 2; ++c) {
-          sa_u32x4 df;      // l dS in the operand type: relative error up to 2^-8 (bf16) / 2^-11 (f16) of each term of dQ's sum
+          sa_u32x4 df;      // dS in the operand type: relative error up to 2^-8 (bf16) / 2^-11 (f16) of each term of dQ's sum
 #pragma unroll
           for (int e = 0; e < 4; ++e) df[e] = sa_pack2<DT>(s[8 * c + 2 * e], s[8 * c + 2 * e + 1]);
 #pragma unroll
@@ -229,8 +237,6 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_dq
 #pragma unroll
     for (int i = 0; i < NT; ++i) dq[i] += acc[i * 64];
   }
-  const float il = on ? p.lse[(long)p.B * p.H * p.Lq + rowi] : 0.f;
-  left *= il;
   if (on && h == 0) {
     // parts of the key axis: plane 0 holds delta, plane 1 + part the part's row sum (seq_attn_delta_kernel adds them up)
     if (p.splits_q == 1) p.delta[rowi] = dl + left;
@@ -249,7 +255,7 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_dq
         if (d >= p.D) continue;
         float o[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) o[e] = dq[i][g * 4 + e] * il * p.scale;
+        for (int e = 0; e < 4; ++e) o[e] = dq[i][g * 4 + e] * p.scale;
         if (p.splits_q == 1)
           *(uint2*)(p.dq + (r1 * p.D + d) * 2) = (uint2){sa_pack2<DT>(o[0], o[1]), sa_pack2<DT>(o[2], o[3])};
         else
@@ -266,7 +272,7 @@ template <int DP, bool REL, bool PAIR>
 struct SaDkvCfg {
   static constexpr bool VLDS = PAIR && DP == 128;
   static constexpr int WAVES = PAIR ? 2 * SA_WAVES : SA_WAVES;
-  static constexpr int TILES = 4 * SaTile<DP>::BYTES, ROWS = 6 * SA_KT * 4;      // two stages of two tiles; mu, delta and 1 / l of their rows
+  static constexpr int TILES = 4 * SaTile<DP>::BYTES, ROWS = 6 * SA_KT * 4;      // two stages of two tiles; log-sums and deltas of their rows
   static constexpr int LDS = TILES + ROWS + (VLDS ? SA_ROWS * SaTile<DP>::PITCH : 0);
   static int bytes(int W) { return LDS + (REL ? (2 * W + 1 + WAVES * (2 * (W + SA_REACH) + 1 + SA_DIAG)) * 4 : 0); }
 };
@@ -278,7 +284,7 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, (DP == 128 && REL ?
   constexpr int NW = SaDkvCfg<DP, REL, PAIR>::WAVES;
   extern __shared__ __attribute__((aligned(16))) char smem[];
   using C = SaDkvCfg<DP, REL, PAIR>;
-  float* const ldsL = (float*)(smem + C::TILES);                // [stage][mu | delta | 1 / l][SA_KT]
+  float* const ldsL = (float*)(smem + C::TILES);                // [stage][log-sum | delta | its wide part][SA_KT]
   char* const ldsV = smem + C::TILES + C::ROWS;
   float* const ldsB = (float*)(smem + C::LDS);
   float* const ldsH = ldsB + (REL ? 2 * p.rel.W + 1 : 0);       // [wave][distance]
@@ -373,7 +379,7 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, (DP == 128 && REL ?
     const int head = hkv * G + fg;
     const long oq = ((long)b * p.q_sb + (long)head * p.q_sh) * 2, og = ((long)b * p.do_sb + (long)head * p.do_sh) * 2;
     qg.load(qg.a + (half ? og : oq), qg.b + og, fq, p.Lq, smem + stage * 2 * T::BYTES);
-    // the rows' mu, delta and 1 / l, a lane each
+    // the rows' log-sums and deltas, a lane each
     const long r = ((long)b * p.H + head) * p.Lq + min(fq + lane, p.Lq - 1);
     float* const ll = ldsL + stage * 3 * SA_KT;
     if (w == 0) __builtin_amdgcn_global_load_lds((const void*)(p.lse + r), (sa_lds_ptr)ll, 4, 0, 0);
@@ -402,6 +408,7 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, (DP == 128 && REL ?
       sa_lds_barrier();
     }
     if (!wave_on) return;
+    const bool wide = __ballot(ll[2 * SA_KT + lane] != 0.f) != 0;
 #pragma unroll
     for (int qb = 0; qb < (PAIR ? 1 : 2); ++qb) {
       const int qs = (PAIR ? half : qb) * 32;
@@ -427,17 +434,25 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, (DP == 128 && REL ?
           for (int r = 0; r < 16; ++r) s[r] = __builtin_fmaf(s[r], p.sl2, myb[min(max(d0 - 8 * (r >> 2) - (r & 3), -p.rel.W), p.rel.W)]);
         }
       }
+      float mult = p.sl2;
+      if (__builtin_expect(wide, 0)) {
+        mult = 1.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float base = ll[2 * SA_KT + qs + 8 * (r >> 2) + 4 * h + (r & 3)];
+          s[r] = REL ? s[r] - base : sa_exponent(s[r], p.sl2, base);
+        }
+      }
 #pragma unroll
       for (int g = 0; g < 4; ++g) {
         const f32x4 rl = *(const f32x4*)(ll + qs + g * 8 + h * 4);
         const f32x4 rd = *(const f32x4*)(ll + SA_KT + qs + g * 8 + h * 4);
-        const f32x4 ri = *(const f32x4*)(ll + 2 * SA_KT + qs + g * 8 + h * 4);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int r = g * 4 + e;
           // a masked key's column holds products with zeros: whatever comes of them stays in that column, which is not stored (only the
           // bias gradient sums over columns)
-          const float x = sa_exp2(REL ? s[r] - rl[e] : __builtin_fmaf(s[r], p.sl2, -rl[e])) * ri[e];
+          const float x = sa_exp2(REL ? s[r] - rl[e] : __builtin_fmaf(s[r], mult, -rl[e]));
           s[r] = REL ? (key_on ? x : 0.f) : x;
           dp[r] = s[r] * (dp[r] - rd[e]);
         }

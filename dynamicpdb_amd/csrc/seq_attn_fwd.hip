@@ -1,9 +1,7 @@
 // Attention of one sequence over another, forward:  o = softmax(scale q k^T + bias) v  per head, one pass over the keys with the
 // running maximum and sum of the softmax.
 //
-// What is kept of a row are two numbers, the reference mu of its exponents (log2 units, as rounded where it is subtracted) and the sum l of
-// exp2(logit - mu): one, mu + log2(l), would lose l wherever |mu| is large (a row of nothing but keys whose bias is -1e9: the sum of n ones
-// drops out).  Parts and pairs meet with weights exp2(mu_part - mu) l_part, the backward takes P = exp2(logit - mu) / l.
+// Parts of the keys and pairs of waves meet by their references and sums: weights exp2(mu_part - mu) l_part.
 //
 // A workgroup owns 128 softmax rows of one key head (4 waves x 32 rows; with pack > 1 the rows of the query heads of a group are
 // interleaved, head fastest, so that one token of a grouped layer fills its tile), walks its part of the keys in tiles of 64 and
@@ -32,11 +30,12 @@ struct SaFwdParams {
 #define SA_LAZY 8.f
 #define SA_MAX_SPLITS 1024
 
-// a row's statistics for the backward: plane 0 the reference of its exponents (+inf: no keys), plane 1 the inverse of their sum
-__device__ __forceinline__ void sa_row_stat(const SaFwdParams& p, int b, int head, int qi, float mu, float inv) {
+// a row for the backward, planes of lse: P = exp2(logit - plane 1 - plane 0).  any: the row has keys
+__device__ __forceinline__ void sa_row_stat(const SaFwdParams& p, int b, int head, int qi, bool any, float mu, float l) {
   float* const st = p.lse + ((long)b * p.H + head) * p.Lq + qi;
-  st[0] = mu;
-  st[(long)p.B * p.H * p.Lq] = inv;
+  const bool wide = any && fabsf(mu) >= SA_WIDE;
+  st[0] = any ? (wide ? 0.f : mu) + __log2f(l) : INFINITY;
+  st[(long)p.B * p.H * p.Lq] = wide ? mu : 0.f;
 }
 
 // PAIR: eight waves, two for the same 32 rows, one per half of a key tile, joined in LDS at the end: a launch of at most one workgroup
@@ -177,12 +176,18 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_fw
         for (int r = 0; r < 16; ++r) O[i][r] *= a;
     }
     const float nm = m == -INFINITY ? 0.f : -m * us;
+    float mult = sl2;
+    if (!REL && __builtin_expect(__ballot(fabsf(nm) >= SA_HUGE) != 0, 0)) {
+      mult = 1.f;
+#pragma unroll
+      for (int kb = 0; kb < NB; ++kb) s[kb] *= sl2;
+    }
     sa_u32x4 pf[2 * NB];
 #pragma unroll
     for (int kb = 0; kb < NB; ++kb) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) {
-        s[kb][r] = sa_exp2(REL ? s[kb][r] + nm : __builtin_fmaf(s[kb][r], sl2, nm));
+        s[kb][r] = sa_exp2(REL ? s[kb][r] + nm : __builtin_fmaf(s[kb][r], mult, nm));
         l += s[kb][r];
       }
 #pragma unroll
@@ -228,7 +233,7 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_fw
   if (!on) return;
   const int head = head0 + hl;
   if (p.splits == 1) {
-    if (p.lse && h == 0) sa_row_stat(p, b, head, qi, any ? m * us : INFINITY, inv);
+    if (p.lse && h == 0) sa_row_stat(p, b, head, qi, any, m * us, l);
     char* const dst = p.o + ((long)b * p.o_sb + (long)qi * p.o_sl + (long)head * p.o_sh) * 2;
 #pragma unroll
     for (int i = 0; i < NT; ++i)
@@ -285,7 +290,7 @@ __global__ __launch_bounds__(256) void seq_attn_combine_kernel(const SaFwdParams
   const int head = (int)(r % p.H);
   const long bq = r / p.H;
   const int qi = (int)(bq % p.Lq), b = (int)(bq / p.Lq);
-  if (p.lse && c == 0) sa_row_stat(p, b, head, qi, l > 0.f || l != l ? m : INFINITY, inv);
+  if (p.lse && c == 0) sa_row_stat(p, b, head, qi, l > 0.f || l != l, m, l);
   sa_u32x4 u;
 #pragma unroll
   for (int e = 0; e < 4; ++e) u[e] = sa_pack2<DT>(o[2 * e] * inv, o[2 * e + 1] * inv);
@@ -331,7 +336,7 @@ __global__ __launch_bounds__(256) void seq_attn_combine_row_kernel(const SaFwdPa
   const int head = (int)(r % p.H);
   const long bq = r / p.H;
   const int qi = (int)(bq % p.Lq), b = (int)(bq / p.Lq);
-  if (p.lse && tid == 0) sa_row_stat(p, b, head, qi, l > 0.f || l != l ? m : INFINITY, inv);
+  if (p.lse && tid == 0) sa_row_stat(p, b, head, qi, l > 0.f || l != l, m, l);
   *(uint2*)(p.o + ((long)b * p.o_sb + (long)qi * p.o_sl + (long)head * p.o_sh + tid * 4) * 2) =
       (uint2){sa_pack2<DT>(o[0] * inv, o[1] * inv), sa_pack2<DT>(o[2] * inv, o[3] * inv)};
 }

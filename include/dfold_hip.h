@@ -638,8 +638,8 @@ int dfold_relpos_ws(int32_t H, int32_t Lq, int32_t num_buckets);
  * strides in elements, multiples of 8, row strides (*_sl) below 2^24, base pointers 16-byte aligned; D a multiple of 8, <= 128; H a multiple of Hkv (query head h
  * reads key head h / (H / Hkv)).  Keys j >= kv_lens[b] and keys with key_mask[b * mask_sb + j] == 0 do not exist: their K and V
  * are never used (they may hold NaN); a row without any key gives zeros.
- *   lse [2][B][H][Lq] fp32 (optional): what the backward needs of a row -- a reference mu near the maximum of its logits x log2 e (+inf for a
- *   row without keys), and 1 / the row's sum of exp2(logits x log2 e - mu) (0 for such a row).
+ *   lse [2][B][H][Lq] fp32 (optional): log2 of a row's sum of exp2(logits x log2 e) as the sum of two numbers; plane 1 is 0 where one fp32 holds
+ *   it well, else a reference near the row's maximum; plane 0 is +inf for a row without keys.
  *   splits > 1: the keys are cut into that many parts; ws: splits * B * H * Lq * (D + 2) floats.
  *   pack = 1, or H / Hkv (rows of the query heads of a group share tiles: few queries).
  *   scale: 2^-120 to 2^120 in magnitude, either sign.

@@ -856,3 +856,64 @@ def test_forward_mode_and_tracing_are_not_silent():
         except (RuntimeError, ValueError, ArgumentError):
             continue
         assert "Fn" in graph
+
+
+@pytest.mark.parametrize("scale", [2.0 ** -120, -(2.0 ** -60), 2.0 ** 120])
+@pytest.mark.parametrize("rel", [False, True])
+def test_attention_extreme_scales(scale, rel):
+    """the smallest scales: uniform rows (or the bias' own softmax); the largest: one key per row, the others' logits far below"""
+    B, Lq, Lk, H, Hkv, D = 1, 70, 90, 4, 2, 32
+    q, k, v, g = make(B, Lq, Lk, H, Hkv, D, BF, seed=4)
+    live, kw = make_mask("keys", B, Lk)
+    table = torch.randn(32, H, device=DEV) if rel else None
+    if scale > 1:                                # gradients would be rounding errors of 0 times 2^120
+        o = S.cross_attention(q, k, v, rel_table=table, scale=scale, **kw)
+        s = (q.double().transpose(1, 2).cpu() @ k.double().repeat_interleave(H // Hkv, 2).permute(0, 2, 3, 1).contiguous().cpu()).masked_fill(~live.cpu()[:, None, None], -math.inf)
+        best = s.argmax(-1)[..., None].expand(B, H, Lq, D)
+        assert torch.equal(o.cpu(), v.repeat_interleave(H // Hkv, 2).transpose(1, 2).cpu().gather(2, best).transpose(1, 2))
+        return
+    got = run(q, k, v, g, table, scale=scale, **kw)
+    ref = reference(q, k, v, g, live, table, bucket_matrix(Lq, Lk, 32, 128, True, 0) if rel else None, scale)
+    for n in ref:
+        within(n, got[n], ref[n])
+
+
+@pytest.mark.parametrize("dt,big", [(BF, 2.0 ** 17), (BF, 2.0 ** 13), (BF, 2.0 ** 9), (BF, 16.0), (HF, 2.0 ** 15), (HF, 64.0)])
+@pytest.mark.parametrize("B,Lq,Lk,H,Hkv,D", [(1, 3, 700, 2, 1, 64), (1, 130, 300, 2, 2, 32), (2, 40, 500, 2, 1, 128)])
+def test_attention_rows_of_huge_logits(B, Lq, Lk, H, Hkv, D, dt, big):
+    """logits of 2^8 to 2^34 on the even rows (half a step of fp32 is up to 2^10 in the exponent there), ordinary ones on the odd rows"""
+    q, k, v, g = make(B, Lq, Lk, H, Hkv, D, dt, seed=13)
+    q[:, ::2] = 0
+    q[:, ::2, :, 0], q[:, 1::2, :, 0], k[..., 0] = big, 0.0, big
+    live, kw = make_mask("lens", B, Lk, seed=2)
+    # (scale 1 would give the odd rows logits of sqrt(D) x randn: fine, |logit| < 64)
+    ref = reference(q, k, v, g, live, None, None, 1.0)
+    for parts, pair in ((1, 0), (1, 1), (3, 1), (7, 0)):
+        with forms(parts, pair):
+            got = run(q, k, v, g, scale=1.0, **kw)
+        for n in ref:
+            within(f"{n} in {parts} parts", got[n], ref[n])
+
+
+@pytest.mark.parametrize("rel", [False, True])
+@pytest.mark.parametrize("B,Lq,Lk,H,Hkv,D,dt", [(1, 130, 300, 2, 1, 32, BF), (2, 70, 200, 2, 2, 64, HF), (1, 200, 150, 4, 2, 128, BF), (1, 5, 2000, 2, 1, 128, HF)])
+def test_attention_steep_rows(B, Lq, Lk, H, Hkv, D, dt, rel, monkeypatch):
+    """logits of some hundreds, rows on both sides of the size from which their statistics are kept apart.  E of the bounds is that of |logit| < 64: it
+    grows with the logits"""
+    import sys
+    q, k, v, g = make(B, Lq, Lk, H, Hkv, D, dt, seed=14)
+    live, kw = make_mask("keys", B, Lk)
+    scale = 60.0 / D ** 0.5
+    top = ((q.double().transpose(1, 2).cpu() @ k.double().repeat_interleave(H // Hkv, 2).permute(0, 2, 3, 1).contiguous().cpu()) * scale).masked_fill(~live.cpu()[:, None, None], -math.inf)
+    assert top.amax(-1).min() < 177 < top.amax(-1).max() < 512
+    monkeypatch.setattr(sys.modules[__name__], "E", 8 * E)
+    table = buckets = None
+    if rel:
+        table = torch.randn(32, H, device=DEV, generator=torch.Generator(device=DEV).manual_seed(1))
+        buckets = bucket_matrix(Lq, Lk, 32, 128, True, 0)
+    ref = reference(q, k, v, g, live, table, buckets, scale)
+    for parts, pair in ((1, 0), (1, 1), (3, 1)):
+        with forms(parts, pair):
+            got = run(q, k, v, g, table, scale=scale, **kw)
+        for n in ref:
+            within(f"{n} in {parts} parts", got[n], ref[n])
