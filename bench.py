@@ -778,9 +778,11 @@ def main():
     torch.cuda.set_device(local)
     dev = torch.device("cuda", local)
     import __graft_entry__
-    from dynamicpdb_amd import _lib
-    if rank == 0 and not os.path.exists(_lib.LIB_PATH):
-        __graft_entry__.build()
+    from dynamicpdb_amd import _lib, build_ext
+    if rank == 0:
+        if not os.path.exists(_lib.LIB_PATH):
+            __graft_entry__.build()
+        build_ext.require_current()
     if world > 1:
         dist.barrier()
     from dynamicpdb_amd import experiment, synthetic

@@ -15,6 +15,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 INCLUDE = os.path.join(HERE, "..", "include")
 LIB = os.path.join(CSRC, "libdfold_hip.so")
+STAMP = os.path.join(CSRC, ".build_stamp")      # digest of what LIB was built from
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-ffp-contract=off", "-Wno-unused-result",
          # the 2x5-tile GEMM epilogue must unroll completely (160 accumulator registers indexed statically), else the
@@ -52,10 +53,21 @@ def _digest(srcs=None):
     return h.hexdigest()
 
 
+def _remove(path):
+    if os.path.exists(path):
+        os.remove(path)
+
+
+def require_current():
+    """Raises if the in-tree library was built from other sources, headers or flags than lie beside it: an edited kernel must not run, or be
+    timed, as the binary from before the edit.  (Compiles nothing; a library without a stamp is taken as it is.)"""
+    if os.path.exists(LIB) and os.path.exists(STAMP) and open(STAMP).read() != _digest():
+        raise RuntimeError(f"{LIB} was built from other sources than are here: rebuild with `python -m dynamicpdb_amd.build_ext`")
+
+
 def build(force=False, verbose=True):
-    stamp = os.path.join(CSRC, ".build_stamp")
     dig = _digest()
-    if not force and os.path.exists(LIB) and os.path.exists(stamp) and open(stamp).read() == dig:
+    if not force and os.path.exists(LIB) and os.path.exists(STAMP) and open(STAMP).read() == dig:
         return LIB
     objdir = os.path.join(CSRC, "build")
     os.makedirs(objdir, exist_ok=True)
@@ -65,6 +77,7 @@ def build(force=False, verbose=True):
         obj_stamp, obj_dig = obj + ".stamp", _digest([src])
         if not force and os.path.exists(obj) and os.path.exists(obj_stamp) and open(obj_stamp).read() == obj_dig:
             return obj                              # (an object whose source, headers and flags have not changed)
+        _remove(obj_stamp)                          # (a compile that is cut short leaves no object that looks finished)
         cmd = [HIPCC] + FLAGS + ["-I", INCLUDE, "-c", os.path.join(CSRC, src), "-o", obj]
         r = subprocess.run(cmd, capture_output=True, text=True)
         if r.returncode != 0:
@@ -75,11 +88,12 @@ def build(force=False, verbose=True):
 
     with ThreadPoolExecutor(max_workers=8) as ex:
         objs = list(ex.map(cc, sources()))
+    _remove(STAMP)
     cmd = [HIPCC, "--offload-arch=gfx950", "-shared", "-fPIC", "-o", LIB] + objs
     r = subprocess.run(cmd, capture_output=True, text=True)
     if r.returncode != 0:
         raise RuntimeError(f"link failed:\n{r.stderr}")
-    with open(stamp, "w") as fh:
+    with open(STAMP, "w") as fh:
         fh.write(dig)
     if verbose:
         print(f"built {LIB} from {len(objs)} sources")
