@@ -127,8 +127,8 @@ struct SaAddr {
 
 // SA_KT (or ROWS) rows of a [rows][D] matrix with row stride `rs` elements (< SA_MAX_ROW) into an LDS tile, by LDS-DMA: no registers and
 // no LDS write instructions.  A wave's instruction fills 1 KB of the tile in lane order, so the chunk permutation is applied to the
-// source.  Rows past the last one repeat it (never out of range; their content is masked by the caller), columns past D repeat
-// column 0: they meet zeros of the other operand, or results that are not stored, or zero_columns() clears them.
+// source.  Rows past the last one repeat it (never out of range; their content is masked by the caller).  Lanes whose chunk lies past D load
+// nothing: zero_columns() clears their places once, and they stay zeros under every tile that follows.
 #define SA_MAX_ROW (1 << 24)
 typedef __attribute__((address_space(3))) void* sa_lds_ptr;
 template <int DP, int NW = SA_WAVES, int ROWS = SA_KT>
@@ -137,12 +137,15 @@ struct SaDma {
   static constexpr int NCH = ROWS * T::CPR / (64 * NW);    // instructions per wave
   static constexpr int STEP = 64 * NW / T::CPR;            // rows between a lane's chunks (a multiple of 16: one permutation key)
   static_assert(NCH >= 1 && STEP % 16 == 0, "whole instructions, one key per lane");
-  int row, col;
+  int row, col, plain;     // plain: rows from which a tile is loaded without a test
+  bool in;                 // the lane's columns are below D
   unsigned rs2, voff;      // bytes of a row, of this lane's first chunk
   __device__ __forceinline__ SaDma(long rs, int D, int tid) {
     row = tid / T::CPR;
     const int cc = (tid % T::CPR) ^ T::key(row);
-    col = cc * 8 < D ? cc * 16 : 0;
+    in = cc * 8 < D;
+    col = cc * 16;
+    plain = D == DP ? ROWS : INT32_MAX;
     rs2 = (unsigned)rs * 2u;
     voff = row * rs2 + col;
   }
@@ -150,20 +153,19 @@ struct SaDma {
   __device__ __forceinline__ void load(const char* base, int row0, int end, char* tile, int w) const {
     const char* const src = base + (long)row0 * rs2;
     const int last = end - 1 - row0;
-    if (last >= ROWS - 1) {
+    if (last + 1 >= plain) {
 #pragma unroll
       for (int i = 0; i < NCH; ++i)
         __builtin_amdgcn_global_load_lds((const void*)(src + (long)(i * STEP) * rs2 + voff), (sa_lds_ptr)(tile + (i * NW + w) * 1024), 16, 0, 0);
-    } else {
+    } else if (in) {
 #pragma unroll
       for (int i = 0; i < NCH; ++i)
         __builtin_amdgcn_global_load_lds((const void*)(src + (min(row + i * STEP, last) * rs2 + col)), (sa_lds_ptr)(tile + (i * NW + w) * 1024), 16, 0, 0);
     }
   }
-  // columns past D of what this wave loaded become zeros (its loads have landed by then; a barrier before others read)
-  __device__ __forceinline__ void zero_columns(int D, char* tile, int tid) const {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if ((((tid % T::CPR) ^ T::key(row)) * 8) < D) return;
+  // columns past D of this lane's share of a tile become zeros (before the first load's barrier)
+  __device__ __forceinline__ void zero_columns(char* tile, int tid) const {
+    if (in) return;
 #pragma unroll
     for (int i = 0; i < NCH; ++i) *(sa_u32x4*)(tile + (i * 64 * NW + tid) * 16) = (sa_u32x4){0u, 0u, 0u, 0u};
   }
@@ -197,6 +199,15 @@ struct SaKvTiles {
   __device__ __forceinline__ void load(const char* sa, const char* sb, int row0, int end, char* tile) const {
     la.load(sa, row0, end, tile + (PAIR ? half * T::BYTES : 0), w);
     if constexpr (!PAIR) lb.load(sb, row0, end, tile + T::BYTES, w);
+  }
+  // columns past D of both stages at `tiles`
+  __device__ __forceinline__ void zero_columns(int D, char* tiles) const {
+    if (D == DP) return;
+#pragma unroll
+    for (int stage = 0; stage < 2; ++stage) {
+      la.zero_columns(tiles + (2 * stage + (PAIR ? half : 0)) * T::BYTES, tid);
+      if constexpr (!PAIR) lb.zero_columns(tiles + (2 * stage + 1) * T::BYTES, tid);
+    }
   }
   __device__ __forceinline__ void zero(unsigned long live, char* tile) const {
     la.zero(live, tile + (PAIR ? half * T::BYTES : 0), tid);

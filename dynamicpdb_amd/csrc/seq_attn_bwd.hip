@@ -219,6 +219,7 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_dq
       });
     }
   };
+  kv.zero_columns(p.D, smem);
   sa_walk(t0, t1, fetch, step);
 
   left = sa_xsum(left);
@@ -328,7 +329,7 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, (DP == 128 && REL ?
     if (u0 < u1) {
       const SaDma<DP, NW, SA_ROWS> ldv(p.v_sl, p.D, tid);
       ldv.load(p.v + ((long)b * p.v_sb + (long)hkv * p.v_sh) * 2, kbk * SA_ROWS, kv_end, ldsV, w);
-      if (p.D < DP) ldv.zero_columns(p.D, ldsV, tid);      // both operands of dP come from LDS: one of them holds zeros past D
+      ldv.zero_columns(ldsV, tid);
     }
   f32x16 dk[NT], dv[NT];
 #pragma unroll
@@ -498,6 +499,7 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, (DP == 128 && REL ?
       });
     }
   };
+  qg.zero_columns(p.D, smem);
   sa_walk(u0, u1, fetch, step);
 
   if constexpr (REL)

@@ -200,6 +200,7 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_fw
 #pragma unroll
       for (int i = 0; i < NT; ++i) O[i] = sa_mfma<DT>(ad.cols(lv, c * 16, i), pf[c], O[i]);
   };
+  kv.zero_columns(p.D, smem);
   sa_walk(t0, t1, fetch, step);
 
   l = sa_xsum(l);

@@ -1008,3 +1008,49 @@ def test_attention_long_offset_many_heads_of_a_group():
     q, k, v, g = make(1, 498, 1106, 28, 4, 32, HF)
     table = torch.randn(128, 28, device=DEV)
     run(q, k, v, g, table, max_distance=173, q_offset=1199)
+
+
+@pytest.mark.parametrize("D", [8, 24, 32, 40, 64, 72, 96, 120, 128])
+@pytest.mark.parametrize("rel", [False, True])
+def test_attention_keys_of_infinite_logits(D, rel):
+    """keys whose logits are -inf because K is infinite (no mask): as if they were masked, at every head size; rows of +inf or NaN logits are NaN,
+    the other rows are not"""
+    B, Lq, Lk, H, Hkv = 1, 45, 150, 4, 2
+    q, k, v, _ = make(B, Lq, Lk, H, Hkv, D, BF, seed=15)
+    q[..., 0] = -q[..., 0].abs() - 0.5
+    table = torch.randn(32, H, device=DEV) if rel else None
+    dead = torch.zeros(B, Lk, dtype=torch.bool, device=DEV)
+    dead[:, [0, 70, 149]] = True
+    k2 = k.clone()
+    k2[..., 0] = torch.where(dead[..., None], torch.full_like(k[..., 0], math.inf), k[..., 0])
+    for parts, pair in ((1, 0), (1, 1), (3, 0)):
+        with forms(parts, pair):
+            want = S.cross_attention(q, k, v, rel_table=table, key_mask=~dead)
+            assert torch.equal(S.cross_attention(q, k2, v, rel_table=table), want)
+            q2 = q.clone()
+            q2[:, 3] = -q2[:, 3]                 # +inf on three keys
+            got = S.cross_attention(q2, k2, v, rel_table=table)
+            others = [i for i in range(Lq) if i != 3]
+            assert bool(torch.isnan(got[:, 3]).all()) and bool(torch.isfinite(got[:, others]).all())
+            # (rows of a wave share the moments at which their references move: two independent roundings of P and of the result)
+            assert (got[:, others].double() - want[:, others].double()).abs().max() <= 2 * 2.0 ** -8 * (v.abs().max().double() * 2)
+
+
+@pytest.mark.parametrize("D", [32, 40, 96, 128])
+@pytest.mark.parametrize("rel", [False, True])
+def test_attention_masked_places_may_hold_anything_at_every_size(D, rel):
+    """as above, at head sizes whose kernels differ, also where the bias' gradient sums over columns"""
+    B, Lq, Lk, H, Hkv = 3, 70, 300, 4, 2
+    q, k, v, g = make(B, Lq, Lk, H, Hkv, D, BF, seed=16)
+    live, kw = make_mask("both", B, Lk)
+    live[1] = False
+    kw["key_mask"] = live.clone()
+    table = torch.randn(32, H, device=DEV) if rel else None
+    for parts, pair in ((1, 0), (1, 1), (3, 0)):
+        with forms(parts, pair):
+            clean = run(q, k, v, g, table, **kw)
+            k2, v2 = k.clone(), v.clone()
+            k2[~live], v2[~live] = float("nan"), float("inf")
+            k2[0, Lk - 1], v2[0, Lk - 1], k2[:, 70], v2[:, 70] = float("-inf"), float("nan"), float("inf"), float("nan")
+            got = run(q, k2, v2, g, table, **kw)
+            assert all(torch.equal(got[n], clean[n]) for n in got) and all(bool(torch.isfinite(x).all()) for x in got.values())
