@@ -114,8 +114,11 @@ class LinearFn(Function):
         x2d = x.reshape(-1, K)
         if not x2d.is_contiguous():
             x2d = x2d.contiguous()
-        y = ops.linear_fwd(x2d, CACHE.w(weight), bias.detach() if bias is not None else None,
-                           out_dtype=torch.float32 if out_fp32 else BF16, relu=relu)
+        if x2d.shape[0] == 0:                        # no rows: nothing to launch
+            y = torch.empty((0, weight.shape[0]), dtype=torch.float32 if out_fp32 else BF16, device=weight.device)
+        else:
+            y = ops.linear_fwd(x2d, CACHE.w(weight), bias.detach() if bias is not None else None,
+                               out_dtype=torch.float32 if out_fp32 else BF16, relu=relu)
         ctx.save_for_backward(x2d, weight, y if relu else None)
         ctx.has_bias, ctx.xshape = bias is not None, x.shape
         return y.view(*x.shape[:-1], weight.shape[0])
@@ -124,6 +127,9 @@ class LinearFn(Function):
     def backward(ctx, gy):
         x2d, weight, y = ctx.saved_tensors
         N = weight.shape[0]
+        if x2d.shape[0] == 0:
+            dw = torch.zeros(weight.shape, dtype=torch.float32, device=weight.device)
+            return x2d.new_empty(ctx.xshape), dw, dw.new_zeros(N) if ctx.has_bias else None, None, None
         g2d = gy.reshape(-1, N)
         g2d = ops.cast_bf16(g2d) if g2d.dtype == torch.float32 else g2d.contiguous()
         if y is not None:

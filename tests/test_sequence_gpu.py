@@ -1054,3 +1054,17 @@ def test_attention_masked_places_may_hold_anything_at_every_size(D, rel):
             k2[0, Lk - 1], v2[0, Lk - 1], k2[:, 70], v2[:, 70] = float("-inf"), float("nan"), float("inf"), float("nan")
             got = run(q, k2, v2, g, table, **kw)
             assert all(torch.equal(got[n], clean[n]) for n in got) and all(bool(torch.isfinite(x).all()) for x in got.values())
+
+
+def test_module_without_queries_or_context():
+    """empty sequences through the module: no rows, or rows of the output projection's bias; finite gradients"""
+    c, D, H = 64, 32, 4
+    m = S.CrossAttention(c, c, D, H, 2, rotary_dim=32, num_buckets=32).to(DEV)
+    x, ctx = torch.randn(2, 5, c, device=DEV), torch.randn(2, 7, c, device=DEV)
+    none = m(x[:, :0], ctx)
+    assert none.shape == (2, 0, c)
+    y = m(x, ctx[:, :0])
+    assert torch.equal(y, m.linear_o.bias.detach().expand(2, 5, c)) or (y - m.linear_o.bias).abs().max() <= 2.0 ** -8 * m.linear_o.bias.abs().max()
+    for out in (none, y):
+        grads = torch.autograd.grad(out.sum(), list(m.parameters()), allow_unused=True)
+        assert all(g is None or bool(torch.isfinite(g).all()) for g in grads)
