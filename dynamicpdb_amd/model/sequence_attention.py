@@ -31,6 +31,7 @@ DTYPES = {BF16: 0, F16: 1, F32: 2}                                    # DFOLD_DT
 REL_FAR, REL_MAX_DISTANCE = 256, 1024                                 # DFOLD_REL_*
 MAX_OFFSET, MAX_LEN, MAX_ROW = 1 << 29, 1 << 30, 1 << 24
 MIN_SCALE = 2.0 ** -120                                               # what the kernels form of a scale stays a normal fp32 number
+MAX_EPS = torch.finfo(F32).max
 ROWS, TILE = 128, 64                                                  # softmax rows / keys of a workgroup, rows of an LDS tile
 
 # The C ABI's descriptors as struct formats: one pack per call (filling ctypes structures field by field costs as much host time as the
@@ -394,8 +395,8 @@ def qk_norm_rope(q, k, w_q=None, w_k=None, q_positions=None, k_positions=None, *
         rotary_dim = D
     if not isinstance(rotary_dim, int) or not 0 <= rotary_dim <= D or rotary_dim % 16:
         raise ValueError("rotary_dim must be a multiple of 16, at most the head size")
-    if not (0 < base < math.inf and eps >= 0):
-        raise ValueError("base must be positive and eps not negative")
+    if not (0 < base < math.inf and 0 <= eps <= MAX_EPS):
+        raise ValueError("base must be positive and finite, eps not negative and within fp32")
     grad = ref.requires_grad or (k is not None and k.requires_grad)
     if w_q is not None:
         w_q = _head_weight(w_q, D, dev, "w_q")
@@ -625,6 +626,10 @@ class CrossAttention(nn.Module):
     def forward(self, x, context=None, mask=None, kv_lens=None, q_positions=None, k_positions=None, q_offset=0):
         """mask [B, Lk] (1: key exists), kv_lens [B]; positions of the rotation (default 0, 1, ...), q_offset of the bias."""
         _require_cuda(x)
+        with torch.cuda.device(x.device):            # (the projections launch on the current device)
+            return self._attend(x, context, mask, kv_lens, q_positions, k_positions, q_offset)
+
+    def _attend(self, x, context, mask, kv_lens, q_positions, k_positions, q_offset):
         context = x if context is None else context
         B, Lq, Lk, D = x.shape[0], x.shape[1], context.shape[1], self.c_hidden
         q = linear(x.to(BF16), self.linear_q.weight).view(B, Lq, self.no_heads, D)

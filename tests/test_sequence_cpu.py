@@ -245,3 +245,10 @@ def test_cross_attention_refuses_scales_outside_fp32(scale):
         d.q = d.k = d.v = d.o = 16
         d.B, d.Lq, d.Lk, d.H, d.Hkv, d.D, d.splits, d.pack, d.scale = 1, 4, 4, 4, 2, 64, 1, 1, scale
         assert _lib.lib().dfold_seq_attn_fwd(byref(d), c_void_p(0)) == -1
+
+
+@pytest.mark.parametrize("kw", [dict(eps=1e39), dict(eps=math.inf), dict(eps=math.nan), dict(base=math.inf), dict(base=math.nan)])
+def test_qk_norm_rope_refuses_numbers_outside_fp32(kw):
+    q, k, _ = _qkv()
+    with pytest.raises(ValueError):
+        S.qk_norm_rope(q, k, **kw)
