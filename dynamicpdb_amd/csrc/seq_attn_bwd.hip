@@ -14,7 +14,7 @@
 // Bias gradient: 32 x 32 blocks beyond the last border add to one register per side.  A nearer block goes through LDS: rows of dS at a
 // pitch of 64 whose other half stays zero, so that lane t reads the 32 entries of diagonal t - 31 without a test, and adds its sum to
 // the wave's histogram over distances: 16 writes, 32 reads and 32 additions per block, in a fixed order.  (LDS float atomics on the
-// histogram itself: 110 -> 234 cycles per instruction of 64 lanes, the pass five times slower at 1001 x 1001.)
+// histogram itself: 234 cycles per instruction of 64 lanes, the pass 110 us instead of 44 at 4 x 8 x 1001^2.)
 #include "seq_attn.h"
 #include "seq_dtable.h"
 #include <math.h>
@@ -268,7 +268,7 @@ __global__ __launch_bounds__((PAIR ? 2 : 1) * 64 * SA_WAVES, 2) void seq_attn_dq
 // Four waves of 32 keys each, K^T and V^T operands in registers; PAIR: eight waves, two for the same 32 keys, one per 32-query half of
 // a tile; the two sums meet in LDS at the end.  Small launches then have two waves per SIMD.  At D = 128 the four-wave form needs more
 // than 256 registers, one wave per SIMD, and nothing runs under its products: always PAIR there, with V^T operands from LDS (417 -> 303
-// us) -- except with a bias, where the eight waves' blocks of dS would not fit LDS.
+// us) -- except with a bias, where eight waves' blocks of dS of 32 rows do not fit LDS beside the tiles (blocks of 16 rows would: not built).
 template <int DP, bool REL, bool PAIR>
 struct SaDkvCfg {
   static constexpr bool VLDS = PAIR && DP == 128;

@@ -114,10 +114,13 @@ def _rows16(t):
 
 def _strides(t):
     """strides of the three leading axes, 0 for axes of one entry (theirs may be anything, also in a tensor that is dense for torch)"""
-    n, (a, b, c, _) = t.shape, t.stride()
-    if t.numel() == 0:
+    a, b, c, _ = t.stride()
+    n0, n1, n2, _ = t.shape
+    if n0 > 1 and n1 > 1 and n2 > 1:
+        return a, b, c
+    if n1 == 0:
         return 0, 0, 0
-    return a if n[0] > 1 else 0, b if n[1] > 1 else 0, c if n[2] > 1 else 0
+    return a if n0 > 1 else 0, b if n1 > 1 else 0, c if n2 > 1 else 0
 
 
 def _dense_like(t):
@@ -544,7 +547,7 @@ def cross_attention(q, k, v, *, key_mask=None, kv_lens=None, rel_table=None, max
     whole number or an int32 / int64 tensor [B] (one token at its own position per sequence).  scale defaults to D^-1/2 (2^-120 to 2^120
     in magnitude, either sign).
     Differentiable (once) in q, k, v and rel_table; repeated calls give the same bits.  P and dS are rounded to the operand type between
-    the products (an fp16 dS beyond 65504 in units of a power of two that holds it: only the gradients themselves have to fit the type)."""
+    the products (an fp16 dS beyond 65504 in units of a power of two that holds it; one below 2^-25 is 0: scale an fp16 loss)."""
     dt, dev = q.dtype, q.get_device()
     if q.dim() != 4 or k.dim() != 4:
         raise ValueError("q must be [B, Lq, H, D], k and v [B, Lk, Hkv, D]")
