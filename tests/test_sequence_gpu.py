@@ -1068,3 +1068,78 @@ def test_module_without_queries_or_context():
     for out in (none, y):
         grads = torch.autograd.grad(out.sum(), list(m.parameters()), allow_unused=True)
         assert all(g is None or bool(torch.isfinite(g).all()) for g in grads)
+
+
+def test_bias_matrix_past_32_bits():
+    """a matrix of more than 2^31 elements: every head's last rows, and the table's gradient of a sum (whole counts)"""
+    H, Lq, Lk = 3, 30011, 30013
+    table = torch.randn(32, H, device=DEV, requires_grad=True)
+    out = S.relative_position_bias(table, Lq, Lk, dtype=BF)
+    bk = bucket_matrix(40, Lk, 32, 128, True, Lq - 40)[0]
+    for h in range(H):
+        assert torch.equal(out[h, -40:], table.detach()[:, h][bk].to(BF))
+    (dtable,) = torch.autograd.grad(out, table, torch.ones_like(out))
+    d = torch.arange(-(Lq - 1), Lk)
+    n = (torch.clamp(Lk - d, max=Lq) - torch.clamp(-d, min=0)).double()         # rows of a diagonal
+    half = torch.where(d > 0, 16, 0)
+    far = torch.tensor(S.far_borders(32, 128, True))
+    b = half + torch.where(d.abs() < 8, d.abs(), 8 + torch.searchsorted(far, d.abs().contiguous(), right=True))
+    want = torch.zeros(32, dtype=torch.float64).index_add_(0, b, n)
+    assert want.sum() == Lq * Lk
+    # whole numbers up to 2^24 are exact in a block's sums; adding up the blocks rounds once a block, by 2^-24 of the sum at most
+    blocks = 1280 // H
+    assert ((dtable.double().cpu() - want[:, None]).abs() <= blocks * 2.0 ** -24 * want[:, None]).all()
+
+
+def test_attention_over_a_cache_past_32_bits():
+    """K and V of more than 2^31 elements each, forward and gradients: the last keys against a call on them alone"""
+    B, Lq, Lk, H, Hkv, D, n = 1, 5, (1 << 21) + 77, 16, 8, 128, 1000
+    q, kd, vd, g = make(B, Lq, n, H, Hkv, D, BF)
+    k, v = torch.zeros(B, Lk, Hkv, D, dtype=BF, device=DEV), torch.zeros(B, Lk, Hkv, D, dtype=BF, device=DEV)
+    k[:, -n:], v[:, -n:] = kd, vd
+    keep = torch.zeros(B, Lk, dtype=torch.bool, device=DEV)
+    keep[:, -n:] = True
+    got = run(q, k, v, g, key_mask=keep)
+    ref = reference(q, kd, vd, g, torch.ones(B, n, dtype=torch.bool, device=DEV), None, None, D ** -0.5)
+    within("o", got["o"], ref["o"])
+    within("dq", got["dq"], ref["dq"])
+    for name in ("dk", "dv"):
+        within(name, got[name][:, -n:].clone(), ref[name])
+        assert not bool(got[name][:, :-n].any())
+
+
+def test_attention_of_queries_past_32_bits():
+    """Q, O and their gradients of more than 2^31 elements: the last rows against a call on them alone"""
+    B, Lq, Lk, H, Hkv, D, n = 1, 131101, 70, 128, 128, 128, 50
+    gen = torch.Generator(device=DEV).manual_seed(3)
+    k, v = (torch.randn(B, Lk, Hkv, D, generator=gen, device=DEV).to(BF) for _ in range(2))
+    q, g = torch.zeros(B, Lq, H, D, dtype=BF, device=DEV), torch.zeros(B, Lq, H, D, dtype=BF, device=DEV)
+    q[:, -n:], g[:, -n:] = (torch.randn(B, n, H, D, generator=gen, device=DEV).to(BF) for _ in range(2))
+    assert q.numel() > 1 << 31
+    got = run(q, k, v, g)
+    ref = reference(q[:, -n:].clone(), k, v, g[:, -n:].clone(), torch.ones(B, Lk, dtype=torch.bool, device=DEV), None, None, D ** -0.5)
+    within("o", got["o"][:, -n:].clone(), ref["o"])
+    within("dq", got["dq"][:, -n:].clone(), ref["dq"])
+    within("dk", got["dk"], ref["dk"])
+    within("dv", got["dv"], ref["dv"])
+    assert not bool(got["dq"][:, :-n].any())
+
+
+def test_norm_rope_past_32_bits():
+    """rows of more than 2^31 elements: the last ones against a call on them alone"""
+    B, L, H, D, n = 1, 131101, 128, 128, 33
+    x = torch.ones(B, L, H, D, dtype=BF, device=DEV)
+    x[:, -n:] = torch.randn(B, n, H, D, device=DEV).to(BF)
+    g = torch.zeros_like(x)
+    g[:, -n:] = torch.randn(B, n, H, D, device=DEV).to(BF)
+    x.requires_grad_(True)
+    w = (1 + 0.1 * torch.randn(D, device=DEV)).requires_grad_(True)
+    y, _ = S.qk_norm_rope(x, None, w)
+    dx, dw = torch.autograd.grad(y, [x, w], g)
+    x2 = x.detach()[:, -n:].clone().requires_grad_(True)
+    y2, _ = S.qk_norm_rope(x2, None, w, q_positions=torch.arange(L - n, L, device=DEV))
+    dx2, dw2 = torch.autograd.grad(y2, [x2, w], g[:, -n:].clone())
+    assert torch.equal(y[:, -n:], y2) and torch.equal(dx[:, -n:], dx2) and not bool(dx[:, :-n].any())
+    # the same products in sums of another order: each within the bound of its own
+    bound = 2 * 2.0 ** -24 * (64 + n * H / 256 + 256) * (g[:, -n:].double().abs().sum((0, 1, 2)) * 8)
+    assert ((dw.double() - dw2.double()).abs() <= bound).all()
