@@ -1038,10 +1038,11 @@ def test_attention_keys_of_infinite_logits(D, rel):
 
 @pytest.mark.parametrize("D", [32, 40, 96, 128])
 @pytest.mark.parametrize("rel", [False, True])
-def test_attention_masked_places_may_hold_anything_at_every_size(D, rel):
+@pytest.mark.parametrize("dt", [BF, HF])
+def test_attention_masked_places_may_hold_anything_at_every_size(D, rel, dt):
     """as above, at head sizes whose kernels differ, also where the bias' gradient sums over columns"""
     B, Lq, Lk, H, Hkv = 3, 70, 300, 4, 2
-    q, k, v, g = make(B, Lq, Lk, H, Hkv, D, BF, seed=16)
+    q, k, v, g = make(B, Lq, Lk, H, Hkv, D, dt, seed=16)
     live, kw = make_mask("both", B, Lk)
     live[1] = False
     kw["key_mask"] = live.clone()
